@@ -134,7 +134,7 @@ def _power(amax, most):
     """The smallest power of two whose `most`-fold holds amax (2^-126 at least)."""
     m, e = torch.frexp(amax)
     top = math.frexp(most)
-    e = e - top[1] + (m > top[0]).int()
+    e = torch.where(amax > 0, e - top[1] + (m > top[0]).int(), -126)
     return torch.ldexp(torch.ones_like(amax), e.clamp(min=-126))
 
 
