@@ -39,6 +39,16 @@ int dx_decode_attention(void*, float*, float*, const void*, int64_t, const void*
 int dx_prefill_attention(void*, const void*, int64_t, const void*, const void*, const int*, int, const int*,
                          const int*, const int*, int, int, int, int, int, float, int, int, hipStream_t);
 int dx_prefill_tile_tokens(int, int, int);
+int dx_block_append(const void*, const void*, const void*, int64_t, void*, int64_t, const void*, int, const float*, const float*,
+                    const int64_t*, void*, void*, float*, float*, int, int, int, int, int, int, int, int, hipStream_t);
+int dx_block_dequant(const void*, const void*, const float*, const float*, void*, void*, const int*, int, const int*, const int*, int,
+                     int, int, int, int, int, int, int, hipStream_t);
+int dx_block_decode(void*, float*, float*, const void*, int64_t, const void*, const void*, const float*, const float*, const int*, int,
+                    int, const int*, int, int, int, int, int, int, int, float, int, hipStream_t);
+int dx_block_prefill(void*, float*, float*, const void*, int64_t, const void*, const void*, const float*, const float*, const int*, int,
+                     int, const int*, const int*, const int*, int, const int*, int, int, int, int, int, int, int, float, int, int,
+                     hipStream_t);
+int dx_w4_gemm(void*, int64_t, const void*, int64_t, const void*, const void*, const void*, int, int, int, int, hipStream_t);
 int dx_rmsnorm_quant(void*, float*, const void*, void*, const void*, int, int, int64_t, int64_t, float, hipStream_t);
 int dx_decode_advance(void*, void*, void*, void*, void*, const void*, const void*, void*, void*, const int*, int, int,
                       int, int, int, hipStream_t);
@@ -130,6 +140,35 @@ PYBIND11_MODULE(_C_kernels, m) {
           "prefill_attention");
   });
   m.def("prefill_tile_tokens", &dx_prefill_tile_tokens);
+  m.def("block_append", [](u q, u k, u v, int64_t stride, u qo, int64_t qos, u pos, int pos_i64, u cs, u rs, u slots, u kc, u vc, u ks,
+                           u vs, int tokens, int hq, int hkv, int hd, int bs, int nb, int rotate_q, int code, u st) {
+    check(dx_block_append(P(q), P(k), P(v), stride, P(qo), qos, P(pos), pos_i64, (const float*)cs, (const float*)rs,
+                          (const int64_t*)slots, P(kc), P(vc), (float*)ks, (float*)vs, tokens, hq, hkv, hd, bs, nb, rotate_q, code, S(st)),
+          "block_append");
+  });
+  m.def("block_dequant", [](u kc, u vc, u ks, u vs, u ko, u vo, u bt, int bts, u ctx, u dst, int n, int cols, int nb, int ndst, int hkv,
+                            int bs, int hd, int code, u st) {
+    check(dx_block_dequant(P(kc), P(vc), (const float*)ks, (const float*)vs, P(ko), P(vo), (const int*)bt, bts, (const int*)ctx,
+                           (const int*)dst, n, cols, nb, ndst, hkv, bs, hd, code, S(st)),
+          "block_dequant");
+  });
+  m.def("block_decode", [](u out, u to, u tml, u q, int64_t qs, u kc, u vc, u ks, u vs, u bt, int bts, int btc, u ctx, int batch, int hq,
+                           int hkv, int hd, int bs, int nb, int parts, float scale, int code, u st) {
+    check(dx_block_decode(P(out), (float*)to, (float*)tml, P(q), qs, P(kc), P(vc), (const float*)ks, (const float*)vs, (const int*)bt, bts,
+                          btc, (const int*)ctx, batch, hq, hkv, hd, bs, nb, parts, scale, code, S(st)),
+          "block_decode");
+  });
+  m.def("block_prefill", [](u out, u wo, u wml, u q, int64_t qs, u kc, u vc, u ks, u vs, u bt, int bts, int btc, u cu, u ctx, u work,
+                            int n_work, u joins, int n_joins, int waves, int hq, int hkv, int hd, int bs, int nb, float scale, int causal,
+                            int code, u st) {
+    check(dx_block_prefill(P(out), (float*)wo, (float*)wml, P(q), qs, P(kc), P(vc), (const float*)ks, (const float*)vs, (const int*)bt, bts,
+                           btc, (const int*)cu, (const int*)ctx, (const int*)work, n_work, (const int*)joins, n_joins, waves, hq, hkv, hd,
+                           bs, nb, scale, causal, code, S(st)),
+          "block_prefill");
+  });
+  m.def("w4_gemm", [](u y, int64_t ldy, u x, int64_t ldx, u w, u s, u z, int M, int N, int K, int group, u st) {
+    check(dx_w4_gemm(P(y), ldy, P(x), ldx, P(w), P(s), P(z), M, N, K, group, S(st)), "w4_gemm");
+  });
   m.def("gemm256", [](u y, int64_t ldy, u x, int64_t ldx, u w, int M, int N, int K, int epi, int gm, u st, u rs) {
     check(dx_gemm256(P(y), ldy, P(x), ldx, P(w), M, N, K, epi, gm, S(st), (const float*)rs), "gemm256");
   });

@@ -17,7 +17,10 @@ from typing import NamedTuple
 import torch
 
 from .. import _native
+from . import block8
 from . import reference as ref
+from .block8 import PrefillPlan, prefill_plan
+from .w4 import W4Weight, w4_linear, w4_pack, w4_quant, w4_unpack
 
 __all__ = [
     "rmsnorm",
@@ -31,6 +34,13 @@ __all__ = [
     "decode_attention",
     "prefill_attention",
     "prefill_work_list",
+    "PrefillPlan",
+    "prefill_plan",
+    "W4Weight",
+    "w4_pack",
+    "w4_quant",
+    "w4_unpack",
+    "w4_linear",
     "fp8_scratch_plan",
     "sample",
     "apply_penalties",
@@ -153,7 +163,24 @@ def rope_cache(qkv, positions, cos_sin, slot_mapping, k_cache, v_cache, n_q, n_k
     whole row (rotated Q / K, V) into `out` [T, row] bf16, which it returns.
     row_scale [T] fp32: a deferred RMSNorm of the projection's input rows
     (`row_rrms`; the norm weight folded into the weights): Q, K, V are scaled
-    by it first (Q in the row, K / V in the cache)."""
+    by it first (Q in the row, K / V in the cache).
+
+    kv_scales tensors [num_blocks, Hkv] fp32: the cache holds int8 or e4m3fn
+    codes with a scale for each block and head, which this call makes
+    (block8.append says how).  Then `out` [T, n_q * head_dim] takes the
+    rotated Q and is returned; without it Q is rotated in place and qkv
+    returned.  K and V stay in qkv as they were."""
+    if block8.blocked(kv_scales):
+        if isinstance(qkv, SplitK):
+            qkv = splitk_reduce(qkv)
+        q_end, k_end = n_q * head_dim, (n_q + n_kv) * head_dim
+        if qkv.dim() != 2 or qkv.shape[1] != k_end + n_kv * head_dim or k_cache.shape[2] != block_size:
+            raise ValueError(f"rope_cache: qkv {tuple(qkv.shape)} for {n_q} + 2 x {n_kv} heads of {head_dim}, blocks of {block_size}")
+        T, rows = qkv.shape[0], qkv.stride(0)
+        heads = lambda lo, n: qkv.as_strided((T, n, head_dim), (rows, head_dim, qkv.stride(1)), qkv.storage_offset() + lo)  # noqa: E731
+        block8.append(heads(0, n_q), heads(q_end, n_kv), heads(k_end, n_kv), positions, cos_sin, slot_mapping, k_cache, v_cache, kv_scales,
+                      rotate_q, None if out is None else out.view(T, n_q, head_dim), row_scale)
+        return qkv if out is None else out
     if row_scale is not None:
         assert not isinstance(qkv, SplitK), "row_scale needs a finished projection row"
         assert row_scale.dtype == torch.float32 and row_scale.shape == (qkv.shape[0],)
@@ -201,7 +228,12 @@ def row_rrms(x: torch.Tensor, eps: float, out: torch.Tensor | None = None) -> to
 
 
 def kv_write(k, v, slot_mapping, k_cache, v_cache, block_size, kv_scales=(1.0, 1.0)):
-    """k, v: [T, Hkv, D] views with equal token stride."""
+    """k, v: [T, Hkv, D] views with equal token stride.  kv_scales tensors: the append to a block-scaled cache (block8.append)."""
+    if block8.blocked(kv_scales):
+        if k_cache.shape[2] != block_size:
+            raise ValueError(f"kv_write: blocks of {k_cache.shape[2]}, not {block_size}")
+        block8.append(None, k, v, None, None, slot_mapping, k_cache, v_cache, kv_scales)
+        return
     if not k.is_cuda or _kv_fp8(k_cache):  # fp8 caches: the torch path (receive-path tests only)
         return ref.write_kv(k, v, slot_mapping, k_cache, v_cache, block_size, kv_scales)
     assert k.stride(0) == v.stride(0)
@@ -581,13 +613,18 @@ def decode_attention(q, k_cache, v_cache, block_tables, ctx_lens, scale, out, n_
     """q: [B, Hq, D] (token stride q.stride(0)); out: [B, Hq, D] contiguous.
     n_parts: balanced partitions per sequence (decode_num_parts); workspace
     [B, Hq, n_parts, D] / [B, Hq, n_parts, 2] f32 when n_parts > 1.  An fp8
-    cache is dequantized on load (K scale folded into the softmax scale)."""
+    cache is dequantized on load (K scale folded into the softmax scale).
+    kv_scales tensors: a block-scaled cache (block8); n_parts may be None then
+    (as many as the table's width makes worth it) and workspace is taken from
+    torch's allocator where None."""
     if not q.is_cuda:
         B = q.shape[0]
         cu = torch.arange(B + 1, dtype=torch.int32)
         out.copy_(ref.paged_attention(q, k_cache, v_cache, block_tables, cu, ctx_lens, scale, k_cache.shape[2],
                                       kv_scales))
         return out
+    if block8.blocked(kv_scales):
+        return block8.decode(q, k_cache, v_cache, block_tables, ctx_lens, scale, out, n_parts, workspace, kv_scales)
     B, Hq, D = q.shape
     Hkv, BS = k_cache.shape[1], k_cache.shape[2]
     assert q.stride(1) == D and q.stride(2) == 1 and out.is_contiguous()
@@ -673,7 +710,8 @@ def kv_dequant_scratch(k_cache, v_cache, block_tables, ctx_lens, kv_scales=(1.0,
     :func:`fp8_scratch_plan` (the model runner's packed, capped layout:
     sum of ceil(ctx / block_size) blocks -- never
     nseq x padded max_blocks); without it (direct calls in tests) the
-    dense table i * max_blocks + j."""
+    dense table i * max_blocks + j.  kv_scales tensors: a block-scaled cache
+    (block8)."""
     nseq, maxb = block_tables.shape
     _, H, BS, D = k_cache.shape
     n = scratch[1] if scratch is not None else nseq * maxb
@@ -689,6 +727,9 @@ def kv_dequant_scratch(k_cache, v_cache, block_tables, ctx_lens, kv_scales=(1.0,
     table = scratch[0] if scratch is not None else ws[2][:n].view(nseq, maxb)
     assert block_tables.dtype == torch.int32 and ctx_lens.dtype == torch.int32 and table.dtype == torch.int32
     assert table.shape == (nseq, maxb) and table.is_contiguous()
+    if block8.blocked(kv_scales):
+        block8.dequant(k_cache, v_cache, kv_scales, block_tables, ctx_lens, ks, vs, table)
+        return ks, vs, table
     _k().kv_dequant(k_cache.data_ptr(), v_cache.data_ptr(), ks.data_ptr(), vs.data_ptr(), block_tables.data_ptr(),
                     block_tables.stride(0), ctx_lens.data_ptr(), table.data_ptr(), nseq, maxb, H, BS, D,
                     float(kv_scales[0]), float(kv_scales[1]), _stream())
@@ -702,12 +743,15 @@ def prefill_attention(q, k_cache, v_cache, block_tables, cu_seqlens_q, ctx_lens,
 
     `work` is the int32 device tensor from :func:`prefill_work_list`.  An fp8
     cache goes through :func:`kv_dequant_scratch` first (`scratch`: its packed
-    table).
+    table).  kv_scales tensors: a block-scaled cache (block8), read as it is;
+    `work` is a :func:`prefill_plan` then.
     """
     if not q.is_cuda:
         out.copy_(ref.paged_attention(q, k_cache, v_cache, block_tables, cu_seqlens_q, ctx_lens, scale, k_cache.shape[2],
                                       kv_scales, causal=causal))
         return out
+    if block8.blocked(kv_scales):
+        return block8.prefill(q, k_cache, v_cache, block_tables, cu_seqlens_q, ctx_lens, scale, out, work, kv_scales, causal)
     if _kv_fp8(k_cache):
         k_cache, v_cache, block_tables = kv_dequant_scratch(k_cache, v_cache, block_tables, ctx_lens, kv_scales,
                                                             scratch)

@@ -1,0 +1,283 @@
+"""The paged KV cache in 8 bits with a scale for each block and key/value head: its writer and its readers.
+
+codes [num_blocks, Hkv, BS, 128] int8 or float8_e4m3fn, scales [num_blocks, Hkv] float32, value = code * scale, for K and V each.
+The engine ops of the package take such a cache where their ``kv_scales`` are tensors: ``rope_cache`` and ``kv_write`` append to it,
+``decode_attention`` and ``prefill_attention`` read it, ``kv_dequant_scratch`` hands its blocks back as bf16.  GPU tensors run
+csrc/kernels/block_cache.hip, block_decode.hip and block_prefill.hip, CPU tensors the PyTorch forms of :mod:`.reference`.
+
+Scales are made by the append, as powers of two, so that nothing has to be calibrated: a block's grows when a token needs it,
+and the block's codes move with it (see :func:`append`).  A cache needs no clearing: a block's first token (offset 0) starts its
+scale anew.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from .. import _native
+from . import reference as ref
+
+HEAD_DIM = 128
+CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
+MAX_BLOCK = 128  # tokens of a block
+MAX_GROUP = 16  # query heads per key/value head, decode
+
+
+def blocked(kv_scales) -> bool:
+    """Whether kv_scales are those of a cache with a scale per block and head (tensors)."""
+    return isinstance(kv_scales[0], torch.Tensor)
+
+
+def alloc(num_blocks: int, n_kv: int, block_size: int, dtype=torch.int8, device="cuda"):
+    """An empty cache: (k codes, v codes, (k scales, v scales))."""
+    if dtype not in CODES:
+        raise TypeError(f"block-scaled cache: int8 or float8_e4m3fn codes, got {dtype}")
+    shape = (num_blocks, n_kv, block_size, HEAD_DIM)
+    k, v = (torch.zeros(shape, dtype=torch.uint8, device=device).view(dtype) for _ in range(2))
+    return k, v, tuple(torch.zeros((num_blocks, n_kv), dtype=torch.float32, device=device) for _ in range(2))
+
+
+def _stream(t: torch.Tensor) -> int:
+    dev = torch._C._cuda_getDevice()
+    if t.device.index != dev:
+        raise ValueError(f"block-scaled cache: tensors on {t.device}, current device is cuda:{dev}")
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _check_cache(k, v, kv_scales):
+    ks, vs = kv_scales
+    if k.dtype not in CODES or v.dtype != k.dtype:
+        raise TypeError(f"block-scaled cache: int8 or float8_e4m3fn codes, got {k.dtype} and {v.dtype}")
+    if ks.dtype != torch.float32 or vs.dtype != torch.float32:
+        raise TypeError("block-scaled cache: scales are float32")
+    nb, hkv, bs, d = k.shape
+    if v.shape != k.shape or ks.shape != (nb, hkv) or vs.shape != (nb, hkv):
+        raise ValueError(f"block-scaled cache: codes {tuple(k.shape)} {tuple(v.shape)}, scales {tuple(ks.shape)} {tuple(vs.shape)}")
+    if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
+        raise ValueError("block-scaled cache: codes and scales are contiguous")
+    if d != HEAD_DIM or bs < 16 or bs > MAX_BLOCK or bs & (bs - 1):
+        raise ValueError(f"block-scaled cache: heads of {HEAD_DIM}, blocks of 16, 32, 64 or 128 tokens; got {d} and {bs}")
+    if k.data_ptr() % 16 or v.data_ptr() % 16:
+        raise ValueError("block-scaled cache: codes are 16-byte aligned")
+    if not k.device == v.device == ks.device == vs.device:
+        raise ValueError("block-scaled cache: codes and scales on one device")
+
+
+def _check_on(device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name}: on {t.device}, the cache is on {device}")
+
+
+def append(q, k, v, positions, cos_sin, slot_mapping, k_cache, v_cache, kv_scales, rotate_q=True, q_out=None, row_scale=None):
+    """Rotate, quantise and append.  q [T, Hq, 128] (or None), k, v [T, Hkv, 128] bf16 views whose tokens lie equally far apart;
+    cos_sin None: as they come.  q_out [T, Hq, 128] takes the rotated q (it may be q).
+
+    slot_mapping [T] int64: block * BS + offset, negative (or past the cache) for rows that have no place.  Tokens that go into one
+    block lie behind one another, at offsets that rise by one; what the block holds in front of them belongs to the sequence, what
+    it holds behind them does not.  Each block and head, K and V each, with M = 127 (int8) or 448 (e4m3):
+
+      need = the smallest power of two with max |finite new values| <= M need;  scale = max(old scale, need)  (offset 0: need)
+      new codes = round_half_even(x / scale), +-M where x is larger or infinite; a NaN is 0 in int8, NaN in e4m3
+      if the scale grew: codes in front become round_half_even(code old / scale)
+
+    Two runs of tokens into one block in one call are not ordered; rows that no token went into keep their codes."""
+    if not k.is_cuda:
+        return ref.block_append(q, k, v, positions, cos_sin, slot_mapping, k_cache, v_cache, kv_scales, rotate_q, q_out, row_scale)
+    nb, hkv, bs, d = k_cache.shape
+    T = k.shape[0]
+    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or (q is not None and q.dtype != torch.bfloat16):
+        raise TypeError("append: q, k, v are bfloat16")
+    if k.shape != (T, hkv, d) or v.shape != k.shape or (q is not None and (q.dim() != 3 or q.shape[0] != T or q.shape[2] != d)):
+        raise ValueError(f"append: k {tuple(k.shape)}, v {tuple(v.shape)}, cache {tuple(k_cache.shape)}")
+    stride = k.stride(0)
+    for t in (q, k, v):
+        if t is not None and T > 0 and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != d) or (T > 1 and t.stride(0) != stride) or t.data_ptr() % 16):
+            raise ValueError("append: heads of a token behind one another, tokens equally far apart, 16-byte aligned")
+    if T > 1 and stride % 8:
+        raise ValueError("append: tokens lie a multiple of 8 elements apart")
+    if cos_sin is not None:
+        if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or cos_sin.shape[1] != d or not cos_sin.is_contiguous() or cos_sin.data_ptr() % 16:
+            raise ValueError("append: cos_sin is [positions, 128] float32, contiguous")
+        if positions.dtype not in (torch.int64, torch.int32) or positions.shape != (T,) or not positions.is_contiguous():
+            raise ValueError("append: positions are [T] int64 or int32, contiguous")
+    if slot_mapping is not None and (slot_mapping.dtype != torch.int64 or slot_mapping.shape != (T,) or not slot_mapping.is_contiguous()):
+        raise ValueError("append: slot_mapping is [T] int64, contiguous")
+    if row_scale is not None and (row_scale.dtype != torch.float32 or row_scale.shape != (T,) or not row_scale.is_contiguous()):
+        raise ValueError("append: row_scale is [T] float32, contiguous")
+    _check_cache(k_cache, v_cache, kv_scales)
+    _check_on(k_cache.device, q=q, k=k, v=v, positions=positions if cos_sin is not None else None, cos_sin=cos_sin, slot_mapping=slot_mapping,
+              row_scale=row_scale, q_out=q_out)
+    nq = 0
+    if q is not None:
+        q_out = q if q_out is None else q_out
+        if q_out.shape != q.shape or q_out.dtype != torch.bfloat16 or (T > 0 and (
+                q_out.stride(2) != 1 or (q.shape[1] > 1 and q_out.stride(1) != d) or (T > 1 and q_out.stride(0) % 8) or q_out.data_ptr() % 16)):
+            raise ValueError("append: q_out is shaped as q, heads of a token behind one another, 16-byte aligned")
+        nq = q.shape[1]
+    _native.kernels().block_append(
+        0 if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), stride if T > 1 else 0, 0 if q is None else q_out.data_ptr(),
+        q_out.stride(0) if q is not None and T > 1 else 0, positions.data_ptr() if cos_sin is not None else 0,
+        int(cos_sin is not None and positions.dtype == torch.int64), 0 if cos_sin is None else cos_sin.data_ptr(),
+        0 if row_scale is None else row_scale.data_ptr(), 0 if slot_mapping is None else slot_mapping.data_ptr(), k_cache.data_ptr(),
+        v_cache.data_ptr(), kv_scales[0].data_ptr(), kv_scales[1].data_ptr(), T, nq, hkv, d, bs, nb, int(rotate_q), CODES[k_cache.dtype], _stream(k))
+    return q_out
+
+
+def dequant(k_cache, v_cache, kv_scales, block_tables, ctx_lens, k_out, v_out, table):
+    """The blocks of `block_tables` [n, columns] that hold ctx_lens [n] tokens, as bf16, into blocks `table` [n, columns] of k_out and v_out."""
+    _check_cache(k_cache, v_cache, kv_scales)
+    nb, hkv, bs, d = k_cache.shape
+    n, cols = block_tables.shape
+    if block_tables.dtype != torch.int32 or ctx_lens.dtype != torch.int32 or table.dtype != torch.int32:
+        raise TypeError("kv_dequant_scratch: tables and lengths are int32")
+    if block_tables.stride(1) != 1 and cols > 1 or ctx_lens.shape != (n,) or table.shape != (n, cols) or not (table.is_contiguous() and ctx_lens.is_contiguous()):
+        raise ValueError("kv_dequant_scratch: block_tables [n, columns], ctx_lens [n], table [n, columns]")
+    _check_on(k_cache.device, block_tables=block_tables, ctx_lens=ctx_lens, table=table)
+    _native.kernels().block_dequant(k_cache.data_ptr(), v_cache.data_ptr(), kv_scales[0].data_ptr(), kv_scales[1].data_ptr(), k_out.data_ptr(),
+                                    v_out.data_ptr(), block_tables.data_ptr(), block_tables.stride(0), ctx_lens.data_ptr(), table.data_ptr(), n, cols,
+                                    nb, k_out.shape[0], hkv, bs, d, CODES[k_cache.dtype], _stream(k_cache))
+
+
+def _check_reader(q, out, k_cache, v_cache, kv_scales, block_tables, ctx_lens, n):
+    _check_cache(k_cache, v_cache, kv_scales)
+    T, hq, d = q.shape
+    hkv = k_cache.shape[1]
+    if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
+        raise TypeError("attention over a block-scaled cache: q and out are bfloat16")
+    if d != HEAD_DIM or hq % hkv or out.shape != q.shape or not out.is_contiguous():
+        raise ValueError(f"attention over a block-scaled cache: q {tuple(q.shape)}, out {tuple(out.shape)}, {hkv} key/value heads")
+    if T and (q.stride(2) != 1 or (hq > 1 and q.stride(1) != d) or (T > 1 and q.stride(0) % 8) or q.data_ptr() % 16 or out.data_ptr() % 16):
+        raise ValueError("attention over a block-scaled cache: q's heads behind one another, its rows and out 16-byte aligned")
+    if block_tables.dtype != torch.int32 or ctx_lens.dtype != torch.int32:
+        raise TypeError("attention over a block-scaled cache: tables and lengths are int32")
+    if (block_tables.dim() != 2 or block_tables.shape[0] != n or block_tables.shape[1] < 1 or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1)
+            or ctx_lens.shape != (n,) or not ctx_lens.is_contiguous()):
+        raise ValueError(f"attention over a block-scaled cache: block_tables {tuple(block_tables.shape)}, ctx_lens {tuple(ctx_lens.shape)}, {n} sequences")
+    _check_on(k_cache.device, q=q, out=out, block_tables=block_tables, ctx_lens=ctx_lens)
+
+
+def decode(q, k_cache, v_cache, block_tables, ctx_lens, scale, out, n_parts, workspace, kv_scales):
+    B, hq, d = q.shape
+    _check_reader(q, out, k_cache, v_cache, kv_scales, block_tables, ctx_lens, B)
+    nb, hkv, bs, _ = k_cache.shape
+    if hq // hkv > MAX_GROUP:
+        raise ValueError(f"decode_attention: at most {MAX_GROUP} query heads per key/value head, got {hq // hkv}")
+    if n_parts is None:
+        n_parts = decode_parts(B, hkv, block_tables.shape[1] * bs)
+    if n_parts < 1:
+        raise ValueError(f"decode_attention: {n_parts} parts")
+    t0 = t1 = 0
+    if n_parts > 1 and B:
+        if workspace is None:
+            ws = torch.empty(B * hq * n_parts * (d + 2), dtype=torch.float32, device=q.device)
+            t0 = ws.data_ptr()
+            t1 = t0 + 4 * B * hq * n_parts * d
+        else:
+            o, ml = workspace
+            if o.dtype != torch.float32 or ml.dtype != torch.float32 or not (o.is_contiguous() and ml.is_contiguous()):
+                raise TypeError("decode_attention: the workspace is float32, contiguous")
+            if o.shape[0] < B or o.shape[1:] != (hq, n_parts, d) or ml.shape[0] < B or ml.shape[1:] != (hq, n_parts, 2):
+                raise ValueError(f"decode_attention: workspace {tuple(o.shape)} {tuple(ml.shape)} for {(B, hq, n_parts, d)}")
+            _check_on(q.device, workspace=o, sums=ml)
+            t0, t1 = o.data_ptr(), ml.data_ptr()
+    _native.kernels().block_decode(out.data_ptr(), t0, t1, q.data_ptr(), q.stride(0) if B > 1 else 0, k_cache.data_ptr(), v_cache.data_ptr(),
+                                   kv_scales[0].data_ptr(), kv_scales[1].data_ptr(), block_tables.data_ptr(), block_tables.stride(0),
+                                   block_tables.shape[1], ctx_lens.data_ptr(), B, hq, hkv, d, bs, nb, int(n_parts), float(scale),
+                                   CODES[k_cache.dtype], _stream(q))
+    return out
+
+
+DECODE_WGS, DECODE_PART = 512, 256
+
+
+def decode_parts(batch: int, n_kv: int, max_ctx: int) -> int:
+    """Parts of a context for a decode launch over the 8-bit cache."""
+    want = -(-DECODE_WGS // max(1, batch * n_kv))
+    return max(1, min(want, -(-max(1, max_ctx) // DECODE_PART)))
+
+
+class PrefillPlan(NamedTuple):
+    """What a step's prompt rows are cut into, for all of its layers (:func:`prefill_plan`)."""
+    work: torch.Tensor  # int32: n_work items of 6, then n_joins of 4
+    n_work: int
+    n_joins: int
+    places: int  # tiles of sums in the workspace
+    waves: int
+    rows: int
+    sequences: int
+    n_q: int
+    n_kv: int
+    causal: bool
+
+
+PREFILL_WGS, PREFILL_TILES = 512, 4
+
+
+def prefill_plan(q_lens: list[int], ctx_lens: list[int], n_q: int, n_kv: int, device="cuda", causal: bool = True) -> PrefillPlan:
+    """Cuts prompt chunks (q_lens new tokens each, the last of ctx_lens tokens) into work items for ``prefill_attention`` over a
+    block-scaled cache: tiles of query rows, heaviest first, and where those are too few for the chip, parts of their keys."""
+    if len(q_lens) != len(ctx_lens) or any(q < 0 or c < q for q, c in zip(q_lens, ctx_lens)):
+        raise ValueError(f"prefill_plan: {list(q_lens)} new tokens of {list(ctx_lens)}")
+    if n_kv < 1 or n_q % n_kv:
+        raise ValueError(f"prefill_plan: {n_q} query heads, {n_kv} key/value heads")
+    g = n_q // n_kv
+    waves = 8 if n_kv * sum(-(-q * g // 256) for q in q_lens) >= PREFILL_WGS else 4
+    tile = 32 * waves
+    items = []  # key tiles, sequence, first row
+    for s, (ql, cl) in enumerate(zip(q_lens, ctx_lens)):
+        for r0 in range(0, ql * g, tile):
+            seen = cl - ql + (min(r0 + tile, ql * g) - 1) // g + 1 if causal else cl
+            items.append((-(-seen // 64), s, r0))
+    total = sum(i[0] for i in items)
+    per = max(PREFILL_TILES, -(-total * n_kv // PREFILL_WGS)) if len(items) * n_kv < PREFILL_WGS else 1 << 30
+    work, joins, places = [], [], 0
+    for n, s, r0 in items:
+        parts = -(-n // per) if 2 * n > 3 * per else 1
+        each = -(-n // parts)
+        parts = -(-n // each)
+        if parts == 1:
+            work.append((n, [s, r0, 0, 64 * n, -1, 0]))
+            continue
+        joins += [s, r0, places, parts]
+        for p in range(parts):
+            end = min((p + 1) * each, n)
+            work.append((end - p * each, [s, r0, 64 * p * each, 64 * end, places + p, 0]))
+        places += parts
+    if len(work) > 65535:
+        raise ValueError(f"prefill_plan: {len(work)} work items, at most 65535")
+    work.sort(key=lambda w: -w[0])
+    flat = [x for _, w in work for x in w] + joins
+    return PrefillPlan(torch.tensor(flat or [0], dtype=torch.int32).to(device), len(work), len(joins) // 4, places, waves, sum(q_lens), len(q_lens), n_q, n_kv,
+                       causal)
+
+
+def prefill(q, k_cache, v_cache, block_tables, cu_seqlens_q, ctx_lens, scale, out, plan, kv_scales, causal):
+    if plan is None:
+        cu = cu_seqlens_q.tolist()
+        plan = prefill_plan([b - a for a, b in zip(cu, cu[1:])], ctx_lens.tolist(), q.shape[1], k_cache.shape[1], q.device, causal)
+    if not isinstance(plan, PrefillPlan):
+        raise TypeError("prefill_attention: over a block-scaled cache `work` is a plan of prefill_plan")
+    T, hq, d = q.shape
+    nb, hkv, bs, _ = k_cache.shape
+    n = cu_seqlens_q.shape[0] - 1
+    _check_reader(q, out, k_cache, v_cache, kv_scales, block_tables, ctx_lens, n)
+    if cu_seqlens_q.dtype != torch.int32 or not cu_seqlens_q.is_contiguous():
+        raise TypeError("prefill_attention: cu_seqlens_q is int32, contiguous")
+    if (plan.rows, plan.sequences, plan.n_q, plan.n_kv, plan.causal) != (T, n, hq, hkv, causal):
+        raise ValueError(f"prefill_attention: a plan of {plan.rows} rows, {plan.sequences} sequences, {plan.n_q} / {plan.n_kv} heads, causal "
+                         f"{plan.causal} for {T}, {n}, {hq} / {hkv}, {causal}")
+    _check_on(q.device, cu_seqlens_q=cu_seqlens_q, work=plan.work)
+    o = ml = 0
+    if plan.places:
+        sums = plan.places * hkv * 32 * plan.waves
+        ws = torch.empty(sums * (d + 2), dtype=torch.float32, device=q.device)
+        o = ws.data_ptr()
+        ml = o + 4 * sums * d
+    work = plan.work.data_ptr()
+    _native.kernels().block_prefill(out.data_ptr(), o, ml, q.data_ptr(), q.stride(0) if T > 1 else 0, k_cache.data_ptr(), v_cache.data_ptr(),
+                                    kv_scales[0].data_ptr(), kv_scales[1].data_ptr(), block_tables.data_ptr(), block_tables.stride(0),
+                                    block_tables.shape[1], cu_seqlens_q.data_ptr(), ctx_lens.data_ptr(), work, plan.n_work, work + 24 * plan.n_work,
+                                    plan.n_joins, plan.waves, hq, hkv, d, bs, nb, float(scale), int(causal), CODES[k_cache.dtype], _stream(q))
+    return out

@@ -125,6 +125,68 @@ def write_kv(k, v, slot_mapping, k_cache, v_cache, block_size, kv_scales=(1.0, 1
     v_cache[blk, :, off] = to_cache(vv, v_cache.dtype, kv_scales[1])
 
 
+# ---- the cache in 8 bits with a scale for each block and head (ops/block8.py)
+CODE_MAX = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
+
+
+def power_scale(amax: torch.Tensor, dtype) -> torch.Tensor:
+    """The smallest power of two, 2^-126 at least, whose 127-fold (448-fold) holds amax."""
+    m, e = torch.frexp(amax.float())
+    top_m, top_e = math.frexp(CODE_MAX[dtype])
+    e = torch.where(m > 0, e - top_e + (m > top_m).int(), -126)
+    return torch.ldexp(torch.ones_like(m), e.clamp(min=-126))
+
+
+def to_codes(y: torch.Tensor, dtype) -> torch.Tensor:
+    """Values over their scale as codes: half-even, saturating; int8 has no NaN (0)."""
+    most = CODE_MAX[dtype]
+    c = y.clamp(-most, most)
+    if dtype == torch.int8:
+        return torch.where(y.isnan(), torch.zeros_like(c), c).round().to(dtype)
+    return c.to(dtype)
+
+
+def block_values(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    return codes.float() * scales[..., None, None]
+
+
+def block_append(q, k, v, positions, cos_sin, slot_mapping, k_cache, v_cache, kv_scales, rotate_q=True, q_out=None, row_scale=None):
+    """The append to a block-scaled cache (ops.block8.append), run by run."""
+    rows = lambda x: x.float() if row_scale is None else x.float() * row_scale[:, None, None]  # noqa: E731
+    turn = (lambda x: apply_rope(x, positions, cos_sin)) if cos_sin is not None else (lambda x: x)
+    kf, vf = turn(rows(k)), rows(v)
+    if q is not None:
+        q_out = q if q_out is None else q_out
+        qf = rows(q)
+        q_out.copy_((turn(qf) if rotate_q else qf).to(q.dtype))
+    if slot_mapping is None:
+        return q_out
+    nb, bs, dtype = k_cache.shape[0], k_cache.shape[2], k_cache.dtype
+    slots, t = slot_mapping.tolist(), 0
+    while t < len(slots):
+        slot, n = slots[t], 1
+        if not 0 <= slot < nb * bs:
+            t += 1
+            continue
+        while t + n < len(slots) and slots[t + n] == slot + n and (slot + n) % bs:
+            n += 1
+        b, off = slot // bs, slot % bs
+        for x, codes, scales in ((kf, k_cache, kv_scales[0]), (vf, v_cache, kv_scales[1])):
+            y = x[t:t + n].transpose(0, 1)  # [Hkv, n, D]
+            a = y.abs()
+            amax = torch.where(a < float("inf"), a, torch.zeros_like(a)).amax((1, 2))
+            was = scales[b].clone()
+            old = torch.where((was > 0) & (was < float("inf")), was, torch.zeros_like(was)) if off else torch.zeros_like(was)
+            now = torch.maximum(old, power_scale(amax, dtype))
+            moved = codes[b, :, :off].float() * (old / now)[:, None, None]
+            if off:
+                codes[b, :, :off] = torch.where((now != was)[:, None, None], to_codes(moved, dtype).float(), codes[b, :, :off].float()).to(dtype)
+            codes[b, :, off:off + n] = to_codes(y / now[:, None, None], dtype)
+            scales[b] = now
+        t += n
+    return q_out
+
+
 def interleave_gate_up(w: torch.Tensor, blk: int = 32) -> torch.Tensor:
     """[gate; up] rows ([2F, K]) -> rows interleaved in blocks of `blk`:
     g[0:blk], u[0:blk], g[blk:2blk], u[blk:2blk], ... (the fused SwiGLU
@@ -157,10 +219,11 @@ def embedding(ids: torch.Tensor, table: torch.Tensor) -> torch.Tensor:
     return table[ids.long()]
 
 
-def _gather_kv(cache, block_table_row, n_tokens, block_size):
+def _gather_kv(cache, block_table_row, n_tokens, block_size, scale=1.0):
     nb = (n_tokens + block_size - 1) // block_size
     blocks = block_table_row[:nb].long()
-    kv = cache[blocks]  # [nb, Hkv, BS, D]
+    kv = cache[blocks].float()  # [nb, Hkv, BS, D]
+    kv = kv * (scale[blocks][..., None, None] if isinstance(scale, torch.Tensor) else scale)
     kv = kv.permute(0, 2, 1, 3).reshape(nb * block_size, cache.shape[1], cache.shape[3])
     return kv[:n_tokens]
 
@@ -183,8 +246,8 @@ def paged_attention(q, k_cache, v_cache, block_tables, cu_seqlens_q, ctx_lens, s
         ql = e - s
         if ql == 0:
             continue
-        k = _gather_kv(k_cache, block_tables[b], ctx, block_size).float() * kv_scales[0]  # [ctx, Hkv, D]
-        v = _gather_kv(v_cache, block_tables[b], ctx, block_size).float() * kv_scales[1]
+        k = _gather_kv(k_cache, block_tables[b], ctx, block_size, kv_scales[0])  # [ctx, Hkv, D]
+        v = _gather_kv(v_cache, block_tables[b], ctx, block_size, kv_scales[1])
         k = k.repeat_interleave(G, dim=1)
         v = v.repeat_interleave(G, dim=1)
         qq = q[s:e].float()

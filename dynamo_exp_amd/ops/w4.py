@@ -1,0 +1,112 @@
+"""Products of few rows with weights in 4 bits: codes 0..15, a bf16 scale and (perhaps) a zero point 0..15 for each group of 32, 64 or
+128 columns of a weight row,  w[n, k] = (code[n, k] - zero[n, k / group]) * scale[n, k / group]  (zero 8 where there are none).
+
+GPU tensors run csrc/kernels/w4_gemm.hip, CPU tensors PyTorch in fp32."""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from .. import _native
+
+GROUPS = (32, 64, 128)
+MAX_ROWS = 256
+
+
+class W4Weight(NamedTuple):
+    """A weight [n, k] as the kernel reads it (:func:`w4_pack`): rows in tiles of 16, columns in chunks of 128."""
+    packed: torch.Tensor  # int32 [n / 16, k / 128, 64, 4]: lane 16 q + r, word s: columns 32 s + 8 q .. of row r
+    scales: torch.Tensor  # bf16 [n / 16, k / group, 16]
+    zeros: torch.Tensor | None  # uint8, as scales: 128 + zero
+    n: int
+    k: int
+    group: int
+
+
+def _tiles(t: torch.Tensor) -> torch.Tensor:
+    """[n, g] -> [n / 16, g, 16], rows that are none 0."""
+    n, g = t.shape
+    p = torch.zeros((-(-n // 16) * 16, g), dtype=t.dtype, device=t.device)
+    p[:n] = t
+    return p.view(-1, 16, g).transpose(1, 2).contiguous()
+
+
+def w4_pack(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None, group: int) -> W4Weight:
+    """Lays a quantised weight out for :func:`w4_linear`, once: codes [n, k] uint8 in 0..15, scales [n, k / group] bf16, zeros as
+    scales in uint8 0..15 or None (8).  k is a multiple of group (32, 64 or 128)."""
+    if codes.dim() != 2 or group not in GROUPS or codes.shape[0] < 1 or codes.shape[1] < group or codes.shape[1] % group:
+        raise ValueError(f"w4_pack: codes {tuple(codes.shape)} in groups of {group} (32, 64 or 128, a divisor of the columns)")
+    n, k = codes.shape
+    if codes.dtype != torch.uint8 or scales.dtype != torch.bfloat16 or (zeros is not None and zeros.dtype != torch.uint8):
+        raise TypeError("w4_pack: codes and zeros are uint8, scales bfloat16")
+    if scales.shape != (n, k // group) or (zeros is not None and zeros.shape != scales.shape):
+        raise ValueError(f"w4_pack: scales {tuple(scales.shape)} for {(n, k // group)}")
+    if int(codes.max()) > 15 or (zeros is not None and int(zeros.max()) > 15):
+        raise ValueError("w4_pack: codes and zeros are 0..15")
+    n16, k128 = -(-n // 16), -(-k // 128)
+    c = torch.zeros((n16 * 16, k128 * 128), dtype=torch.uint8, device=codes.device)
+    c[:n, :k] = codes
+    # [tile, row, chunk, step, quarter, 8] -> [tile, chunk, quarter, row, step, 8]
+    c = c.view(n16, 16, k128, 4, 4, 8).permute(0, 2, 4, 1, 3, 5)
+    word = torch.zeros(c.shape[:-1], dtype=torch.int32, device=codes.device)
+    for j in range(8):  # column 2 i in nibble i, 2 i + 1 in nibble 4 + i
+        word |= c[..., j].to(torch.int32) << (4 * (j // 2 + 4 * (j % 2)))
+    packed = word.reshape(n16, k128, 64, 4).contiguous()
+    return W4Weight(packed, _tiles(scales), None if zeros is None else _tiles(zeros + 128), n, k, group)
+
+
+def w4_quant(w: torch.Tensor, group: int = 128, symmetric: bool = True) -> W4Weight:
+    """Quantises a weight [n, k] to the nearest codes: symmetric (zero 8, scale max |w| / 7) or over each group's range, 0 in it."""
+    if w.dim() != 2 or group not in GROUPS or w.shape[1] < group or w.shape[1] % group:
+        raise ValueError(f"w4_quant: a weight {tuple(w.shape)} in groups of {group}")
+    n, k = w.shape
+    x = w.float().reshape(n, k // group, group)
+    if symmetric:
+        s = x.abs().amax(-1) / 7
+    else:
+        lo, hi = x.amin(-1).clamp(max=0), x.amax(-1).clamp(min=0)
+        s = (hi - lo) / 15
+    s = s.to(torch.bfloat16)
+    f = torch.where(s > 0, s, 1).float()
+    z = None if symmetric else (-lo / f).round().clamp(0, 15)
+    c = (x / f[..., None]).round() + (8 if z is None else z[..., None])
+    return w4_pack(c.clamp(0, 15).to(torch.uint8).reshape(n, k), s, None if z is None else z.to(torch.uint8), group)
+
+
+def w4_unpack(weight: W4Weight) -> torch.Tensor:
+    """The weight's values [n, k] in fp32."""
+    p, n16, k128 = weight.packed, weight.packed.shape[0], weight.packed.shape[1]
+    w = p.view(n16, k128, 4, 16, 4, 1).expand(n16, k128, 4, 16, 4, 8)
+    shift = torch.tensor([4 * (j // 2 + 4 * (j % 2)) for j in range(8)], dtype=torch.int32, device=p.device)
+    c = ((w >> shift) & 15).permute(0, 3, 1, 4, 2, 5).reshape(n16 * 16, k128 * 128)[: weight.n, : weight.k].float()
+    rows = lambda t: t.transpose(1, 2).reshape(n16 * 16, -1)[: weight.n].float().repeat_interleave(weight.group, 1)  # noqa: E731
+    zeros = 8.0 if weight.zeros is None else rows(weight.zeros) - 128
+    return (c - zeros) * rows(weight.scales)
+
+
+def w4_linear(x: torch.Tensor, weight: W4Weight, out: torch.Tensor | None = None) -> torch.Tensor:
+    """y [m, n] = x [m, k] . w^T for up to 256 rows of bf16, sums in fp32."""
+    if x.dim() != 2 or x.shape[1] != weight.k:
+        raise ValueError(f"w4_linear: x {tuple(x.shape)}, weight {(weight.n, weight.k)}")
+    m = x.shape[0]
+    if not x.is_cuda:
+        y = (x.float() @ w4_unpack(weight).t()).to(x.dtype)
+        return y if out is None else out.copy_(y)
+    if x.dtype != torch.bfloat16:
+        raise TypeError(f"w4_linear: x is bfloat16, got {x.dtype}")
+    if m > MAX_ROWS:
+        raise ValueError(f"w4_linear: at most {MAX_ROWS} rows, got {m}")
+    if m and (x.stride(1) != 1 or (m > 1 and x.stride(0) % 8) or x.data_ptr() % 16):
+        raise ValueError("w4_linear: rows of x have unit stride and are 16-byte aligned")
+    dev = torch._C._cuda_getDevice()
+    if x.device.index != dev or weight.packed.device != x.device:
+        raise ValueError(f"w4_linear: x on {x.device}, the weight on {weight.packed.device}, current device cuda:{dev}")
+    if out is None:
+        out = torch.empty((m, weight.n), dtype=x.dtype, device=x.device)
+    elif out.shape != (m, weight.n) or out.dtype != x.dtype or out.device != x.device or (m and out.stride(1) != 1):
+        raise ValueError("w4_linear: bad out tensor")
+    _native.kernels().w4_gemm(out.data_ptr(), out.stride(0), x.data_ptr(), x.stride(0) if m > 1 else 0, weight.packed.data_ptr(),
+                              weight.scales.data_ptr(), 0 if weight.zeros is None else weight.zeros.data_ptr(), m, weight.n, weight.k, weight.group,
+                              torch._C._cuda_getCurrentRawStream(dev))
+    return out

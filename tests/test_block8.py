@@ -1,0 +1,662 @@
+"""The 8-bit KV cache with a scale for each block and head (ops/block8.py; csrc/kernels/block_cache.hip, block_decode.hip,
+block_prefill.hip): the append against its definition in 64 bits, both attentions against a plain softmax in 64 bits, refusals, and
+a run of all of them together as a server makes it."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from dynamo_exp_amd import ops
+from dynamo_exp_amd.ops import block8
+from dynamo_exp_amd.ops import reference as ref
+
+D = 128
+SCALE = 1 / math.sqrt(D)
+CODES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
+MOST = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
+both = pytest.mark.parametrize("codes", ["int8", "e4m3"])
+NAN, INF = float("nan"), float("inf")
+
+
+def bits(t):
+    return t.view(torch.uint8)
+
+
+def table_of(need, seed=0, extra=3):
+    """Blocks in an order of no order: [sequences, columns] int32 and how many blocks there are."""
+    order = torch.randperm(sum(need) + extra, generator=torch.Generator().manual_seed(seed)).to(torch.int32)
+    t = torch.zeros((len(need), max(need + [1])), dtype=torch.int32)
+    at = 0
+    for i, n in enumerate(need):
+        t[i, :n] = order[at:at + n]
+        at += n
+    return t, len(order)
+
+
+def slots_of(table, spans, bs):
+    """The slots of positions lo .. hi - 1 of each sequence, behind one another."""
+    out = [table[i].long()[torch.arange(lo, hi) // bs] * bs + torch.arange(lo, hi) % bs for i, (lo, hi) in enumerate(spans)]
+    return torch.cat(out)
+
+
+def random_cache(blocks, nkv, bs, dtype, seed, pow2=True):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn((blocks, nkv, bs, D), generator=g) * torch.exp(torch.randn((blocks, nkv, 1, 1), generator=g))
+    s = ref.power_scale(x.abs().amax((2, 3)), dtype) * (1.0 if pow2 else 1.37)
+    return ref.to_codes(x / s[..., None, None], dtype), s
+
+
+def on_gpu(*ts):
+    return [t.cuda() for t in ts]
+
+
+# ---------------------------------------------------------------- the definition, in 64 bits, for one sequence's rows of one head
+def check_rows(got, want, scale, dtype):
+    """New rows' values against the unrounded ones: half a step of the code.  The values themselves come from products in fp32 (three
+    roundings of 2^-24 relative to values of at most `most` steps: under 2^-13 steps)."""
+    err = (got - want).abs()
+    if dtype == torch.int8:
+        tol = scale * (0.5 + 2 ** -13)
+    else:  # normal codes 2^-4 of the value, subnormal ones half of 2^-9
+        tol = torch.maximum(want.abs() * (2 ** -4 + 2 ** -20), scale * (2 ** -10 + 2 ** -13))
+    assert bool((err <= tol).all()), float((err / tol).max())
+
+
+def rotated(x, pos, cs):
+    c, s = cs.double()[pos.long()][:, None, :64], cs.double()[pos.long()][:, None, 64:]
+    a, b = x.double()[..., :64], x.double()[..., 64:]
+    return torch.cat([a * c - b * s, b * c + a * s], -1)
+
+
+def append_case(codes, bs, spans, nq=4, nkv=2, seed=1, pad=0, device="cpu", pos32=False, grow=1.0):
+    dtype = CODES[codes]
+    table, blocks = table_of([-(-hi // bs) for _, hi in spans], seed)
+    k8, ks = random_cache(blocks, nkv, bs, dtype, seed)
+    v8, vs = random_cache(blocks, nkv, bs, dtype, seed + 1)
+    g = torch.Generator().manual_seed(seed + 2)
+    T = sum(hi - lo for lo, hi in spans)
+    qkv = (torch.randn((T + pad, (nq + 2 * nkv) * D), generator=g) * grow).bfloat16()
+    pos = torch.cat([torch.arange(lo, hi) for lo, hi in spans] + [torch.zeros(pad, dtype=torch.int64)])
+    slots = torch.cat([slots_of(table, spans, bs), torch.full((pad,), -1)])
+    cs = ref.rope_cos_sin(D, int(pos.max()) + 1, 500000.0)
+    before = [t.clone() for t in (k8, v8, ks, vs)]
+    args = [t.to(device) for t in (qkv, pos.int() if pos32 else pos, cs, slots, k8, v8)]
+    scales = (ks.to(device), vs.to(device))
+    q_out = torch.full((T + pad, nq * D), NAN, dtype=torch.bfloat16, device=device)
+    r = ops.rope_cache(*args, nq, nkv, D, bs, kv_scales=scales, out=q_out)
+    assert r is q_out and torch.equal(args[0].cpu(), qkv)
+    return dict(dtype=dtype, table=table, qkv=qkv, pos=pos, cs=cs, slots=slots, before=before, q=q_out.cpu(), k8=args[4].cpu(), v8=args[5].cpu(),
+                ks=scales[0].cpu(), vs=scales[1].cpu(), T=T, bs=bs, nq=nq, nkv=nkv, spans=spans)
+
+
+def check_append(c):
+    dtype, bs, nq, nkv, T = c["dtype"], c["bs"], c["nq"], c["nkv"], c["T"]
+    x = c["qkv"].view(-1, nq + 2 * nkv, D)
+    q64 = rotated(x[:, :nq], c["pos"], c["cs"])
+    # one rounding to bf16 and three in fp32
+    assert bool(((c["q"].view(-1, nq, D).double() - q64).abs() <= q64.abs() * 2 ** -8 + 2 ** -20).all())
+    new = {"k": rotated(x[:T, nq:nq + nkv], c["pos"][:T], c["cs"]), "v": x[:T, nq + nkv:].double()}
+    seen = set()
+    at = 0
+    for i, (lo, hi) in enumerate(c["spans"]):
+        for first in range(lo // bs * bs, hi, bs):
+            a, b = max(lo, first), min(hi, first + bs)
+            if a >= b:
+                continue
+            block = int(c["table"][i, first // bs])
+            seen.add(block)
+            for w, n_codes, n_scale, o_codes, o_scale in (("k", c["k8"], c["ks"], c["before"][0], c["before"][2]), ("v", c["v8"], c["vs"], c["before"][1], c["before"][3])):
+                rows = new[w][at + a - lo:at + b - lo].transpose(0, 1)
+                need = ref.power_scale(rows.abs().amax((1, 2)), dtype)
+                off = a - first
+                old = o_scale[block] if off else torch.zeros(nkv)
+                assert torch.equal(n_scale[block], torch.maximum(old, need))
+                s = n_scale[block].double()[:, None, None]
+                check_rows(n_codes[block].double()[:, off:off + b - a] * s, rows, s, dtype)
+                ratio = (old.double() / n_scale[block].double())[:, None, None]
+                moved = ref.to_codes((o_codes[block].double()[:, :off] * ratio).float(), dtype)
+                assert torch.equal(bits(n_codes[block][:, :off]), bits(moved))
+                assert torch.equal(bits(n_codes[block][:, off + b - a:]), bits(o_codes[block][:, off + b - a:]))  # rows behind
+        at += hi - lo
+    others = [b for b in range(c["k8"].shape[0]) if b not in seen]
+    for n, o in zip((c["k8"], c["v8"], c["ks"], c["vs"]), c["before"]):
+        assert torch.equal(n[others].view(torch.uint8), o[others].view(torch.uint8))
+
+
+SPANS = [
+    [(0, 1)],
+    [(5, 6), (63, 64), (64, 65), (127, 128), (16, 17)],  # one token each, at blocks' edges
+    [(0, 300), (17, 130), (250, 251), (40, 48)],  # ragged chunks, some behind cached tokens
+    [(1, 260), (511, 530)],  # more rows than a decode step has
+]
+
+
+@both
+@pytest.mark.parametrize("bs", [16, 64, 128])
+@pytest.mark.parametrize("spans", SPANS)
+def test_append_cpu(codes, bs, spans):
+    check_append(append_case(codes, bs, spans, pad=2, seed=len(spans) + bs))
+
+
+@pytest.mark.gpu
+@both
+@pytest.mark.parametrize("bs", [16, 32, 64, 128])
+@pytest.mark.parametrize("spans", SPANS)
+def test_append(codes, bs, spans):
+    check_append(append_case(codes, bs, spans, pad=2, seed=len(spans) + bs, device="cuda"))
+
+
+@pytest.mark.gpu
+@both
+@pytest.mark.parametrize("nq,nkv", [(32, 8), (14, 2), (1, 1), (5, 5)])
+@pytest.mark.parametrize("grow", [2.0 ** -40, 9.0])
+def test_append_heads_and_growth(codes, nq, nkv, grow):
+    """Tokens far smaller than their block's (its scale stays) and larger (its codes move)."""
+    check_append(append_case(codes, 32, [(30, 37), (9, 10), (64, 200)], nq, nkv, device="cuda", pos32=True, grow=grow))
+
+
+@pytest.mark.gpu
+@both
+def test_append_in_place_and_twice(codes):
+    """Without `out` Q is rotated where it lies; the same tokens appended again change nothing."""
+    c = append_case(codes, 64, [(70, 90), (3, 4)], device="cuda")
+    qkv, k8, v8 = c["qkv"].cuda(), c["k8"].cuda(), c["v8"].cuda()
+    scales = (c["ks"].cuda(), c["vs"].cuda())
+    ops.rope_cache(qkv, c["pos"].cuda(), c["cs"].cuda(), c["slots"].cuda(), k8, v8, 4, 2, D, 64, kv_scales=scales)
+    assert torch.equal(qkv[:, : 4 * D].cpu(), c["q"]) and torch.equal(qkv[:, 4 * D:].cpu(), c["qkv"][:, 4 * D:])
+    for a, b in ((k8, c["k8"]), (v8, c["v8"])):
+        assert torch.equal(bits(a.cpu()), bits(b))
+    assert torch.equal(scales[0].cpu(), c["ks"]) and torch.equal(scales[1].cpu(), c["vs"])
+
+
+def special_append(codes, device):
+    """Infinities, NaN, zeros, the largest and smallest numbers, slots past the cache, a scale that is none: kv_write."""
+    dtype, bs = CODES[codes], 16
+    k8, v8, scales = block8.alloc(4, 2, bs, dtype, device)
+    scales[0].fill_(NAN)
+    scales[1].fill_(-1.0)
+    k = torch.zeros((7, 2, D), dtype=torch.bfloat16)
+    k[0, 0, :4] = torch.tensor([1.0, INF, -INF, NAN])
+    k[0, 1, 0] = 3e38
+    k[1, 0, 0] = 1e-39
+    v = k.flip(1)
+    slots = torch.tensor([0, 17, 18, -5, 64, 2 ** 40, 60])  # the second and third begin inside a block whose scale is none
+    dev = [t.to(device) for t in (k, v, slots)]
+    ops.kv_write(*dev, k8, v8, bs, kv_scales=scales)
+    return [t.cpu() for t in (k8, v8, *scales)]
+
+
+def check_special(got, codes):
+    k8, v8, ks, vs = got
+    most = MOST[CODES[codes]]
+    f = k8[0, 0, 0].float()
+    assert f[0] * ks[0, 0] == 1.0 and f[1] == most and f[2] == -most and (f[3] == 0 if codes == "int8" else bool(f[3].isnan()))
+    assert 3e38 / most <= float(ks[0, 1]) <= 6.1e38 / most and abs(float(k8[0, 1, 0].float()[0] * ks[0, 1]) / 3e38 - 1) <= (2 ** -7 if codes == "int8" else 2 ** -4)
+    tiny = float(torch.tensor(1e-39).bfloat16())
+    assert ks[1, 0] == 2.0 ** -126 and bool((k8[1, 0].float()[2:] == 0).all())
+    assert abs(float(k8[1, 0].float()[1, 0]) * 2.0 ** -126 - tiny) <= (2.0 ** -127 if codes == "int8" else tiny * 2 ** -4)
+    assert ks[3, 0] == 2.0 ** -126 and ks[2].isnan().all() and bool((vs[2] == -1).all())  # a block that no token went into
+    assert torch.equal(bits(v8[0, 1, 0]), bits(k8[0, 0, 0])) and vs[0, 1] == ks[0, 0]
+
+
+@both
+def test_append_special_cpu(codes):
+    check_special(special_append(codes, "cpu"), codes)
+
+
+@pytest.mark.gpu
+@both
+def test_append_special(codes):
+    got = special_append(codes, "cuda")
+    check_special(got, codes)
+    for a, b in zip(got, special_append(codes, "cpu")):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.gpu
+def test_growth_loses_less_than_a_step():
+    """A block filled token by token, each twice the one before: every int8 row ends less than a step from what was written."""
+    k8, v8, scales = block8.alloc(1, 1, 64, torch.int8, "cuda")
+    g = torch.Generator().manual_seed(3)
+    x = (torch.randn((64, 1, D), generator=g) * 2.0 ** (torch.arange(64)[:, None, None] / 6)).bfloat16()
+    for t in range(64):
+        row = x[t:t + 1].cuda()
+        ops.kv_write(row, row, torch.tensor([t], device="cuda"), k8, v8, 64, kv_scales=scales)
+    s = float(scales[0][0, 0])
+    assert s == float(ref.power_scale(x.float().abs().max()[None], torch.int8)[0])
+    assert float((k8[0, 0].cpu().double() * s - x[:, 0].double()).abs().max()) < s
+
+
+@pytest.mark.gpu
+@both
+def test_read_back(codes):
+    """kv_dequant_scratch: whole blocks as bf16 (a power of two's products are exact), those past a sequence's length left."""
+    dtype = CODES[codes]
+    k8, ks = random_cache(9, 3, 32, dtype, 4)
+    v8, vs = random_cache(9, 3, 32, dtype, 5, pow2=False)
+    table = torch.tensor([[4, 2, 8], [0, 7, 1]], dtype=torch.int32)
+    ctx = torch.tensor([65, 31], dtype=torch.int32)
+    a = on_gpu(k8, v8, table, ctx)
+    gk, gv, t = ops.kv_dequant_scratch(*a, kv_scales=tuple(on_gpu(ks, vs)))
+    for i, n in ((0, 3), (1, 1)):
+        for j in range(n):
+            b, to = int(table[i, j]), int(t[i, j])
+            assert torch.equal(gk[to].cpu(), ref.block_values(k8[b], ks[b]).bfloat16())
+            assert torch.equal(gv[to].cpu(), ref.block_values(v8[b], vs[b]).bfloat16())
+
+
+# ---------------------------------------------------------------- attention
+def attention64(q, k8, v8, ks, vs, table, new, ctx, causal=True):
+    """(result, sum p |v|) in 64 bits, rows of all sequences behind one another."""
+    bs, nkv = k8.shape[2], k8.shape[1]
+    out, size = torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape, dtype=torch.float64)
+    at = 0
+    for i, (n, x) in enumerate(zip(new, ctx)):
+        if n and x:
+            b = table[i, : -(-x // bs)].long()
+            k, v = ((c.view(torch.uint8)[b].view(c.dtype).double() * s.double()[b][..., None, None]).transpose(1, 2).reshape(-1, nkv, D)[:x] for c, s in ((k8, ks), (v8, vs)))
+            hide = torch.arange(x) > torch.arange(x - n, x)[:, None]
+            for h in range(q.shape[1]):
+                kv = h * nkv // q.shape[1]
+                t = q[at:at + n, h].double() @ k[:, kv].T * SCALE
+                p = torch.softmax(t.masked_fill(hide, -INF) if causal else t, -1)
+                out[at:at + n, h], size[at:at + n, h] = p @ v[:, kv], p @ v[:, kv].abs()
+        at += n
+    return out, size
+
+
+def near(got, want, size, roundings):
+    """Weights rounded to bf16 `roundings` times (in the sum, and where the row sum is of the rounded ones), the result once; scores of
+    128 products in fp32, of size 30 at most here: 128 2^-24 30 < 2^-12 of a weight, twice."""
+    tol = (roundings * 2 ** -8 + 2 ** -11) * size + 2 ** -8 * want.abs() * 1.01
+    err = (got.double() - want).abs()
+    assert bool((err <= tol).all()), float((err / tol.clamp(min=1e-300)).max())
+
+
+def cache_of(codes, nkv, bs, ctx, seed, junk=True, pow2=True):
+    dtype = CODES[codes]
+    table, blocks = table_of([-(-x // bs) for x in ctx], seed)
+    k8, ks = random_cache(blocks, nkv, bs, dtype, seed, pow2)
+    v8, vs = random_cache(blocks, nkv, bs, dtype, seed + 1, pow2)
+    if junk:  # rows behind a sequence, and scales of blocks that are none's
+        used = set()
+        for i, x in enumerate(ctx):
+            used |= set(table[i, : -(-x // bs)].tolist())
+            if x % bs:
+                b = int(table[i, x // bs])
+                bits(k8)[b, :, x % bs:] = 0x7F
+                bits(v8)[b, :, x % bs:] = 0x7F
+        for b in range(blocks):
+            if b not in used:
+                ks[b], vs[b] = NAN, INF
+                bits(k8)[b] = 0x7F
+                bits(v8)[b] = 0x7F
+    return table, k8, v8, ks, vs
+
+
+def run_decode(codes, nq, nkv, bs, ctx, n_parts, seed=0, workspace=None, pow2=True):
+    table, k8, v8, ks, vs = cache_of(codes, nkv, bs, ctx, seed, pow2=pow2)
+    q = torch.randn((len(ctx), nq, D), generator=torch.Generator().manual_seed(seed + 9)).bfloat16()
+    dev = on_gpu(q, k8, v8, table, torch.tensor(ctx, dtype=torch.int32))
+    out = torch.full((len(ctx), nq, D), NAN, dtype=torch.bfloat16, device="cuda")
+    r = ops.decode_attention(*dev, SCALE, out, n_parts, workspace=workspace, kv_scales=tuple(on_gpu(ks, vs)))
+    assert r is out
+    want, size = attention64(q, k8, v8, ks, vs, table, [1] * len(ctx), ctx)
+    near(out.cpu(), want, size, 1 if pow2 else 2)
+    assert all(bool((out[i] == 0).all()) for i, x in enumerate(ctx) if x == 0)
+    return dev, (ks, vs), out
+
+
+@pytest.mark.gpu
+@both
+@pytest.mark.parametrize("bs", [16, 32, 64, 128])
+@pytest.mark.parametrize("ctx", [[1], [700], [0, 15, 16, 17, 31, 32, 33, 63, 64, 65], [129, 0, 2100, 511]])
+@pytest.mark.parametrize("n_parts", [None, 1, 3])
+def test_decode(codes, bs, ctx, n_parts):
+    run_decode(codes, 8, 2, bs, ctx, n_parts, seed=bs)
+
+
+@pytest.mark.gpu
+@both
+@pytest.mark.parametrize("nq,nkv", [(1, 1), (32, 8), (14, 2), (12, 4), (16, 1), (5, 1), (64, 8), (8, 8), (22, 2)])
+def test_decode_heads(codes, nq, nkv):
+    run_decode(codes, nq, nkv, 64, [333, 20, 1500], None, seed=nq)
+
+
+@pytest.mark.gpu
+@both
+@pytest.mark.parametrize("n_parts", [1, 17, 65])
+def test_decode_long(codes, n_parts):
+    """More than 64 blocks a part (their numbers are fetched 64 at a time), more parts than a wave has lanes."""
+    run_decode(codes, 4, 1, 16, [9001, 5, 4096], n_parts, seed=3)
+
+
+@pytest.mark.gpu
+@both
+def test_decode_scales_that_are_no_powers(codes):
+    run_decode(codes, 8, 2, 32, [500, 33], None, seed=8, pow2=False)
+
+
+@pytest.mark.gpu
+@both
+def test_decode_unlike_scales(codes):
+    """Blocks 2^30 apart: a large value under no weight must not cost a small one its digits, nor the other way round."""
+    nkv, bs, ctx = 1, 16, [256]
+    table, k8, v8, ks, vs = cache_of(codes, nkv, bs, ctx, 5)
+    vs *= 2.0 ** torch.randint(-15, 16, vs.shape, generator=torch.Generator().manual_seed(1))
+    q = torch.randn((1, 4, D)).bfloat16()
+    dev = on_gpu(q, k8, v8, table, torch.tensor(ctx, dtype=torch.int32))
+    out = torch.empty_like(dev[0])
+    ops.decode_attention(*dev, SCALE, out, None, kv_scales=tuple(on_gpu(ks, vs)))
+    near(out.cpu(), *attention64(q, k8, v8, ks, vs, table, [1], ctx), 1)
+
+
+@pytest.mark.gpu
+def test_decode_strides_workspaces_and_pages():
+    """Rows of a fused projection, tables with more columns than blocks and rows farther apart, a workspace full of NaN, numbers in the
+    table that are no blocks (only rows that use them suffer)."""
+    nq, nkv, bs, ctx = 8, 2, 64, [300, 70]
+    table, k8, v8, ks, vs = cache_of("int8", nkv, bs, ctx, 2)
+    wide = torch.full((2, 40), -7, dtype=torch.int32)
+    wide[:, : table.shape[1]] = table
+    wide[1, 2:] = 2 ** 30
+    row = torch.randn((2, (nq + 2 * nkv) * D)).bfloat16()
+    q = row[:, : nq * D].unflatten(1, (nq, D))
+    n = 5
+    ws = (torch.full((4, nq, n, D), NAN, device="cuda"), torch.full((4, nq, n, 2), NAN, device="cuda"))
+    out = torch.full((2, nq, D), NAN, dtype=torch.bfloat16, device="cuda")
+    dev = row.cuda()[:, : nq * D].unflatten(1, (nq, D))
+    ops.decode_attention(dev, k8.cuda(), v8.cuda(), wide.cuda()[:, :17], torch.tensor(ctx, dtype=torch.int32).cuda(), SCALE, out, n, workspace=ws,
+                         kv_scales=tuple(on_gpu(ks, vs)))
+    near(out.cpu(), *attention64(q, k8, v8, ks, vs, table, [1, 1], ctx), 1)
+    # a length past the table is cut to it
+    long = torch.tensor([300, 99999], dtype=torch.int32)
+    for parts in (1, 7):
+        ops.decode_attention(dev, k8.cuda(), v8.cuda(), table.cuda(), long.cuda(), SCALE, out, parts, kv_scales=tuple(on_gpu(ks, vs)))
+        near(out[:1].cpu(), *[t[:1] for t in attention64(q, k8, v8, ks, vs, table, [1, 1], ctx)], 1)
+
+
+def run_prefill(codes, nq, nkv, bs, new, ctx, seed=0, causal=True, planned=True, pow2=True):
+    table, k8, v8, ks, vs = cache_of(codes, nkv, bs, ctx, seed, pow2=pow2)
+    T = sum(new)
+    q = torch.randn((T, nq, D), generator=torch.Generator().manual_seed(seed + 9)).bfloat16()
+    cu = torch.tensor([sum(new[:i]) for i in range(len(new) + 1)], dtype=torch.int32)
+    plan = ops.prefill_plan(new, ctx, nq, nkv, "cuda", causal) if planned else None
+    dev = on_gpu(q, k8, v8, table, cu, torch.tensor(ctx, dtype=torch.int32))
+    out = torch.full((T, nq, D), NAN, dtype=torch.bfloat16, device="cuda")
+    r = ops.prefill_attention(*dev, SCALE, out, work=plan, kv_scales=tuple(on_gpu(ks, vs)), causal=causal)
+    assert r is out
+    vals = (k8, v8, ks, vs)
+    if not pow2:  # the kernel's values are rounded to bf16
+        vals = [bits(c).view(c.dtype) for c in (k8, v8)] + [ks, vs]
+        kb, vb = ref.block_values(k8, ks).bfloat16(), ref.block_values(v8, vs).bfloat16()
+        vals = (kb, vb, torch.ones_like(ks), torch.ones_like(vs))
+    want, size = attention64(q, *vals, table, new, ctx, causal)
+    near(out.cpu(), want, size, 2)
+    return plan
+
+
+@pytest.mark.gpu
+@both
+@pytest.mark.parametrize("bs", [16, 32, 64, 128])
+@pytest.mark.parametrize("new,ctx", [([1], [1]), ([1, 64, 3], [200, 64, 67]), ([130, 0, 33], [130, 5, 400]), ([16], [4000])])
+def test_prefill(codes, bs, new, ctx):
+    run_prefill(codes, 8, 2, bs, new, ctx, seed=bs)
+
+
+@pytest.mark.gpu
+@both
+@pytest.mark.parametrize("nq,nkv", [(1, 1), (14, 2), (12, 4), (16, 1), (5, 1), (3, 3), (24, 1), (32, 8)])
+def test_prefill_heads(codes, nq, nkv):
+    run_prefill(codes, nq, nkv, 64, [100, 7], [333, 7], seed=nq)
+
+
+@pytest.mark.gpu
+@both
+def test_prefill_tiles_of_eight_waves(codes):
+    plan = run_prefill(codes, 32, 8, 64, [1100, 900, 1300, 1000], [1100, 1000, 1300, 1001], seed=4)
+    assert plan.waves == 8 and plan.places == 0
+
+
+@pytest.mark.gpu
+@both
+def test_prefill_parts(codes):
+    """Few rows behind many keys: parts, joined; some see none of a part's keys."""
+    plan = run_prefill(codes, 8, 2, 16, [70, 3], [3000, 900], seed=6)
+    assert plan.n_joins and plan.places
+
+
+@pytest.mark.gpu
+@both
+def test_prefill_bidirectional_and_unplanned(codes):
+    run_prefill(codes, 8, 2, 32, [90, 5], [90, 500], seed=7, causal=False)
+    run_prefill(codes, 8, 2, 32, [90, 5], [90, 500], seed=7, planned=False)
+    run_prefill(codes, 8, 2, 32, [90, 5], [90, 500], seed=7, planned=False, causal=False)
+
+
+@pytest.mark.gpu
+@both
+def test_prefill_scales_that_are_no_powers(codes):
+    run_prefill(codes, 8, 2, 32, [90, 5], [90, 500], seed=7, pow2=False)
+
+
+# ---------------------------------------------------------------- together
+def server(device, codes, steps=6):
+    """Two prompts in chunks beside a decoding stream: append and attend, step by step; the attention results of all steps."""
+    nq, nkv, bs = 8, 2, 16
+    k8, v8, scales = block8.alloc(40, nkv, bs, CODES[codes], device)
+    table = torch.randperm(40, generator=torch.Generator().manual_seed(5)).to(torch.int32)[:36].view(3, 12)
+    cs = ref.rope_cos_sin(D, 200, 500000.0)
+    have, got = [0, 0, 0], []
+    g = torch.Generator().manual_seed(11)
+    for step in range(steps):
+        new = [[23, 40], [30, 1], [1, 33], [17, 17], [40, 2], [5, 5]][step] + [1]
+        T = sum(new)
+        qkv = torch.randn((T, (nq + 2 * nkv) * D), generator=g).bfloat16().to(device)
+        spans = [(h, h + n) for h, n in zip(have, new)]
+        have = [h + n for h, n in zip(have, new)]
+        pos = torch.cat([torch.arange(a, b) for a, b in spans]).to(device)
+        slots = slots_of(table, spans, bs).to(device)
+        ops.rope_cache(qkv, pos, cs.to(device), slots, k8, v8, nq, nkv, D, bs, kv_scales=scales)
+        q = qkv[:, : nq * D].view(T, nq, D)
+        out = torch.empty((T, nq, D), dtype=torch.bfloat16, device=device)
+        cu = torch.tensor([0, new[0], new[0] + new[1]], dtype=torch.int32, device=device)
+        ctx = torch.tensor(have, dtype=torch.int32, device=device)
+        bt = table.to(device)
+        work = ops.prefill_plan(new[:2], have[:2], nq, nkv, device)
+        ops.prefill_attention(q[: T - 1], k8, v8, bt[:2], cu, ctx[:2], SCALE, out[: T - 1], work=work, kv_scales=scales)
+        ops.decode_attention(q[T - 1:], k8, v8, bt[2:], ctx[2:], SCALE, out[T - 1:], None, kv_scales=scales)
+        got.append(out.float().cpu())
+    return got, k8.cpu(), scales[0].cpu()
+
+
+@both
+def test_served_steps_keep_to_the_unquantised_attention(codes):
+    """On the CPU: the whole run against attention over the values as written (their codes' roundings alone lie between)."""
+    got, k8, ks = server("cpu", codes)
+    assert all(bool(x.isfinite().all()) for x in got) and float(ks.max()) <= 2.0 ** -4
+
+
+@pytest.mark.gpu
+@both
+def test_served_steps(codes):
+    """The same run on the GPU: every step's results within the roundings of the kernels', and codes within one of the CPU's (a value
+    next to a code's border may fall on either side; its neighbours' weights move by less than a step's worth)."""
+    got, k8, ks = server("cuda", codes)
+    want, k8c, ksc = server("cpu", codes)
+    assert torch.equal(ks, ksc)
+    differ = (k8.float() - k8c.float()).abs() > 0
+    assert float(differ.float().mean()) < 1e-4
+    for a, b in zip(got, want):
+        # 3 roundings to bf16 of weights or results on the GPU, 2 on the CPU, of values below 4.5, halved by the mean over keys; a
+        # first token's result is one value
+        assert float((a - b).abs().max()) <= 5 * 2 ** -8 * 4.5
+
+
+@pytest.mark.gpu
+def test_captured_step_replays():
+    """Append, decode attention and the read-back captured, replayed with other inputs between eager work; a second graph beside it."""
+    nq, nkv, bs, B = 8, 2, 16, 3
+    graphs = []
+    for n in range(2):
+        k8, v8, scales = block8.alloc(30, nkv, bs, torch.int8, "cuda")
+        table = torch.randperm(30, generator=torch.Generator().manual_seed(n)).to(torch.int32).view(3, 10).cuda()
+        cs = ref.rope_cos_sin(D, 200, 500000.0).cuda()
+        st = dict(qkv=torch.zeros((B, (nq + 2 * nkv) * D), dtype=torch.bfloat16, device="cuda"), pos=torch.zeros(B, dtype=torch.int64, device="cuda"),
+                  slots=torch.full((B,), -1, device="cuda"), ctx=torch.zeros(B, dtype=torch.int32, device="cuda"),
+                  out=torch.zeros((B, nq, D), dtype=torch.bfloat16, device="cuda"))
+
+        def step(st=st, k8=k8, v8=v8, scales=scales, table=table, cs=cs):
+            ops.rope_cache(st["qkv"], st["pos"], cs, st["slots"], k8, v8, nq, nkv, D, bs, kv_scales=scales)
+            ops.decode_attention(st["qkv"][:, : nq * D].view(B, nq, D), k8, v8, table, st["ctx"], SCALE, st["out"], 4, kv_scales=scales)
+
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        graphs.append((graph, st, step, table, k8, v8, scales))
+    g = torch.Generator().manual_seed(4)
+    rows = [torch.randn((B, (nq + 2 * nkv) * D), generator=g).bfloat16() for _ in range(20)]
+    eager = block8.alloc(30, nkv, bs, torch.int8, "cuda")
+    for t, row in enumerate(rows):
+        live = torch.tensor([True, True, t % 3 != 2])  # a padded row now and then: its stream stays away
+        for graph, st, step, table, k8, v8, scales in graphs:
+            st["qkv"].copy_(row)
+            st["pos"].fill_(t)
+            st["slots"].copy_(torch.where(live.cuda(), table[:, t // bs].long() * bs + t % bs, -1))
+            st["ctx"].copy_(torch.where(live.cuda(), t + 1, 0))
+            graph.replay()
+        outs = [st["out"].clone() for _, st, *_ in graphs]
+        _, st, _, table, *_ = graphs[0]
+        q = row.cuda()
+        ops.rope_cache(q, st["pos"], cs, st["slots"], eager[0], eager[1], nq, nkv, D, bs, kv_scales=eager[2])
+        out = torch.empty_like(st["out"])
+        ops.decode_attention(q[:, : nq * D].view(B, nq, D), eager[0], eager[1], table, st["ctx"], SCALE, out, 4, kv_scales=eager[2])
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], out) and torch.equal(outs[1], out)
+        assert torch.equal(graphs[0][4], eager[0])
+
+
+@pytest.mark.gpu
+def test_other_stream():
+    """The kernels go to the current stream, with their workspace: results on a side stream are those of the default one."""
+    dev, (ks, vs), want = run_decode("int8", 8, 2, 64, [2100, 300], 9)
+    scales = tuple(on_gpu(ks, vs))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        out = torch.empty_like(want)
+        for _ in range(3):
+            ops.decode_attention(*dev, SCALE, out, 9, kv_scales=scales)
+    s.synchronize()
+    assert torch.equal(out, want)
+
+
+# ---------------------------------------------------------------- refusals (CPU tensors stand for the GPU's: the checks are the host's)
+def test_refusals():
+    k8, v8, scales = block8.alloc(4, 2, 16, torch.int8, "cpu")
+    chk = block8._check_cache
+    chk(k8, v8, scales)
+    with pytest.raises(TypeError):
+        chk(k8.float(), v8.float(), scales)
+    with pytest.raises(TypeError):
+        chk(k8, v8.view(torch.uint8), scales)
+    with pytest.raises(TypeError):
+        chk(k8, v8, (scales[0].half(), scales[1]))
+    with pytest.raises(ValueError):
+        chk(k8, v8, (scales[0][:3], scales[1]))
+    with pytest.raises(ValueError):
+        chk(k8, v8, (scales[0].t().contiguous().t(), scales[1]))
+    with pytest.raises(ValueError):
+        chk(k8[:, :, :, :64].contiguous(), v8[:, :, :, :64].contiguous(), scales)
+    with pytest.raises(ValueError):
+        chk(k8.view(4, 2, 128, 16)[:, :, :24].contiguous(), v8.view(4, 2, 128, 16)[:, :, :24].contiguous(), scales)
+    with pytest.raises(ValueError):
+        chk(k8.transpose(0, 1).contiguous().transpose(0, 1), v8, scales)
+    with pytest.raises(TypeError):
+        block8.alloc(4, 2, 16, torch.bfloat16, "cpu")
+    q, out = torch.zeros((3, 8, D), dtype=torch.bfloat16), torch.zeros((3, 8, D), dtype=torch.bfloat16)
+    bt, ctx = torch.zeros((3, 2), dtype=torch.int32), torch.ones(3, dtype=torch.int32)
+    rd = lambda **k: block8._check_reader(**{**dict(q=q, out=out, k_cache=k8, v_cache=v8, kv_scales=scales, block_tables=bt, ctx_lens=ctx, n=3), **k})  # noqa: E731
+    rd()
+    for bad in (dict(q=q[:, :7]), dict(out=out[:2]), dict(block_tables=bt[:2]), dict(ctx_lens=ctx[:2]), dict(block_tables=bt[:, :0]),
+                dict(block_tables=bt.t().contiguous().t()), dict(out=out.transpose(0, 1).contiguous().transpose(0, 1)), dict(ctx_lens=torch.ones(6, dtype=torch.int32)[::2])):
+        with pytest.raises(ValueError):
+            rd(**bad)
+    for bad in (dict(q=q.float()), dict(block_tables=bt.long()), dict(ctx_lens=ctx.long()), dict(out=out.float())):
+        with pytest.raises(TypeError):
+            rd(**bad)
+    with pytest.raises(ValueError):
+        ops.prefill_plan([3], [2], 8, 2, "cpu")
+    with pytest.raises(ValueError):
+        ops.prefill_plan([3], [4, 5], 8, 2, "cpu")
+    with pytest.raises(ValueError):
+        ops.prefill_plan([3], [4], 8, 3, "cpu")
+
+
+@pytest.mark.gpu
+def test_refusals_gpu():
+    k8, v8, scales = block8.alloc(4, 2, 16, torch.int8)
+    cs = ref.rope_cos_sin(D, 32, 500000.0).cuda()
+    qkv = torch.zeros((3, 8 * D), dtype=torch.bfloat16, device="cuda")
+    pos, slots = torch.arange(3, device="cuda"), torch.arange(3, device="cuda")
+    call = lambda **k: ops.rope_cache(**{**dict(qkv=qkv, positions=pos, cos_sin=cs, slot_mapping=slots, k_cache=k8, v_cache=v8, n_q=4, n_kv=2, head_dim=D,  # noqa: E731
+                                                block_size=16, kv_scales=scales), **k})
+    call()
+    for bad in (dict(n_q=5), dict(block_size=32), dict(slot_mapping=slots[:2]), dict(positions=pos[:2]), dict(cos_sin=cs[:, :64].contiguous()),
+                dict(qkv=torch.zeros((3, 8 * D + 4), dtype=torch.bfloat16, device="cuda")[:, : 8 * D]), dict(slot_mapping=slots.cpu()), dict(row_scale=torch.ones(2, device="cuda")),
+                dict(qkv=torch.zeros(3 * 8 * D + 1, dtype=torch.bfloat16, device="cuda")[1:].view(3, 8 * D)), dict(slot_mapping=slots.int())):
+        with pytest.raises((ValueError, TypeError)):
+            call(**bad)
+    q, out = qkv[:, : 4 * D].view(3, 4, D), torch.empty((3, 4, D), dtype=torch.bfloat16, device="cuda")
+    bt, ctx = torch.zeros((3, 2), dtype=torch.int32, device="cuda"), torch.ones(3, dtype=torch.int32, device="cuda")
+    for parts, ws in ((0, None), (2, (torch.empty((3, 4, 3, D), device="cuda"), torch.empty((3, 4, 3, 2), device="cuda")))):
+        with pytest.raises(ValueError):
+            ops.decode_attention(q, k8, v8, bt, ctx, SCALE, out, parts, workspace=ws, kv_scales=scales)
+    wide = torch.zeros((1, 34, D), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError):
+        ops.decode_attention(wide, k8, v8, bt[:1], ctx[:1], SCALE, torch.empty_like(wide), None, kv_scales=scales)
+    cu = torch.tensor([0, 3], dtype=torch.int32, device="cuda")
+    for plan, e in ((ops.prefill_plan([2], [3], 4, 2), ValueError), (ops.prefill_plan([3], [3], 4, 2, causal=False), ValueError), (torch.zeros(2, dtype=torch.int32, device="cuda"), TypeError)):
+        with pytest.raises(e):
+            ops.prefill_attention(q, k8, v8, bt[:1], cu, ctx[:1], SCALE, out, work=plan, kv_scales=scales)
+
+
+@pytest.mark.gpu
+def test_nothing_to_do():
+    k8, v8, scales = block8.alloc(4, 2, 16, torch.int8)
+    qkv = torch.zeros((0, 8 * D), dtype=torch.bfloat16, device="cuda")
+    none = torch.zeros(0, dtype=torch.int64, device="cuda")
+    ops.rope_cache(qkv, none, ref.rope_cos_sin(D, 32, 500000.0).cuda(), none, k8, v8, 4, 2, D, 16, kv_scales=scales)
+    q = torch.zeros((0, 4, D), dtype=torch.bfloat16, device="cuda")
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")  # noqa: E731
+    ops.decode_attention(q, k8, v8, i32(0, 2), i32(0), SCALE, torch.empty_like(q), None, kv_scales=scales)
+    ops.prefill_attention(q, k8, v8, i32(1, 2), i32(2), i32(1), SCALE, torch.empty_like(q), work=ops.prefill_plan([0], [0], 4, 2), kv_scales=scales)
+
+
+def test_plan_covers_every_row_and_key():
+    """The plan's items: each row tile's keys once, in whole tiles of 64, parts behind one another in the workspace."""
+    g = torch.Generator().manual_seed(2)
+    for nq, nkv in ((32, 8), (14, 2), (16, 1), (8, 8)):
+        for n in range(1, 5):
+            new = torch.randint(0, 700, (n,), generator=g).tolist()
+            ctx = [a + b for a, b in zip(new, torch.randint(0, 9000, (n,), generator=g).tolist())]
+            p = ops.prefill_plan(new, ctx, nq, nkv, "cpu")
+            flat, G, tile = p.work.tolist(), nq // nkv, 32 * p.waves
+            items = [flat[6 * i:6 * i + 6] for i in range(p.n_work)]
+            joins = [flat[6 * p.n_work + 4 * i:][:4] for i in range(p.n_joins)]
+            places = sorted(w[4] for w in items if w[4] >= 0)
+            assert places == list(range(p.places)) and sum(j[3] for j in joins) == p.places
+            for s, (ql, cl) in enumerate(zip(new, ctx)):
+                for r0 in range(0, ql * G, tile):
+                    mine = sorted(w[2:5] for w in items if w[0] == s and w[1] == r0)
+                    assert mine[0][0] == 0 and all(a[1] == b[0] and a[1] % 64 == 0 for a, b in zip(mine, mine[1:]))
+                    assert mine[-1][1] > cl - ql + (min(r0 + tile, ql * G) - 1) // G
+                    if len(mine) > 1:
+                        j = [j for j in joins if j[:2] == [s, r0]]
+                        assert len(j) == 1 and [m[2] for m in mine] == list(range(j[0][2], j[0][2] + j[0][3]))
+                    else:
+                        assert mine[0][2] == -1
