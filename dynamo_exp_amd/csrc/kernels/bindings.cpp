@@ -48,7 +48,7 @@ int dx_block_decode(void*, float*, float*, const void*, int64_t, const void*, co
 int dx_block_prefill(void*, float*, float*, const void*, int64_t, const void*, const void*, const float*, const float*, const int*, int,
                      int, const int*, const int*, const int*, int, const int*, int, int, int, int, int, int, int, float, int, int,
                      hipStream_t);
-int dx_w4_gemm(void*, int64_t, const void*, int64_t, const void*, const void*, const void*, int, int, int, int, hipStream_t);
+int dx_w4_gemm(void*, int64_t, const void*, int64_t, const void*, const void*, const void*, float*, int, int, int, int, int, int, int, hipStream_t);
 int dx_rmsnorm_quant(void*, float*, const void*, void*, const void*, int, int, int64_t, int64_t, float, hipStream_t);
 int dx_decode_advance(void*, void*, void*, void*, void*, const void*, const void*, void*, void*, const int*, int, int,
                       int, int, int, hipStream_t);
@@ -166,8 +166,9 @@ PYBIND11_MODULE(_C_kernels, m) {
                            bs, nb, scale, causal, code, S(st)),
           "block_prefill");
   });
-  m.def("w4_gemm", [](u y, int64_t ldy, u x, int64_t ldx, u w, u s, u z, int M, int N, int K, int group, u st) {
-    check(dx_w4_gemm(P(y), ldy, P(x), ldx, P(w), P(s), P(z), M, N, K, group, S(st)), "w4_gemm");
+  m.def("w4_gemm", [](u y, int64_t ldy, u x, int64_t ldx, u w, u s, u z, u ws, int M, int N, int K, int group, int waves, int rt,
+                     int splits, u st) {
+    check(dx_w4_gemm(P(y), ldy, P(x), ldx, P(w), P(s), P(z), (float*)ws, M, N, K, group, waves, rt, splits, S(st)), "w4_gemm");
   });
   m.def("gemm256", [](u y, int64_t ldy, u x, int64_t ldx, u w, int M, int N, int K, int epi, int gm, u st, u rs) {
     check(dx_gemm256(P(y), ldy, P(x), ldx, P(w), M, N, K, epi, gm, S(st), (const float*)rs), "gemm256");

@@ -1,8 +1,8 @@
 // Products of few rows with weights in 4 bits, for gfx950:  y[m, n] = sum_k x[m, k] (c[n, k] - z[n, k / g]) s[n, k / g]
 // c, z in 0..15, s bf16, groups of g = 32, 64 or 128 columns; x and y bf16, sums in fp32.
 //
-// Bound by the weights' bytes: each is read once by one wave and goes straight into a matrix product's A operand (16 weight rows),
-// the x rows are its 16 columns.  A code becomes bf16 by being put in the mantissa of 128 (0x4300 | c = 128 + c, exact), two by
+// Bound by the weights' bytes: each is read once by one wave and goes straight into a matrix product's B operand (16 weight rows),
+// the x rows are the rows of A.  A code becomes bf16 by being put in the mantissa of 128 (0x4300 | c = 128 + c, exact), two by
 // one and-or; what that adds is taken off group by group, with the sum of the group's x from a product with ones:
 //   sum x (c - z) = sum x (128 + c) - (128 + z) sum x
 // The two sums are exact to fp32's 2^-24 of their size, 136 / 4.6 times the wanted one's at random codes: 2^-19, against the
@@ -10,14 +10,16 @@
 //
 // Weights are laid out once (ops.w4_pack): [N / 16][K / 128][lane][4] words, lane = 16 (k quarter) + row, word s the lane's eight
 // columns 32 s + 8 (lane / 16) .. of the 128, column 2 i in nibble i, 2 i + 1 in nibble 4 + i: one 1 KB load of a wave is 16 rows x
-// 128 columns.  Scales [N / 16][K / g][16] bf16, zeros (128 + z) the same in bytes.  The K axis is split over the waves of a
-// workgroup, whose sums are added in LDS in the waves' order.
+// 128 columns.  Scales [N / 16][K / 128][row][group] bf16, zeros (128 + z) the same in bytes: a lane's products are all of one row.
+// The K axis is split over the waves of a workgroup, whose sums are added in LDS in the waves' order, and over workgroups where rows
+// are few (their sums in fp32, added by a second kernel).  x rows come from L2 once for RT tiles.
 #include "block8.h"
 
 namespace {
 
 struct W4Args {
   bf16_t* y;
+  float* ws;  // [splits][M][N], where K is split over workgroups
   const bf16_t* x;
   const raw4* w;
   const uint16_t* s;
@@ -26,63 +28,81 @@ struct W4Args {
   int M, N, K, chunks;  // chunks of 128 columns, the last one perhaps not whole
 };
 
-__device__ __forceinline__ bf16x8_t codes_bf16(uint32_t w) {
+// (`base` is 0x43004300 in a vector register: with both constants in scalar ones the and-or would be two instructions)
+__device__ __forceinline__ bf16x8_t codes_bf16(uint32_t w, uint32_t base) {
   raw4 o;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = ((w >> (4 * i)) & 0x000F000Fu) | 0x43004300u;
+  for (int i = 0; i < 4; ++i) o[i] = ((w >> (4 * i)) & 0x000F000Fu) | base;
   return __builtin_bit_cast(bf16x8_t, o);
 }
 
-// RT: 16-row tiles of weights a wave; T: 16-row tiles of x; GS: k steps of 32 in a group
-template <int RT, int T, int GS, bool ZERO>
+// RT: 16-row tiles of weights a wave; T: tiles of 4 E rows of x (E of every four rows of A); GS: k steps of 32 in a group; DW: chunks on
+// their way
+template <int RT, int T, int E, int GS, bool ZERO, int DW>
 __global__ void __launch_bounds__(512) w4_kernel(const W4Args a) {
-  extern __shared__ __attribute__((aligned(16))) float red[];  // [waves][RT][T][16 tokens][16 rows]
+  extern __shared__ __attribute__((aligned(16))) float red[];  // [waves][RT][T][4 E tokens][16 rows]
+  static_assert(DW % 2 == 0, "x alternates between two places");
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int r = lane & 15, q = lane >> 4;
-  const int tiles = (a.N + 15) >> 4, nt0 = blockIdx.x * RT, m0 = blockIdx.y * (16 * T);
+  const int tiles = (a.N + 15) >> 4, nt0 = blockIdx.x * RT, m0 = blockIdx.y * (4 * E * T);
   constexpr int GC = 4 / GS;  // groups in a chunk
-  const int groups = (a.K + 32 * GS - 1) / (32 * GS);
+  uint32_t base = 0x43004300u;
+  asm("" : "+v"(base));
   const raw4 kOnes = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
 
-  f32x4 acc[RT][T];
+  float acc[RT][T][E];
 #pragma unroll
   for (int i = 0; i < RT; ++i)
 #pragma unroll
-    for (int t = 0; t < T; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  const bf16_t* xp[T];
+    for (int t = 0; t < T; ++t)
 #pragma unroll
-  for (int t = 0; t < T; ++t) xp[t] = a.x + (int64_t)min(m0 + 16 * t + r, a.M - 1) * a.ldx + 8 * q;
+      for (int e = 0; e < E; ++e) acc[i][t][e] = 0.f;
 
   struct Chunk {
-    raw4 w[RT], x[T][4];
-    raw2 s[RT][GC];
-    uint32_t z[RT][GC];
+    raw4 w[RT];
+    uint32_t s[RT][(GC + 1) / 2], z[RT];
   };
-  auto load = [&](int kc, Chunk& c) {
+  struct Rows {
+    raw4 x[T][4];
+  };
+  const bf16_t* xp[T];  // row 4 i + j of A is token E i + j % E
+#pragma unroll
+  for (int t = 0; t < T; ++t) xp[t] = a.x + (int64_t)min(m0 + 4 * E * t + E * (r >> 2) + (r & (E - 1)), a.M - 1) * a.ldx + 8 * q;
+  int64_t tile_at[RT];  // first chunk of a tile (one behind the last is the last again, and goes nowhere)
+#pragma unroll
+  for (int i = 0; i < RT; ++i) tile_at[i] = (int64_t)min(nt0 + i, tiles - 1) * a.chunks;
+  const int step = waves * gridDim.z, first = wid + waves * blockIdx.z;  // this wave's chunks: first, first + step, ..
+  const int n = a.chunks > first ? (a.chunks - first + step - 1) / step : 0;
+  auto load_w = [&](int j, Chunk& c) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
-      const int nt = min(nt0 + i, tiles - 1);
-      c.w[i] = __builtin_nontemporal_load(a.w + ((int64_t)nt * a.chunks + kc) * 64 + lane);
-#pragma unroll
-      for (int g = 0; g < GC; ++g) {
-        const int64_t at = ((int64_t)nt * groups + min(kc * GC + g, groups - 1)) * 16 + 4 * q;
-        c.s[i][g] = *reinterpret_cast<const raw2*>(a.s + at);
-        if constexpr (ZERO) c.z[i][g] = *reinterpret_cast<const uint32_t*>(a.z + at);
-      }
-    }
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const int k = 128 * kc + 32 * s;
-      const bool in = k < a.K;  // (K is a multiple of 32)
-#pragma unroll
-      for (int t = 0; t < T; ++t) {
-        c.x[t][s] = *reinterpret_cast<const raw4*>(xp[t] + (in ? k : 0));
-        if (!in) c.x[t][s] = raw4{0u, 0u, 0u, 0u};
+      const int64_t at = tile_at[i] + first + j * step;
+      c.w[i] = __builtin_nontemporal_load(a.w + at * 64 + lane);
+      const uint16_t* s = a.s + (at * 16 + r) * GC;
+      const uint8_t* z = a.z + (at * 16 + r) * GC;
+      if constexpr (GC == 1) {
+        c.s[i][0] = *s;
+        if constexpr (ZERO) c.z[i] = *z;
+      } else if constexpr (GC == 2) {
+        c.s[i][0] = *reinterpret_cast<const uint32_t*>(s);
+        if constexpr (ZERO) c.z[i] = *reinterpret_cast<const uint16_t*>(z);
+      } else {
+        const raw2 v = *reinterpret_cast<const raw2*>(s);
+        c.s[i][0] = v[0], c.s[i][1] = v[1];
+        if constexpr (ZERO) c.z[i] = *reinterpret_cast<const uint32_t*>(z);
       }
     }
   };
-  auto compute = [&](const Chunk& c) {
+  auto load_x = [&](int j, Rows& c) __attribute__((always_inline)) {
+    const int k0 = 128 * (first + j * step);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int k = k0 + 32 * s < a.K ? k0 + 32 * s : 0;  // (behind the columns, whose scales are 0, any x of the row will do)
+#pragma unroll
+      for (int t = 0; t < T; ++t) c.x[t][s] = *reinterpret_cast<const raw4*>(xp[t] + k);
+    }
+  };
+  auto compute = [&](const Chunk& c, const Rows& y) __attribute__((always_inline)) {
 #pragma unroll
     for (int g = 0; g < GC; ++g) {
       f32x4 xs[T];
@@ -91,7 +111,7 @@ __global__ void __launch_bounds__(512) w4_kernel(const W4Args a) {
         xs[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = g * GS; s < (g + 1) * GS; ++s)
-          xs[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, kOnes), __builtin_bit_cast(bf16x8_t, c.x[t][s]), xs[t], 0, 0, 0);
+          xs[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, y.x[t][s]), __builtin_bit_cast(bf16x8_t, kOnes), xs[t], 0, 0, 0);
       }
 #pragma unroll
       for (int i = 0; i < RT; ++i) {
@@ -100,78 +120,114 @@ __global__ void __launch_bounds__(512) w4_kernel(const W4Args a) {
         for (int t = 0; t < T; ++t) part[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int s = g * GS; s < (g + 1) * GS; ++s) {
-          const bf16x8_t w = codes_bf16(c.w[i][s]);
+          const bf16x8_t w = codes_bf16(c.w[i][s], base);
 #pragma unroll
-          for (int t = 0; t < T; ++t) part[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, __builtin_bit_cast(bf16x8_t, c.x[t][s]), part[t], 0, 0, 0);
+          for (int t = 0; t < T; ++t) part[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, y.x[t][s]), w, part[t], 0, 0, 0);
         }
+        const float sc = g & 1 ? bf16hi(c.s[i][g >> 1]) : bf16lo(c.s[i][g >> 1]);
+        const float zc = ZERO ? (float)((c.z[i] >> (8 * g)) & 0xffu) : 136.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float sc = e & 1 ? bf16hi(c.s[i][g][e >> 1]) : bf16lo(c.s[i][g][e >> 1]);
-          const float zc = ZERO ? (float)((c.z[i][g] >> (8 * e)) & 0xffu) : 136.f;
+        for (int t = 0; t < T; ++t)
 #pragma unroll
-          for (int t = 0; t < T; ++t) acc[i][t][e] += sc * (part[t][e] - zc * xs[t][e]);
-        }
+          for (int e = 0; e < E; ++e) acc[i][t][e] += sc * (part[t][e] - zc * xs[t][e]);
       }
     }
   };
-  Chunk c0, c1;
-  int kc = wid;
-  if (kc < a.chunks) load(kc, c0);
-  while (kc < a.chunks) {
-    if (kc + waves < a.chunks) load(kc + waves, c1);
-    compute(c0);
-    kc += waves;
-    if (kc >= a.chunks) break;
-    if (kc + waves < a.chunks) load(kc + waves, c0);
-    compute(c1);
-    kc += waves;
+  if (n > 0) {
+    Chunk c[DW];
+    Rows y[2];
+#pragma unroll
+    for (int u = 0; u < DW - 1; ++u) load_w(min(u, n - 1), c[u]);
+    load_x(0, y[0]);
+    int j = 0;
+    for (; j + 2 * DW - 1 <= n; j += DW) {  // (no load of these lies in a branch: each is waited for by count)
+#pragma unroll
+      for (int u = 0; u < DW; ++u) {
+        load_x(j + u + 1, y[(u + 1) & 1]);
+        load_w(j + u + DW - 1, c[(u + DW - 1) % DW]);
+        __builtin_amdgcn_sched_barrier(0);
+        compute(c[u], y[u & 1]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    for (; j < n; j += DW)
+#pragma unroll
+      for (int u = 0; u < DW; ++u)
+        if (j + u < n) {
+          if (j + u + 1 < n) load_x(j + u + 1, y[(u + 1) & 1]);
+          if (j + u + DW - 1 < n) load_w(j + u + DW - 1, c[(u + DW - 1) % DW]);
+          compute(c[u], y[u & 1]);
+        }
   }
-  // lane (q, r): rows 4 q + e of a tile, token r
+  // lane (q, r): tokens E q + e of row r
 #pragma unroll
   for (int i = 0; i < RT; ++i)
 #pragma unroll
-    for (int t = 0; t < T; ++t) *reinterpret_cast<f32x4*>(red + (((wid * RT + i) * T + t) * 16 + r) * 16 + 4 * q) = acc[i][t];
+    for (int t = 0; t < T; ++t)
+#pragma unroll
+      for (int e = 0; e < E; ++e) red[((wid * RT + i) * T + t) * (64 * E) + (E * q + e) * 16 + r] = acc[i][t][e];
   __syncthreads();
-  for (int o = threadIdx.x; o < RT * T * 256; o += blockDim.x) {
-    const int n = o & 15, i = (o >> 4) % RT, m = (o >> 4) / RT;  // rows of tiles next to each other, then tokens
-    const int row = 16 * (nt0 + i) + n, tok = m0 + m;
+  for (int o = threadIdx.x; o < RT * T * E * 64; o += blockDim.x) {
+    const int i = o / (T * E * 64), in = o % (T * E * 64);  // (in: token, then row)
+    const int row = 16 * (nt0 + i) + (o & 15), tok = m0 + (in >> 4);
     if (row >= a.N || tok >= a.M) continue;
     float sum = 0.f;
-    for (int w = 0; w < waves; ++w) sum += red[(((w * RT + i) * T + (m >> 4)) * 16 + (m & 15)) * 16 + n];
-    a.y[(int64_t)tok * a.ldy + row] = f32_to_bf16(sum);
+    for (int w = 0; w < waves; ++w) sum += red[w * (RT * T * E * 64) + o];
+    if (gridDim.z == 1) a.y[(int64_t)tok * a.ldy + row] = f32_to_bf16(sum);
+    else a.ws[((int64_t)blockIdx.z * a.M + tok) * a.N + row] = sum;
   }
 }
 
-template <int RT, int T, int GS, bool ZERO> int launch(const W4Args& a, int waves, hipStream_t st) {
-  const size_t lds = (size_t)waves * RT * T * 1024;
-  if (lds > 64 * 1024) return -3;
-  const dim3 grid(((a.N + 15) / 16 + RT - 1) / RT, (a.M + 16 * T - 1) / (16 * T));
-  w4_kernel<RT, T, GS, ZERO><<<grid, 64 * waves, lds, st>>>(a);
+// y = the splits' sums, in their order
+__global__ void __launch_bounds__(256) w4_sum_kernel(bf16_t* __restrict__ y, int64_t ldy, const float* __restrict__ ws, int M, int N, int splits) {
+  const int n = blockIdx.x * 256 + threadIdx.x, m = blockIdx.y;
+  if (n >= N) return;
+  float sum = 0.f;
+#pragma unroll 8
+  for (int s = 0; s < splits; ++s) sum += ws[((int64_t)s * M + m) * N + n];
+  y[(int64_t)m * ldy + n] = f32_to_bf16(sum);
+}
+
+template <int RT, int T, int E, int GS, bool ZERO> int launch(const W4Args& a, int waves, int splits, hipStream_t st) {
+  const size_t lds = (size_t)waves * RT * T * E * 256;
+  if (lds > 64 * 1024 || waves < 1 || waves > 8 || splits < 1 || (splits > 1 && a.ws == nullptr)) return -3;
+  const dim3 grid(((a.N + 15) / 16 + RT - 1) / RT, (a.M + 4 * E * T - 1) / (4 * E * T), splits);
+  w4_kernel<RT, T, E, GS, ZERO, 2><<<grid, 64 * waves, lds, st>>>(a);
+  if (splits > 1) w4_sum_kernel<<<dim3((a.N + 255) / 256, a.M), 256, 0, st>>>(a.y, a.ldy, a.ws, a.M, a.N, splits);
   return (int)hipGetLastError();
 }
 
-template <int RT, int T> int launch_group(const W4Args& a, int group, int waves, hipStream_t st) {
+template <int RT, int T, int E> int launch_group(const W4Args& a, int group, int waves, int splits, hipStream_t st) {
   const bool z = a.z != nullptr;
   switch (group) {
-    case 32: return z ? launch<RT, T, 1, true>(a, waves, st) : launch<RT, T, 1, false>(a, waves, st);
-    case 64: return z ? launch<RT, T, 2, true>(a, waves, st) : launch<RT, T, 2, false>(a, waves, st);
-    case 128: return z ? launch<RT, T, 4, true>(a, waves, st) : launch<RT, T, 4, false>(a, waves, st);
+    case 32: return z ? launch<RT, T, E, 1, true>(a, waves, splits, st) : launch<RT, T, E, 1, false>(a, waves, splits, st);
+    case 64: return z ? launch<RT, T, E, 2, true>(a, waves, splits, st) : launch<RT, T, E, 2, false>(a, waves, splits, st);
+    case 128: return z ? launch<RT, T, E, 4, true>(a, waves, splits, st) : launch<RT, T, E, 4, false>(a, waves, splits, st);
   }
   return -1;
 }
 
 }  // namespace
 
-extern "C" int dx_w4_gemm(void* y, int64_t ldy, const void* x, int64_t ldx, const void* w, const void* s, const void* z, int M, int N, int K,
-                          int group, hipStream_t stream) {
+extern "C" int dx_w4_gemm(void* y, int64_t ldy, const void* x, int64_t ldx, const void* w, const void* s, const void* z, float* ws, int M, int N, int K,
+                          int group, int waves, int rt, int splits, hipStream_t stream) {
   if (M < 0 || N < 1 || K < 32 || K % group || ldx % 8) return -1;
   if (M == 0) return 0;
   W4Args a{};
-  a.y = (bf16_t*)y, a.x = (const bf16_t*)x, a.w = (const raw4*)w, a.s = (const uint16_t*)s, a.z = (const uint8_t*)z;
+  a.y = (bf16_t*)y, a.ws = ws, a.x = (const bf16_t*)x, a.w = (const raw4*)w, a.s = (const uint16_t*)s, a.z = (const uint8_t*)z;
   a.ldy = ldy, a.ldx = ldx, a.M = M, a.N = N, a.K = K, a.chunks = (K + 127) / 128;
-  int waves = 8;
-  while (waves > 1 && waves > a.chunks) waves >>= 1;
-  if (M <= 16) return launch_group<1, 1>(a, group, waves, stream);
-  if (M <= 32) return launch_group<1, 2>(a, group, waves, stream);
-  return launch_group<1, 4>(a, group, waves, stream);
+#define DX_W4(T_, E_)                                                                        \
+  do {                                                                                       \
+    if (rt == 4) return launch_group<4, T_, E_>(a, group, waves, splits, stream);            \
+    if (rt == 2) return launch_group<2, T_, E_>(a, group, waves, splits, stream);            \
+    return launch_group<1, T_, E_>(a, group, waves, splits, stream);                         \
+  } while (0)
+  if (M <= 4) DX_W4(1, 1);
+  if (M <= 8) DX_W4(1, 2);
+  if (M <= 16) DX_W4(1, 4);
+  if (M <= 32) DX_W4(2, 4);
+  if (rt == 4) rt = 2;
+  if (rt == 2) return launch_group<2, 4, 4>(a, group, waves, splits, stream);
+  return launch_group<1, 4, 4>(a, group, waves, splits, stream);
+#undef DX_W4
 }

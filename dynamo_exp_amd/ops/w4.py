@@ -17,19 +17,23 @@ MAX_ROWS = 256
 class W4Weight(NamedTuple):
     """A weight [n, k] as the kernel reads it (:func:`w4_pack`): rows in tiles of 16, columns in chunks of 128."""
     packed: torch.Tensor  # int32 [n / 16, k / 128, 64, 4]: lane 16 q + r, word s: columns 32 s + 8 q .. of row r
-    scales: torch.Tensor  # bf16 [n / 16, k / group, 16]
+    scales: torch.Tensor  # bf16 [n / 16, k / 128, 16, groups of a chunk]
     zeros: torch.Tensor | None  # uint8, as scales: 128 + zero
     n: int
     k: int
     group: int
 
 
-def _tiles(t: torch.Tensor) -> torch.Tensor:
-    """[n, g] -> [n / 16, g, 16], rows that are none 0."""
+def _tiles(t: torch.Tensor, per: int) -> torch.Tensor:
+    """[n, groups] -> [n / 16, chunks, 16, per], `per` groups a chunk; rows and groups that are none 0."""
     n, g = t.shape
-    p = torch.zeros((-(-n // 16) * 16, g), dtype=t.dtype, device=t.device)
-    p[:n] = t
-    return p.view(-1, 16, g).transpose(1, 2).contiguous()
+    p = torch.zeros((-(-n // 16) * 16, -(-g // per) * per), dtype=t.dtype, device=t.device)
+    p[:n, :g] = t
+    return p.view(-1, 16, p.shape[1] // per, per).transpose(1, 2).contiguous()
+
+
+def _rows(t: torch.Tensor, n: int, groups: int) -> torch.Tensor:
+    return t.transpose(1, 2).reshape(16 * t.shape[0], -1)[:n, :groups]
 
 
 def w4_pack(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None, group: int) -> W4Weight:
@@ -53,7 +57,7 @@ def w4_pack(codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | Non
     for j in range(8):  # column 2 i in nibble i, 2 i + 1 in nibble 4 + i
         word |= c[..., j].to(torch.int32) << (4 * (j // 2 + 4 * (j % 2)))
     packed = word.reshape(n16, k128, 64, 4).contiguous()
-    return W4Weight(packed, _tiles(scales), None if zeros is None else _tiles(zeros + 128), n, k, group)
+    return W4Weight(packed, _tiles(scales, 128 // group), None if zeros is None else _tiles(zeros + 128, 128 // group), n, k, group)
 
 
 def w4_quant(w: torch.Tensor, group: int = 128, symmetric: bool = True) -> W4Weight:
@@ -80,9 +84,31 @@ def w4_unpack(weight: W4Weight) -> torch.Tensor:
     w = p.view(n16, k128, 4, 16, 4, 1).expand(n16, k128, 4, 16, 4, 8)
     shift = torch.tensor([4 * (j // 2 + 4 * (j % 2)) for j in range(8)], dtype=torch.int32, device=p.device)
     c = ((w >> shift) & 15).permute(0, 3, 1, 4, 2, 5).reshape(n16 * 16, k128 * 128)[: weight.n, : weight.k].float()
-    rows = lambda t: t.transpose(1, 2).reshape(n16 * 16, -1)[: weight.n].float().repeat_interleave(weight.group, 1)  # noqa: E731
+    rows = lambda t: _rows(t, weight.n, weight.k // weight.group).float().repeat_interleave(weight.group, 1)  # noqa: E731
     zeros = 8.0 if weight.zeros is None else rows(weight.zeros) - 128
     return (c - zeros) * rows(weight.scales)
+
+
+def _shape(m: int, n: int, k: int) -> tuple[int, int, int]:
+    """(waves of a workgroup, 16-row tiles of weights a wave, workgroups that K is split over).  Tiles share x's way from L2, but need
+    workgroups enough for 256 CUs; us with 1, 2 and 4 tiles, groups of 128, one row: 4096 x 4096 (256 tiles of rows) 4.4, 5.0, -;
+    6144 x 4096 6.3, 5.2, 7.2; 28672 x 4096 13.9, 13.3, 12.4.  More than 8 rows of a long K take two tiles and halve K: 16 rows of
+    4096 x 14336 18.2 -> 12.9 (8 rows 10.9, 10.8).  Few rows of weights split K until there are 256 workgroups or a wave has its one
+    chunk: 17 x 16000 26 -> 4.6, 1000 x 8192 11 -> 5.3."""
+    tiles, chunks = -(-n // 16), -(-k // 128)
+    rt = 4 if tiles >= 1024 else 2 if tiles >= 384 or m > 16 else 1
+    splits = 1
+    if tiles < 512 and (m > 16 or (m > 8 and k >= 8192)):
+        rt = splits = 2
+    groups = -(-tiles // rt)
+    if groups < 128:
+        splits = max(splits, min(chunks // 8, 256 // groups))
+    waves = 8
+    while waves > 1 and waves * splits > chunks:
+        waves //= 2
+    if waves * splits > chunks:
+        splits = 1
+    return waves, rt, splits
 
 
 def w4_linear(x: torch.Tensor, weight: W4Weight, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -106,7 +132,9 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, out: torch.Tensor | None = None
         out = torch.empty((m, weight.n), dtype=x.dtype, device=x.device)
     elif out.shape != (m, weight.n) or out.dtype != x.dtype or out.device != x.device or (m and out.stride(1) != 1):
         raise ValueError("w4_linear: bad out tensor")
+    waves, rt, splits = _shape(m, weight.n, weight.k)
+    ws = torch.empty(splits * m * weight.n, dtype=torch.float32, device=x.device) if splits > 1 and m else None
     _native.kernels().w4_gemm(out.data_ptr(), out.stride(0), x.data_ptr(), x.stride(0) if m > 1 else 0, weight.packed.data_ptr(),
-                              weight.scales.data_ptr(), 0 if weight.zeros is None else weight.zeros.data_ptr(), m, weight.n, weight.k, weight.group,
+                              weight.scales.data_ptr(), 0 if weight.zeros is None else weight.zeros.data_ptr(), 0 if ws is None else ws.data_ptr(), m, weight.n, weight.k, weight.group, waves, rt, splits,
                               torch._C._cuda_getCurrentRawStream(dev))
     return out

@@ -130,7 +130,9 @@ def test_quantised_weights_are_near(symmetric):
     w[3, :64] = 0
     q = ops.w4_quant(w, 64, symmetric)
     s = ops.w4_unpack(q)
-    step = q.scales.transpose(1, 2).reshape(-1, 4)[:40].float().repeat_interleave(64, 1)
+    codes = torch.full((40, 256), 9 if symmetric else 1, dtype=torch.uint8)  # one step above zero: the step itself
+    one = q._replace(packed=ops.w4_pack(codes, torch.ones((40, 4)).bfloat16(), None, 64).packed, zeros=None if symmetric else torch.full_like(q.zeros, 128))
+    step = ops.w4_unpack(one)
     assert bool(((s - w).abs() <= step * (0.5 + (8 if symmetric else 30) * 2 ** -8) + (0 if symmetric else 0.5) * step).all())
     assert bool((s[3, :64] == 0).all())
 
