@@ -171,36 +171,68 @@ __device__ __forceinline__ void append_run(const AppendArgs& g, int64_t t0, int6
 template <int CODE, int PASSES, int WIN>
 __global__ void __launch_bounds__(kThreads) block_append_kernel(const AppendArgs g) {
   __shared__ float red[4];
+  const int lane = threadIdx.x & 63;
   if ((int)blockIdx.x < g.units_x) {  // units: windows x heads x (K, V)
     const int per = 2 * g.n_kv;
     const int64_t w0 = (int64_t)(blockIdx.x / per) * WIN;
     const int u = blockIdx.x % per, head = u >> 1, is_v = u & 1;
-#pragma unroll 1
-    for (int i = 0; i < WIN; ++i) {
-      const int64_t t = w0 + i;
-      if (t >= g.tokens) return;
-      const int64_t slot = g.slots[t];
-      if (slot < 0 || slot >= g.num_slots) continue;
-      const bool inside = t > 0 && (slot & ((1 << g.bs_shift) - 1)) != 0 && g.slots[t - 1] == slot - 1;
-      if (!inside) append_run<CODE, PASSES>(g, t, slot, head, is_v, red);
+    // the runs that begin in the window: every lane looks at one token and the one in front of it
+    int64_t slot = -1;
+    bool begins = false;
+    if (lane < WIN && w0 + lane < g.tokens) {
+      slot = g.slots[w0 + lane];
+      const int64_t before = g.slots[max(w0 + lane - 1, (int64_t)0)];
+      const bool inside = w0 + lane > 0 && (slot & ((1 << g.bs_shift) - 1)) != 0 && before == slot - 1;
+      begins = slot >= 0 && slot < g.num_slots && !inside;
+    }
+    for (uint64_t m = __builtin_amdgcn_ballot_w64(begins); m; m &= m - 1) {
+      const int i = __builtin_ctzll(m);
+      const uint32_t lo = __builtin_amdgcn_readlane((int)slot, i), hi = __builtin_amdgcn_readlane((int)(slot >> 32), i);
+      append_run<CODE, PASSES>(g, w0 + i, (int64_t)((uint64_t)hi << 32 | lo), head, is_v, red);
     }
     return;
   }
-  // Q of one token: n_q heads, eight lanes a head
-  const int64_t t = blockIdx.x - g.units_x;
+  // Q: a token a wave, eight lanes a head; a lane's cosines and sines serve its heads, four of them on their way at once
+  const int64_t t = (int64_t)(blockIdx.x - g.units_x) * 4 + (threadIdx.x >> 6);
+  if (t >= g.tokens) return;
   const float rsc = g.row_scale != nullptr ? g.row_scale[t] : 1.f;
   const float* cs = g.rotate_q ? table_row(g, t) : nullptr;
-  for (int h = threadIdx.x >> 3; h < g.n_q; h += kRows) {
-    const int j = threadIdx.x & 7;
-    float x[16];
-    load_row(g.q + t * g.stride + h * D, cs, rsc, j, x);
-    bf16_t* dst = g.q_out + t * g.q_out_stride + h * D + 8 * j;
+  const int j = lane & 7;
+  f32x4 c[2] = {{1.f, 1.f, 1.f, 1.f}, {1.f, 1.f, 1.f, 1.f}}, s[2] = {};
+  if (cs != nullptr) {
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      raw4 w;
+    for (int h = 0; h < 2; ++h) c[h] = *reinterpret_cast<const f32x4*>(cs + 8 * j + 4 * h), s[h] = *reinterpret_cast<const f32x4*>(cs + 64 + 8 * j + 4 * h);
+  }
+  const bf16_t* src = g.q + t * g.stride + 8 * j;
+  bf16_t* dst = g.q_out + t * g.q_out_stride + 8 * j;
+  constexpr int kHeads = 4;
+  for (int h0 = lane >> 3; h0 < g.n_q; h0 += 8 * kHeads) {
+    raw4 a[kHeads], b[kHeads];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = pack_bf16x2(x[8 * half + 2 * i], x[8 * half + 2 * i + 1]);
-      *reinterpret_cast<raw4*>(dst + 64 * half) = w;
+    for (int k = 0; k < kHeads; ++k) {
+      const int h = min(h0 + 8 * k, g.n_q - 1);
+      a[k] = *reinterpret_cast<const raw4*>(src + h * D);
+      b[k] = *reinterpret_cast<const raw4*>(src + h * D + 64);
+    }
+#pragma unroll
+    for (int k = 0; k < kHeads; ++k) {
+      raw4 oa, ob;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float u[2] = {bf16lo(a[k][i]) * rsc, bf16hi(a[k][i]) * rsc}, w[2] = {bf16lo(b[k][i]) * rsc, bf16hi(b[k][i]) * rsc};
+        float x[2], y[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float cc = c[i >> 1][2 * (i & 1) + e], ss = s[i >> 1][2 * (i & 1) + e];
+          x[e] = cs != nullptr ? u[e] * cc - w[e] * ss : u[e];
+          y[e] = cs != nullptr ? w[e] * cc + u[e] * ss : w[e];
+        }
+        oa[i] = pack_bf16x2(x[0], x[1]), ob[i] = pack_bf16x2(y[0], y[1]);
+      }
+      if (h0 + 8 * k < g.n_q) {
+        *reinterpret_cast<raw4*>(dst + (h0 + 8 * k) * D) = oa;
+        *reinterpret_cast<raw4*>(dst + (h0 + 8 * k) * D + 64) = ob;
+      }
     }
   }
 }
@@ -269,7 +301,7 @@ extern "C" int dx_block_append(const void* q, const void* k, const void* v, int6
   g.pos_i64 = pos_i64, g.rotate_q = rotate_q;
   const bool wide = tokens > 256;
   const int64_t units = slots ? (int64_t)(wide ? (tokens + 7) / 8 : tokens) * 2 * n_kv : 0;
-  const int64_t grid = units + (q_out ? tokens : 0);
+  const int64_t grid = units + (q_out ? (tokens + 3) / 4 : 0);
   if (grid == 0) return 0;
   if (grid > 0x7fffffff) return -2;
   g.units_x = (int)units;

@@ -177,9 +177,21 @@ def rope_cache(qkv, positions, cos_sin, slot_mapping, k_cache, v_cache, n_q, n_k
         if qkv.dim() != 2 or qkv.shape[1] != k_end + n_kv * head_dim or k_cache.shape[2] != block_size:
             raise ValueError(f"rope_cache: qkv {tuple(qkv.shape)} for {n_q} + 2 x {n_kv} heads of {head_dim}, blocks of {block_size}")
         T, rows = qkv.shape[0], qkv.stride(0)
-        heads = lambda lo, n: qkv.as_strided((T, n, head_dim), (rows, head_dim, qkv.stride(1)), qkv.storage_offset() + lo)  # noqa: E731
-        block8.append(heads(0, n_q), heads(q_end, n_kv), heads(k_end, n_kv), positions, cos_sin, slot_mapping, k_cache, v_cache, kv_scales,
-                      rotate_q, None if out is None else out.view(T, n_q, head_dim), row_scale)
+        if not qkv.is_cuda:
+            q, k, v = (t.unflatten(1, (-1, head_dim)) for t in (qkv[:, :q_end], qkv[:, q_end:k_end], qkv[:, k_end:]))
+            block8.append(q, k, v, positions, cos_sin, slot_mapping, k_cache, v_cache, kv_scales, rotate_q,
+                          None if out is None else out.view(T, n_q, head_dim), row_scale)
+            return qkv if out is None else out
+        to = qkv if out is None else out
+        if qkv.dtype != torch.bfloat16 or to.dtype != torch.bfloat16:
+            raise TypeError("rope_cache: rows are bfloat16")
+        if T and (qkv.stride(1) != 1 or (out is not None and (out.shape != (T, q_end) or out.stride(1) != 1))):
+            raise ValueError("rope_cache: rows of unit stride, out [T, n_q * head_dim]")
+        dev, p = k_cache.device, qkv.data_ptr()
+        if qkv.device != dev or to.device != dev or head_dim != block8.HEAD_DIM:
+            raise ValueError(f"rope_cache: rows on {qkv.device}, out on {to.device}, the cache on {dev}; heads of {head_dim}")
+        block8.append_rows(p, p + 2 * q_end, p + 2 * k_end, T, rows if T > 1 else 0, n_q, n_kv, to.data_ptr(), to.stride(0) if T > 1 else 0,
+                           positions, cos_sin, slot_mapping, k_cache, v_cache, kv_scales, rotate_q, row_scale)
         return qkv if out is None else out
     if row_scale is not None:
         assert not isinstance(qkv, SplitK), "row_scale needs a finished projection row"
@@ -723,7 +735,7 @@ def kv_dequant_scratch(k_cache, v_cache, block_tables, ctx_lens, kv_scales=(1.0,
               torch.empty((cap, H, BS, D), dtype=torch.bfloat16, device=k_cache.device),
               torch.arange(cap, dtype=torch.int32, device=k_cache.device))
         _KV_SCRATCH[key] = ws
-    ks, vs = ws[0][:max(n, 1)], ws[1][:max(n, 1)]
+    ks, vs = (ws[0], ws[1]) if ws[0].shape[0] == n else (ws[0][:max(n, 1)], ws[1][:max(n, 1)])
     table = scratch[0] if scratch is not None else ws[2][:n].view(nseq, maxb)
     assert block_tables.dtype == torch.int32 and ctx_lens.dtype == torch.int32 and table.dtype == torch.int32
     assert table.shape == (nseq, maxb) and table.is_contiguous()

@@ -20,7 +20,7 @@ from . import reference as ref
 
 HEAD_DIM = 128
 CODES = {torch.int8: 0, torch.float8_e4m3fn: 1}
-MAX_BLOCK = 128  # tokens of a block
+BLOCKS = (16, 32, 64, 128)  # tokens of a block
 MAX_GROUP = 16  # query heads per key/value head, decode
 
 
@@ -56,11 +56,12 @@ def _check_cache(k, v, kv_scales):
         raise ValueError(f"block-scaled cache: codes {tuple(k.shape)} {tuple(v.shape)}, scales {tuple(ks.shape)} {tuple(vs.shape)}")
     if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
         raise ValueError("block-scaled cache: codes and scales are contiguous")
-    if d != HEAD_DIM or bs < 16 or bs > MAX_BLOCK or bs & (bs - 1):
+    if d != HEAD_DIM or bs not in BLOCKS:
         raise ValueError(f"block-scaled cache: heads of {HEAD_DIM}, blocks of 16, 32, 64 or 128 tokens; got {d} and {bs}")
-    if k.data_ptr() % 16 or v.data_ptr() % 16:
+    if (k.data_ptr() | v.data_ptr()) % 16:
         raise ValueError("block-scaled cache: codes are 16-byte aligned")
-    if not k.device == v.device == ks.device == vs.device:
+    dev = k.device
+    if v.device != dev or ks.device != dev or vs.device != dev:
         raise ValueError("block-scaled cache: codes and scales on one device")
 
 
@@ -85,44 +86,53 @@ def append(q, k, v, positions, cos_sin, slot_mapping, k_cache, v_cache, kv_scale
     Two runs of tokens into one block in one call are not ordered; rows that no token went into keep their codes."""
     if not k.is_cuda:
         return ref.block_append(q, k, v, positions, cos_sin, slot_mapping, k_cache, v_cache, kv_scales, rotate_q, q_out, row_scale)
-    nb, hkv, bs, d = k_cache.shape
-    T = k.shape[0]
+    T, hkv, d = k.shape
     if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or (q is not None and q.dtype != torch.bfloat16):
         raise TypeError("append: q, k, v are bfloat16")
-    if k.shape != (T, hkv, d) or v.shape != k.shape or (q is not None and (q.dim() != 3 or q.shape[0] != T or q.shape[2] != d)):
-        raise ValueError(f"append: k {tuple(k.shape)}, v {tuple(v.shape)}, cache {tuple(k_cache.shape)}")
+    if v.shape != k.shape or (q is not None and (q.dim() != 3 or q.shape[0] != T or q.shape[2] != d)):
+        raise ValueError(f"append: k {tuple(k.shape)}, v {tuple(v.shape)}")
     stride = k.stride(0)
     for t in (q, k, v):
-        if t is not None and T > 0 and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != d) or (T > 1 and t.stride(0) != stride) or t.data_ptr() % 16):
-            raise ValueError("append: heads of a token behind one another, tokens equally far apart, 16-byte aligned")
-    if T > 1 and stride % 8:
-        raise ValueError("append: tokens lie a multiple of 8 elements apart")
+        if t is not None and T > 0 and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != d) or (T > 1 and t.stride(0) != stride)):
+            raise ValueError("append: heads of a token behind one another, tokens equally far apart")
+    q_out = q if q_out is None else q_out
+    if q is not None and (q_out.shape != q.shape or q_out.dtype != torch.bfloat16 or (T > 0 and (
+            q_out.stride(2) != 1 or (q.shape[1] > 1 and q_out.stride(1) != d)))):
+        raise ValueError("append: q_out is shaped as q, heads of a token behind one another")
+    _check_on(k_cache.device, q=q, k=k, v=v, q_out=q_out)
+    append_rows(0 if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), T, stride if T > 1 else 0, 0 if q is None else q.shape[1], hkv,
+                0 if q is None else q_out.data_ptr(), q_out.stride(0) if q is not None and T > 1 else 0, positions, cos_sin, slot_mapping, k_cache,
+                v_cache, kv_scales, rotate_q, row_scale)
+    return q_out
+
+
+def append_rows(qp, kp, vp, T, stride, nq, hkv, qop, q_out_stride, positions, cos_sin, slot_mapping, k_cache, v_cache, kv_scales, rotate_q, row_scale):
+    """append() on rows that the caller has looked at: bf16 at qp, kp, vp, tokens `stride` elements apart, on the cache's device."""
+    _check_cache(k_cache, v_cache, kv_scales)
+    nb, heads, bs, d = k_cache.shape
+    if heads != hkv:
+        raise ValueError(f"append: {hkv} heads, the cache has {heads}")
+    if (qp | kp | vp | qop) % 16 or stride % 8 or q_out_stride % 8:
+        raise ValueError("append: rows are 16-byte aligned")
+    dev = k_cache.device
     if cos_sin is not None:
         if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or cos_sin.shape[1] != d or not cos_sin.is_contiguous() or cos_sin.data_ptr() % 16:
             raise ValueError("append: cos_sin is [positions, 128] float32, contiguous")
-        if positions.dtype not in (torch.int64, torch.int32) or positions.shape != (T,) or not positions.is_contiguous():
+        if positions.dtype not in (torch.int64, torch.int32) or positions.dim() != 1 or positions.shape[0] != T or not positions.is_contiguous():
             raise ValueError("append: positions are [T] int64 or int32, contiguous")
-    if slot_mapping is not None and (slot_mapping.dtype != torch.int64 or slot_mapping.shape != (T,) or not slot_mapping.is_contiguous()):
-        raise ValueError("append: slot_mapping is [T] int64, contiguous")
-    if row_scale is not None and (row_scale.dtype != torch.float32 or row_scale.shape != (T,) or not row_scale.is_contiguous()):
-        raise ValueError("append: row_scale is [T] float32, contiguous")
-    _check_cache(k_cache, v_cache, kv_scales)
-    _check_on(k_cache.device, q=q, k=k, v=v, positions=positions if cos_sin is not None else None, cos_sin=cos_sin, slot_mapping=slot_mapping,
-              row_scale=row_scale, q_out=q_out)
-    nq = 0
-    if q is not None:
-        q_out = q if q_out is None else q_out
-        if q_out.shape != q.shape or q_out.dtype != torch.bfloat16 or (T > 0 and (
-                q_out.stride(2) != 1 or (q.shape[1] > 1 and q_out.stride(1) != d) or (T > 1 and q_out.stride(0) % 8) or q_out.data_ptr() % 16)):
-            raise ValueError("append: q_out is shaped as q, heads of a token behind one another, 16-byte aligned")
-        nq = q.shape[1]
+        if positions.device != dev or cos_sin.device != dev:
+            raise ValueError(f"append: positions on {positions.device}, cos_sin on {cos_sin.device}, the cache on {dev}")
+    if slot_mapping is not None and (slot_mapping.dtype != torch.int64 or slot_mapping.dim() != 1 or slot_mapping.shape[0] != T
+                                     or not slot_mapping.is_contiguous() or slot_mapping.device != dev):
+        raise ValueError("append: slot_mapping is [T] int64, contiguous, on the cache's device")
+    if row_scale is not None and (row_scale.dtype != torch.float32 or row_scale.shape != (T,) or not row_scale.is_contiguous() or row_scale.device != dev):
+        raise ValueError("append: row_scale is [T] float32, contiguous, on the cache's device")
     _native.kernels().block_append(
-        0 if q is None else q.data_ptr(), k.data_ptr(), v.data_ptr(), stride if T > 1 else 0, 0 if q is None else q_out.data_ptr(),
-        q_out.stride(0) if q is not None and T > 1 else 0, positions.data_ptr() if cos_sin is not None else 0,
+        qp, kp, vp, stride, qop, q_out_stride, positions.data_ptr() if cos_sin is not None else 0,
         int(cos_sin is not None and positions.dtype == torch.int64), 0 if cos_sin is None else cos_sin.data_ptr(),
         0 if row_scale is None else row_scale.data_ptr(), 0 if slot_mapping is None else slot_mapping.data_ptr(), k_cache.data_ptr(),
-        v_cache.data_ptr(), kv_scales[0].data_ptr(), kv_scales[1].data_ptr(), T, nq, hkv, d, bs, nb, int(rotate_q), CODES[k_cache.dtype], _stream(k))
-    return q_out
+        v_cache.data_ptr(), kv_scales[0].data_ptr(), kv_scales[1].data_ptr(), T, nq, hkv, d, bs, nb, int(rotate_q), CODES[k_cache.dtype],
+        _stream(k_cache))
 
 
 def dequant(k_cache, v_cache, kv_scales, block_tables, ctx_lens, k_out, v_out, table):
