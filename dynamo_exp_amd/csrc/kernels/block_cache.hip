@@ -11,8 +11,10 @@
 //
 // A unit is one run's K or V of one head, in a workgroup: eight lanes a row, each with eight columns of either half, the rows
 // of a block in registers between the maximum and the rounding, so each value is read once.  Runs are found where the slots
-// stop rising by one: a window of WIN tokens is looked over at once, and the workgroup takes the runs that begin in it (WIN 1
-// for decode steps, whose tokens all begin one; 8 for prompts, where most windows have none).
+// stop rising by one: a workgroup looks a window of tokens over at once and takes the runs that begin in it, those of at most
+// eight rows (decode steps') a wave each, side by side.  Windows of 32 tokens, 4 where tokens are few: a window in which no run
+// begins costs its workgroup a launch and a load, 1 us of a CU's five places (6520 tokens of 8 heads in blocks of 64, windows of 8
+// and no runs a wave: 25 us for K and V; Q, which is a copy, 19).
 #include "block8.h"
 
 namespace {
@@ -60,39 +62,18 @@ struct AppendArgs {
   float *k_scales, *v_scales;
   int64_t stride, q_out_stride;
   int64_t num_slots;
-  int tokens, n_q, n_kv, bs_shift, pos_i64, rotate_q, units_x;
+  int tokens, n_q, n_kv, bs_shift, pos_i64, rotate_q, units_x, window;
 };
 
-// columns 8 j .. + 7 and 64 + 8 j .. of a row, rotated (cs: the position's row of the table) and scaled
-__device__ __forceinline__ void load_row(const bf16_t* p, const float* cs, float rsc, int j, float (&x)[16]) {
-  const raw4 a = *reinterpret_cast<const raw4*>(p + 8 * j), b = *reinterpret_cast<const raw4*>(p + 64 + 8 * j);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    x[2 * i] = bf16lo(a[i]) * rsc, x[2 * i + 1] = bf16hi(a[i]) * rsc;
-    x[8 + 2 * i] = bf16lo(b[i]) * rsc, x[9 + 2 * i] = bf16hi(b[i]) * rsc;
-  }
-  if (cs != nullptr) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const f32x4 c = *reinterpret_cast<const f32x4*>(cs + 8 * j + 4 * h), s = *reinterpret_cast<const f32x4*>(cs + 64 + 8 * j + 4 * h);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float u = x[4 * h + i], w = x[8 + 4 * h + i];
-        x[4 * h + i] = u * c[i] - w * s[i];
-        x[8 + 4 * h + i] = w * c[i] + u * s[i];
-      }
-    }
-  }
+__device__ __forceinline__ int64_t position(const AppendArgs& g, int64_t t) {
+  return g.pos_i64 ? static_cast<const int64_t*>(g.positions)[t] : (int64_t)static_cast<const int32_t*>(g.positions)[t];
 }
 
-__device__ __forceinline__ const float* table_row(const AppendArgs& g, int64_t t) {
-  if (g.cos_sin == nullptr) return nullptr;
-  return g.cos_sin + (g.pos_i64 ? static_cast<const int64_t*>(g.positions)[t] : (int64_t)static_cast<const int32_t*>(g.positions)[t]) * D;
-}
-
-template <int CODE, int PASSES>
-__device__ __forceinline__ void append_run(const AppendArgs& g, int64_t t0, int64_t slot, int head, int is_v, float* red) {
-  const int bs = 1 << g.bs_shift, lane = threadIdx.x & 63, row = threadIdx.x >> 3, j = threadIdx.x & 7;
+// one run: by a workgroup, or (WAVE) n rows by a wave
+template <int CODE, int PASSES, bool WAVE>
+__device__ __forceinline__ void append_run(const AppendArgs& g, int64_t t0, int64_t slot, int n, int head, int is_v, float* red) {
+  constexpr int STEP = WAVE ? 8 : kRows;  // rows of a pass
+  const int bs = 1 << g.bs_shift, lane = threadIdx.x & 63, row = (WAVE ? lane : (int)threadIdx.x) >> 3, j = threadIdx.x & 7;
   const int64_t block = slot >> g.bs_shift;
   const int off = (int)(slot & (bs - 1));
   const int64_t at = block * g.n_kv + head;
@@ -100,23 +81,57 @@ __device__ __forceinline__ void append_run(const AppendArgs& g, int64_t t0, int6
   uint8_t* codes = (is_v ? g.v_codes : g.k_codes) + (at << g.bs_shift) * D + 8 * j;
   const float held = off > 0 ? *scale_at : 0.f;
   const float old = held > 0.f && held < INFINITY ? held : 0.f;
-  // the run's length: up to where the slots stop rising by one, or the block ends
-  int n = 0;
+  // the rows that may be the run's, asked for with what says how many are: 8 j .. + 7 and 64 + 8 j .. + 7 of a row a lane
+  const bf16_t* src = (is_v ? g.v : g.k) + t0 * g.stride + head * D + 8 * j;
+  const bool turn = !is_v && g.cos_sin != nullptr;
+  const int most = min(WAVE ? n : bs - off, (int)min(g.tokens - t0, (int64_t)kMostBlock));
+  raw4 lo[PASSES], hi[PASSES];
+  int64_t pos[PASSES];
+  float rsc[PASSES];
 #pragma unroll
-  for (int h = 0; h < kMostBlock / 64; ++h) {
-    const int i = 64 * h + lane;
-    const bool on = off + i < bs && t0 + i < g.tokens && g.slots[t0 + i] == slot + i;
-    const uint64_t m = __builtin_amdgcn_ballot_w64(!on);
-    if (n == 64 * h) n += m ? __builtin_ctzll(m) : 64;
+  for (int p = 0; p < PASSES; ++p) {
+    const int i = p * STEP + row;
+    if (i < most) {
+      lo[p] = *reinterpret_cast<const raw4*>(src + i * g.stride);
+      hi[p] = *reinterpret_cast<const raw4*>(src + i * g.stride + 64);
+      pos[p] = turn ? position(g, t0 + i) : 0;
+      rsc[p] = g.row_scale != nullptr ? g.row_scale[t0 + i] : 1.f;
+    }
   }
-  const bf16_t* src = (is_v ? g.v : g.k) + t0 * g.stride + head * D;
+  if constexpr (!WAVE) {  // the run's length: up to where the slots stop rising by one, or the block ends
+    n = 0;
+#pragma unroll
+    for (int h = 0; h < kMostBlock / 64; ++h) {
+      const int i = 64 * h + lane;
+      const bool on = i < most && g.slots[t0 + i] == slot + i;
+      const uint64_t m = __builtin_amdgcn_ballot_w64(!on);
+      if (n == 64 * h) n += m ? __builtin_ctzll(m) : 64;
+    }
+  }
   float x[PASSES][16];
   float amax = 0.f;
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
-    const int i = p * kRows + row;
+    const int i = p * STEP + row;
     if (i < n) {
-      load_row(src + i * g.stride, is_v ? nullptr : table_row(g, t0 + i), g.row_scale != nullptr ? g.row_scale[t0 + i] : 1.f, j, x[p]);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        x[p][2 * k] = bf16lo(lo[p][k]) * rsc[p], x[p][2 * k + 1] = bf16hi(lo[p][k]) * rsc[p];
+        x[p][8 + 2 * k] = bf16lo(hi[p][k]) * rsc[p], x[p][9 + 2 * k] = bf16hi(hi[p][k]) * rsc[p];
+      }
+      if (turn) {
+        const float* cs = g.cos_sin + pos[p] * D + 8 * j;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const f32x4 c = *reinterpret_cast<const f32x4*>(cs + 4 * h), s = *reinterpret_cast<const f32x4*>(cs + 64 + 4 * h);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float u = x[p][4 * h + k], w = x[p][8 + 4 * h + k];
+            x[p][4 * h + k] = u * c[k] - w * s[k];
+            x[p][8 + 4 * h + k] = w * c[k] + u * s[k];
+          }
+        }
+      }
 #pragma unroll
       for (int c = 0; c < 16; ++c) {
         const float a = fabsf(x[p][c]);
@@ -125,15 +140,17 @@ __device__ __forceinline__ void append_run(const AppendArgs& g, int64_t t0, int6
     }
   }
   amax = wave_reduce_max(amax);
-  if (lane == 0) red[threadIdx.x >> 6] = amax;
-  __syncthreads();  // (every wave has read the old scale by now)
-  amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  if constexpr (!WAVE) {
+    if (lane == 0) red[threadIdx.x >> 6] = amax;
+    __syncthreads();  // (every wave has read the old scale by now)
+    amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  }
   const float now = fmaxf(old, power_scale<CODE>(amax));
   const float inv = 1.f / now;
-  if (threadIdx.x == 0) *scale_at = now;
+  if ((WAVE ? lane : (int)threadIdx.x) == 0) *scale_at = now;
 #pragma unroll
   for (int p = 0; p < PASSES; ++p) {
-    const int i = p * kRows + row;
+    const int i = p * STEP + row;
     if (i < n) {
       uint8_t* dst = codes + (int64_t)(off + i) * D;
 #pragma unroll
@@ -150,7 +167,7 @@ __device__ __forceinline__ void append_run(const AppendArgs& g, int64_t t0, int6
   }
   if (off > 0 && now != held) {
     const float ratio = old / now;
-    for (int i = row; i < off; i += kRows) {
+    for (int i = row; i < off; i += STEP) {
       uint8_t* dst = codes + (int64_t)i * D;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -165,30 +182,45 @@ __device__ __forceinline__ void append_run(const AppendArgs& g, int64_t t0, int6
       }
     }
   }
-  __syncthreads();  // (the sums' place is used again by the next run)
+  if constexpr (!WAVE) __syncthreads();  // (the maxima's place is used again by the next run)
 }
 
-template <int CODE, int PASSES, int WIN>
+template <int CODE, int PASSES>
 __global__ void __launch_bounds__(kThreads) block_append_kernel(const AppendArgs g) {
   __shared__ float red[4];
   const int lane = threadIdx.x & 63;
   if ((int)blockIdx.x < g.units_x) {  // units: windows x heads x (K, V)
     const int per = 2 * g.n_kv;
-    const int64_t w0 = (int64_t)(blockIdx.x / per) * WIN;
+    const int64_t w0 = (int64_t)(blockIdx.x / per) * g.window;
     const int u = blockIdx.x % per, head = u >> 1, is_v = u & 1;
-    // the runs that begin in the window: every lane looks at one token and the one in front of it
+    // every lane looks at one token and the one in front of it, eight tokens past the window too: there its last runs may end
     int64_t slot = -1;
     bool begins = false;
-    if (lane < WIN && w0 + lane < g.tokens) {
+    if (lane <= g.window + 8 && w0 + lane < g.tokens) {
       slot = g.slots[w0 + lane];
       const int64_t before = g.slots[max(w0 + lane - 1, (int64_t)0)];
       const bool inside = w0 + lane > 0 && (slot & ((1 << g.bs_shift) - 1)) != 0 && before == slot - 1;
       begins = slot >= 0 && slot < g.num_slots && !inside;
     }
-    for (uint64_t m = __builtin_amdgcn_ballot_w64(begins); m; m &= m - 1) {
-      const int i = __builtin_ctzll(m);
+    // a run ends at the next one, at a token that has no place, or behind the last token
+    const uint64_t starts = __builtin_amdgcn_ballot_w64(begins), runs = starts & ((1ull << g.window) - 1);
+    const uint64_t ends = starts | __builtin_amdgcn_ballot_w64(lane <= g.window + 8 && (slot < 0 || slot >= g.num_slots));
+    auto slot_of = [&](int i) {
       const uint32_t lo = __builtin_amdgcn_readlane((int)slot, i), hi = __builtin_amdgcn_readlane((int)(slot >> 32), i);
-      append_run<CODE, PASSES>(g, w0 + i, (int64_t)((uint64_t)hi << 32 | lo), head, is_v, red);
+      return (int64_t)((uint64_t)hi << 32 | lo);
+    };
+    auto rows_of = [&](int i) {  // (more than eight where the window does not say)
+      const uint64_t next = i < 63 ? ends >> (i + 1) : 0;
+      return next ? __builtin_ctzll(next) + 1 : 64;
+    };
+    for (uint64_t m = runs; m; m &= m - 1) {
+      const int i = __builtin_ctzll(m);
+      if (rows_of(i) > 8) append_run<CODE, PASSES, false>(g, w0 + i, slot_of(i), 0, head, is_v, red);
+    }
+    int k = 0;
+    for (uint64_t m = runs; m; m &= m - 1) {
+      const int i = __builtin_ctzll(m), n = rows_of(i);
+      if (n <= 8 && (k++ & 3) == (int)(threadIdx.x >> 6)) append_run<CODE, 1, true>(g, w0 + i, slot_of(i), n, head, is_v, red);
     }
     return;
   }
@@ -196,7 +228,7 @@ __global__ void __launch_bounds__(kThreads) block_append_kernel(const AppendArgs
   const int64_t t = (int64_t)(blockIdx.x - g.units_x) * 4 + (threadIdx.x >> 6);
   if (t >= g.tokens) return;
   const float rsc = g.row_scale != nullptr ? g.row_scale[t] : 1.f;
-  const float* cs = g.rotate_q ? table_row(g, t) : nullptr;
+  const float* cs = g.rotate_q && g.cos_sin != nullptr ? g.cos_sin + position(g, t) * D : nullptr;
   const int j = lane & 7;
   f32x4 c[2] = {{1.f, 1.f, 1.f, 1.f}, {1.f, 1.f, 1.f, 1.f}}, s[2] = {};
   if (cs != nullptr) {
@@ -276,11 +308,6 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-template <int CODE, int PASSES> void launch_append(const AppendArgs& g, bool wide, unsigned grid, hipStream_t st) {
-  if (wide) block_append_kernel<CODE, PASSES, 8><<<grid, kThreads, 0, st>>>(g);
-  else block_append_kernel<CODE, PASSES, 1><<<grid, kThreads, 0, st>>>(g);
-}
-
 }  // namespace
 
 // code: 0 int8, 1 e4m3fn.  q, k, v: bf16 rows `stride` elements apart, 16-byte aligned; q_out nullptr: K and V alone;
@@ -299,17 +326,17 @@ extern "C" int dx_block_append(const void* q, const void* k, const void* v, int6
   g.tokens = tokens, g.n_q = n_q, g.n_kv = n_kv, g.bs_shift = __builtin_ctz((unsigned)block_size);
   g.num_slots = (int64_t)num_blocks << g.bs_shift;
   g.pos_i64 = pos_i64, g.rotate_q = rotate_q;
-  const bool wide = tokens > 256;
-  const int64_t units = slots ? (int64_t)(wide ? (tokens + 7) / 8 : tokens) * 2 * n_kv : 0;
+  g.window = tokens > 512 ? 32 : 4;
+  const int64_t units = slots ? (int64_t)((tokens + g.window - 1) / g.window) * 2 * n_kv : 0;
   const int64_t grid = units + (q_out ? (tokens + 3) / 4 : 0);
   if (grid == 0) return 0;
   if (grid > 0x7fffffff) return -2;
   g.units_x = (int)units;
 #define DX_APPEND(C)                                                                      \
   do {                                                                                    \
-    if (block_size <= 32) launch_append<C, 1>(g, wide, (unsigned)grid, stream);           \
-    else if (block_size == 64) launch_append<C, 2>(g, wide, (unsigned)grid, stream);      \
-    else launch_append<C, 4>(g, wide, (unsigned)grid, stream);                            \
+    if (block_size <= 32) block_append_kernel<C, 1><<<(unsigned)grid, kThreads, 0, stream>>>(g);           \
+    else if (block_size == 64) block_append_kernel<C, 2><<<(unsigned)grid, kThreads, 0, stream>>>(g);      \
+    else block_append_kernel<C, 4><<<(unsigned)grid, kThreads, 0, stream>>>(g);                            \
   } while (0)
   if (code == kE4m3) DX_APPEND(kE4m3);
   else DX_APPEND(kInt8);

@@ -660,3 +660,32 @@ def test_plan_covers_every_row_and_key():
                         assert len(j) == 1 and [m[2] for m in mine] == list(range(j[0][2], j[0][2] + j[0][3]))
                     else:
                         assert mine[0][2] == -1
+
+
+@pytest.mark.gpu
+@both
+def test_append_mixed_step(codes):
+    """Chunks and decode rows in one call of more than 512 tokens: runs of every length up to nine and whole blocks, at every place of a
+    window."""
+    spans = [(3, 700)] + [(16 * i + i % 7, 16 * i + i % 7 + 1 + i % 9) for i in range(60)] + [(640 + i, 641 + i) for i in range(9)]
+    check_append(append_case(codes, 16, spans, nkv=1, nq=1, seed=3, pad=5, device="cuda"))
+    check_append(append_case(codes, 64, spans, nkv=2, nq=2, seed=4, pad=0, device="cuda"))
+
+
+@pytest.mark.gpu
+@both
+def test_append_rows_without_a_place_between(codes):
+    """Rows that have no place lie between the others': they end runs, and nothing of them is written."""
+    dtype, bs, nkv = CODES[codes], 16, 2
+    none = [-1, 10 ** 12, 96, -7]  # the cache has 96 slots
+    slots = none[:1] + list(range(3, 8)) + none[:2] + list(range(16, 32)) + none[2:3] + [33] + none[3:] + list(range(48, 57)) + none + list(range(71, 79)) + none[1:2] + [80]
+    slots = torch.tensor(slots)
+    T = len(slots)
+    k = torch.randn((T, nkv, D), generator=torch.Generator().manual_seed(1)).bfloat16()
+    got = []
+    for device in ("cuda", "cpu"):
+        k8, v8, scales = block8.alloc(6, nkv, bs, dtype, device)
+        ops.kv_write(k.to(device), k.flip(1).contiguous().to(device), slots.to(device), k8, v8, bs, kv_scales=scales)
+        got.append([t.cpu() for t in (k8, v8, *scales)])
+    for a, b in zip(*got):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
