@@ -42,7 +42,7 @@ struct DecodeArgs {
 };
 
 template <int CODE>
-__global__ void __launch_bounds__(kThreads) block_decode_kernel(const DecodeArgs a) {
+__global__ void __launch_bounds__(kThreads, 3) block_decode_kernel(const DecodeArgs a) {
   constexpr float kRescale = 8.0f;  // the running maximum moves when a chunk's exceeds it by 2^8
   __shared__ __attribute__((aligned(16))) char image[4 * CH * D * 2];
   __shared__ float st_m[4 * 16], st_l[4 * 16];
