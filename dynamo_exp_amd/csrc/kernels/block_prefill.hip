@@ -1,16 +1,21 @@
 // Paged causal prompt attention (ragged chunks behind cached tokens, grouped heads of 128) over the 8-bit cache whose scales
 // belong to a block and head (block8.h), for gfx950:
-//   out[i, h] = sum_j p_j v_j,  p = softmax_j(scale q_i . k_j),  j <= position of i (causal) or j < ctx
-// with k_j, v_j the cache's values, rounded to bf16 where their scales are no powers of two.
+//   out[i, h] = sum_j p_j vs_j v_j,  p = softmax_j(scale ks_j (q_i . k_j)),  j <= position of i (causal) or j < ctx
+// with k_j, v_j the codes of token j and ks_j, vs_j the scales of its block.
 //
 // Bound by the matrix products of long chunks and by the cache's bytes of short ones.  A workgroup takes 32 rows a wave of one
 // key/value head, a row being one query head of one token (token-major: row = token G + head), so that chunks of few tokens fill
 // waves at any group size, and a wave's rows span few positions.  Tiles of 64 keys: their codes are asked for a tile ahead, 16
-// bytes a lane, and become bf16 in a swizzled double-buffered LDS image behind the tile's products (a workgroup widens a code once
-// for all its rows).  S^T = K Q^T and O^T = V^T P^T on 32 x 32 x 16 products: a lane's scores are one row's, the softmax is
-// lane-local but for one exchange between the halves, the weights are the second product's operand as they are, V is read
-// transposed, and the row sum is a product with ones (of the bf16 weights that the second product sees).  The running maximum
-// moves when a tile's exceeds it by 2^8.
+// bytes a lane, and become fp16 in a swizzled double-buffered LDS image behind the tile's products (a workgroup widens a code once
+// for all its rows, by 0.5 or 1.25 instructions).  S^T = K Q^T and O^T = V^T P^T on 32 x 32 x 16 products: a lane's scores are one
+// row's, the softmax is lane-local but for one exchange between the halves, the weights are the second product's operand as they are, V
+// is read transposed, and the row sum is a product with ones (of the fp16 weights that the second product sees).  The running maximum
+// moves when a tile's exceeds it by 2^8, and weights are held as 2^7 times themselves, 2^15 at most: fp16 rounds those over 2^-21 (of the
+// running maximum's) to 2^-11 of themselves, smaller ones to 2^-32.  Q is brought under 2 by a power of two a row (what lies 2^14 under the row's largest value loses digits).
+//
+// Scales stay out of the products: ks is a factor of the scores, and O is held in units of the tile's vs, changed when that changes.  In
+// blocks of 16 and 32 a tile has several: the scores take theirs group by group, V is widened in units of the tile's largest (fp16 holds a
+// code 2^-24 times that exactly).  A tile whose vs is 2^-80 of the unit in use adds nothing that fp32 would see, and is left out.
 //
 // Few rows behind many keys are split over the keys (the plan says where), each part leaves its sums in fp32, and a second kernel
 // joins them.
@@ -22,7 +27,9 @@ namespace {
 
 constexpr int D = 128, BQ = 32, BKV = 64;
 constexpr int kTileBytes = BKV * D * 2;
+constexpr float kRescale = 8.0f, kLift = 7.0f;
 constexpr int kItem = 6;  // seq, first row, first key, end of the keys, place of its sums (or -1), 0
+constexpr int kFewRows = 32;  // rows that block_rows_kernel takes
 constexpr int kJoin = 4;  // seq, first row, first place, places
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
@@ -37,40 +44,47 @@ struct PrefillArgs {
   const float *ks, *vs;
   const int *block_tables, *cu, *ctx_lens, *work;
   int64_t q_stride;
-  int bt_stride, bt_cols, n_kv, G, bs_shift, num_blocks, causal;
+  int bt_stride, bt_cols, n_kv, G, bs_shift, num_blocks, causal, tile;  // tile: rows of a place of sums
   float scale_log2e;
 };
 
-template <int CODE, int NW>
-__global__ void __launch_bounds__(64 * NW, 2) block_prefill_kernel(const PrefillArgs a) {
-  constexpr float kRescale = 8.0f;
-  constexpr int PIECES = 8 / NW;  // pieces of 8 rows of a tile that a wave brings
+// RW: row waves of 32 rows; KW: waves that share a tile's keys (1, or 2: 32 each); ONE: a tile's keys lie in one block
+template <int CODE, int RW, int KW, bool ONE>
+__global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const PrefillArgs a) {
+  constexpr int NW = RW * KW, PIECES = 8 / NW;  // pieces of 8 rows of a tile that a wave brings
+  constexpr int SUBS = 2 / KW;                  // 32-key pieces of a tile that a wave multiplies
+  constexpr int NG = ONE ? 1 : 4;               // scales of a tile
   __shared__ __attribute__((aligned(16))) char smem[2 * 2 * kTileBytes];
   const int* item = a.work + (int64_t)blockIdx.y * kItem;
   const int kvh = blockIdx.x, G = a.G;
   const int seq = __builtin_amdgcn_readfirstlane(item[0]), row0 = __builtin_amdgcn_readfirstlane(item[1]);
   const int key0 = __builtin_amdgcn_readfirstlane(item[2]), key1 = __builtin_amdgcn_readfirstlane(item[3]), place = __builtin_amdgcn_readfirstlane(item[4]);
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int rw = wid % RW, kw = wid / RW;
   const int r = lane & 31, h = lane >> 5;
+  const int* bt = a.block_tables + (int64_t)seq * a.bt_stride;
+  // the blocks of the tiles and their scales, 64 at a time, a lane each (a table's columns are all that may be read of it)
+  int first = key0 >> a.bs_shift, ids = bt[min(first + lane, a.bt_cols - 1)];
   const int q_start = __builtin_amdgcn_readfirstlane(a.cu[seq]), qlen = __builtin_amdgcn_readfirstlane(a.cu[seq + 1]) - q_start;
   const int ctx = __builtin_amdgcn_readfirstlane((int)min((int64_t)a.ctx_lens[seq], (int64_t)a.bt_cols << a.bs_shift));
+  const int last = max(ctx - 1, 0) >> a.bs_shift;
+  float ks_l, vs_l;
+  auto scales = [&]() __attribute__((always_inline)) {
+    ids = (unsigned)ids < (unsigned)a.num_blocks ? ids : 0;
+    ks_l = a.ks[(int64_t)ids * a.n_kv + kvh], vs_l = a.vs[(int64_t)ids * a.n_kv + kvh];
+  };
+  scales();
   const int pos0 = ctx - qlen, rows = qlen * G;
-  const int w0 = row0 + BQ * wid, f = w0 + r;
+  const int w0 = row0 + BQ * rw, f = w0 + r;
   const bool valid = f < rows;
   const int tok = f / G, hq = f - tok * G;
   const int my_pos = a.causal ? pos0 + tok : ctx - 1;
   const int wave_min = a.causal ? pos0 + w0 / G : ctx - 1;
   const int wave_max = w0 >= rows ? -1 : a.causal ? pos0 + min(w0 + BQ - 1, rows - 1) / G : ctx - 1;
-  const int wg_max = a.causal ? pos0 + min(row0 + BQ * NW - 1, rows - 1) / G : ctx - 1;
+  const int wg_max = a.causal ? pos0 + min(row0 + BQ * RW - 1, rows - 1) / G : ctx - 1;
   const int kv_end = min(min(key1, ctx), wg_max + 1);
   const int n_tiles = max(kv_end - key0 + BKV - 1, 0) / BKV;
 
-  u16x8 qf[8];
-  {
-    const bf16_t* qp = a.q + (int64_t)(q_start + tok) * a.q_stride + (int64_t)(kvh * G + hq) * D + 8 * h;
-#pragma unroll
-    for (int s = 0; s < 8; ++s) qf[s] = valid ? *reinterpret_cast<const u16x8*>(qp + 16 * s) : u16x8{{0, 0, 0, 0}};
-  }
   int koff[8], voff[4][2];
 #pragma unroll
   for (int s = 0; s < 8; ++s) koff[s] = tile_off(r, 2 * s + h);
@@ -84,140 +98,256 @@ __global__ void __launch_bounds__(64 * NW, 2) block_prefill_kernel(const Prefill
     }
   }
   // ---- a tile's codes: piece p of this wave is rows 8 (PIECES wid + p) .. + 7, a lane 16 columns of one of them
-  const int* bt = a.block_tables + (int64_t)seq * a.bt_stride;
-  const int last = max(ctx - 1, 0) >> a.bs_shift;
-  int first = -64, ids = 0;
   raw4 kr[PIECES], vr[PIECES];
-  float ksc[PIECES], vsc[PIECES];
+  float ks_next[NG], vs_next[NG];  // the scales of the tile on its way
   auto load = [&](int t) __attribute__((always_inline)) {
     const int j0 = key0 + t * BKV;
-    if (min((j0 + BKV - 1) >> a.bs_shift, last) - first >= 64) {  // 64 entries of the table at a time, a lane each
+    if (min((j0 + BKV - 1) >> a.bs_shift, last) - first >= 64) {
       first = j0 >> a.bs_shift;
-      const int id = bt[min(first + lane, last)];
-      ids = (unsigned)id < (unsigned)a.num_blocks ? id : 0;
+      ids = bt[min(first + lane, a.bt_cols - 1)];
+      scales();
     }
+    auto at_block = [&](int j) { return min(j >> a.bs_shift, last) - first; };
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
-      const int at = 8 * (PIECES * wid + p), j = j0 + at;
-      const int64_t block = (int64_t)__builtin_amdgcn_readlane(ids, min(j >> a.bs_shift, last) - first) * a.n_kv + kvh;
+      const int j = j0 + 8 * (PIECES * wid + p);
+      const int64_t block = (int64_t)__builtin_amdgcn_readlane(ids, at_block(j)) * a.n_kv + kvh;
       const int64_t base = ((block << a.bs_shift) + (j & ((1 << a.bs_shift) - 1)) + (lane >> 3)) * D + 16 * (lane & 7);
-      ksc[p] = a.ks[block], vsc[p] = a.vs[block];
       kr[p] = *reinterpret_cast<const raw4*>(a.k + base);
       vr[p] = *reinterpret_cast<const raw4*>(a.v + base);
-      if (j + (lane >> 3) >= ctx) kr[p] = vr[p] = raw4{0u, 0u, 0u, 0u};  // (whatever lies behind the context may be a NaN)
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const int i = at_block(j0 + 16 * g);
+      ks_next[g] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_l), i));
+      vs_next[g] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs_l), i));
     }
   };
-  auto store = [&](char* kb) __attribute__((always_inline)) {
+  auto top_scale = [&](const float (&vs)[NG]) {
+    if constexpr (ONE) return vs[0];
+    else return fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+  };
+  auto store = [&](char* kb, int t) __attribute__((always_inline)) {
+    const int j0 = key0 + t * BKV;
+    if (j0 + BKV > ctx) {  // (whatever lies behind the context may be a NaN)
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p)
+        if (j0 + 8 * (PIECES * wid + p) + (lane >> 3) >= ctx) kr[p] = vr[p] = raw4{0u, 0u, 0u, 0u};
+    }
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
-      const int row = 8 * (PIECES * wid + p) + (lane >> 3);
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const int to = tile_off(row, 2 * (lane & 7) + c);
-        const raw2 k0 = widen4_bf16<CODE, true>(kr[p][2 * c], ksc[p]), k1 = widen4_bf16<CODE, true>(kr[p][2 * c + 1], ksc[p]);
-        const raw2 v0 = widen4_bf16<CODE, true>(vr[p][2 * c], vsc[p]), v1 = widen4_bf16<CODE, true>(vr[p][2 * c + 1], vsc[p]);
-        *reinterpret_cast<raw4*>(kb + to) = raw4{k0[0], k0[1], k1[0], k1[1]};
-        *reinterpret_cast<raw4*>(kb + kTileBytes + to) = raw4{v0[0], v0[1], v1[0], v1[1]};
+      const int row = 8 * (PIECES * wid + p) + (lane >> 3), to = tile_off(row, 2 * (lane & 7)), to1 = tile_off(row, 2 * (lane & 7) + 1);
+      raw4 o[2];
+      widen16_f16<CODE, false>(kr[p], 1.f, o);
+      *reinterpret_cast<raw4*>(kb + to) = o[0];
+      *reinterpret_cast<raw4*>(kb + to1) = o[1];
+      if constexpr (ONE) {
+        widen16_f16<CODE, false>(vr[p], 1.f, o);
+      } else {
+        const int g = (PIECES * wid + p) >> 1;
+        const float mine = g == 0 ? vs_next[0] : g == 1 ? vs_next[NG > 1 ? 1 : 0] : g == 2 ? vs_next[NG > 2 ? 2 : 0] : vs_next[NG > 3 ? 3 : 0];
+        const float top = top_scale(vs_next);
+        widen16_f16<CODE, true>(vr[p], top > 0.f ? mine / top : 0.f, o);
       }
+      *reinterpret_cast<raw4*>(kb + kTileBytes + to) = o[0];
+      *reinterpret_cast<raw4*>(kb + kTileBytes + to1) = o[1];
     }
   };
+  if (n_tiles > 0) load(0);
 
+  // ---- Q in fp16, under 2; what a score is worth then
+  u16x8 qf[8];
+  float q_unit;
+  {
+    const bf16_t* qp = a.q + (int64_t)(q_start + tok) * a.q_stride + (int64_t)(kvh * G + hq) * D + 8 * h;
+    float amax = 0.f;
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      qf[s] = valid ? *reinterpret_cast<const u16x8*>(qp + 16 * s) : u16x8{{0, 0, 0, 0}};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) amax = fmaxf(fmaxf(amax, fabsf(bf16lo(qf[s].w[w]))), fabsf(bf16hi(qf[s].w[w])));
+    }
+    const float unit = unit_factor(halves_max(amax));
+#pragma unroll
+    for (int s = 0; s < 8; ++s)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) qf[s].w[w] = pack_f16x2(bf16lo(qf[s].w[w]) * unit, bf16hi(qf[s].w[w]) * unit);
+    q_unit = a.scale_log2e / unit;
+  }
   f32x16 o_acc[4], l_acc = f32x16{};
 #pragma unroll
   for (int i = 0; i < 4; ++i) o_acc[i] = f32x16{};
   float m_i = -1e30f;
-  const bf16x8_t kOnes = __builtin_bit_cast(bf16x8_t, u16x8{{0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u}});
-  const f32x2 sc2 = {a.scale_log2e, a.scale_log2e};
+  float ks_now[NG], vs_tile = 1.f, vs_unit = n_tiles > 0 ? top_scale(vs_next) : 1.f;
+  const f16x8 kOnes = __builtin_bit_cast(f16x8, u16x8{{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u}});
   auto vread = [&](const char* vb, int i) __attribute__((always_inline)) {  // columns 32 (i % 4) .. + 31 of keys 16 (i / 4) .. + 15
     const i16x4 lo = read_tr16((const lds_i16x4*)(vb + i / 4 * 4096 + voff[i % 4][0]));
     const i16x4 hi = read_tr16((const lds_i16x4*)(vb + i / 4 * 4096 + voff[i % 4][1]));
-    return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   };
-  auto compute = [&](const char* kb, int t) __attribute__((always_inline)) {
-    const int j0 = key0 + t * BKV;
+  constexpr int kAhead = 4;  // fragments asked for ahead of their products
+  auto compute = [&](const char* tile, int t) __attribute__((always_inline)) {
+    const int j0 = key0 + t * BKV + 32 * SUBS * kw;  // this wave's first key
     if (j0 > wave_max) return;
-    const bool live1 = j0 + 32 <= wave_max;
+    const char* kb = tile + 8192 * SUBS * kw;
+    const bool live1 = SUBS == 2 && j0 + 32 <= wave_max;
     f32x16 s0 = f32x16{}, s1 = f32x16{};
-    auto kread = [&](int i) __attribute__((always_inline)) { return __builtin_bit_cast(bf16x8_t, *reinterpret_cast<const raw4*>(kb + 8192 * (i >> 3) + koff[i & 7])); };
+    f16x8 kf[kAhead], vf[kAhead];
+    auto kread = [&](int i) __attribute__((always_inline)) { return __builtin_bit_cast(f16x8, *reinterpret_cast<const raw4*>(kb + 8192 * (i >> 3) + koff[i & 7])); };
 #pragma unroll
-    for (int s = 0; s < 8; ++s) s0 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kread(s), __builtin_bit_cast(bf16x8_t, qf[s]), s0, 0, 0, 0);
+    for (int i = 0; i < kAhead; ++i) kf[i] = kread(i);
+    __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      const f16x8 x = kf[s % kAhead];
+      if (SUBS == 2 || s + kAhead < 8) kf[s % kAhead] = kread(s + kAhead);
+      s0 = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, __builtin_bit_cast(f16x8, qf[s]), s0, 0, 0, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if (SUBS == 2 || s + kAhead < 8) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
     if (live1) {
 #pragma unroll
-      for (int s = 0; s < 8; ++s) s1 = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kread(8 + s), __builtin_bit_cast(bf16x8_t, qf[s]), s1, 0, 0, 0);
+      for (int s = 0; s < 8; ++s) {
+        const f16x8 x = kf[s % kAhead];
+        if (s + kAhead < 8) kf[s % kAhead] = kread(8 + s + kAhead);
+        s1 = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, __builtin_bit_cast(f16x8, qf[s]), s1, 0, 0, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (s + kAhead < 8) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
     }
-    if (j0 + BKV - 1 > wave_min || j0 + BKV > ctx) {  // the diagonal, or the context's end
+    const char* vb = tile + kTileBytes + 8192 * SUBS * kw;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) vf[i] = vread(vb, i);
+    // a score's worth: one factor a tile, or one each 16 keys
+    float sc = q_unit * ks_now[0];
+    if constexpr (!ONE) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float g0 = KW == 2 ? (kw ? ks_now[NG > 2 ? 2 + (i >> 3) : 0] : ks_now[NG > 1 ? i >> 3 : 0]) : ks_now[NG > 1 ? i >> 3 : 0];
+        s0[i] *= q_unit * g0;
+        if constexpr (SUBS == 2) s1[i] *= q_unit * ks_now[NG > 2 ? 2 + (i >> 3) : 0];
+      }
+      sc = 1.f;
+    }
+    if (j0 + 32 * SUBS - 1 > wave_min || j0 + 32 * SUBS > ctx) {  // the diagonal, or the context's end
       const int lim = min(my_pos, ctx - 1) - j0 - 4 * h;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int off = (i & 3) + 8 * (i >> 2);
         s0[i] = off > lim ? -INFINITY : s0[i];
-        s1[i] = off + 32 > lim ? -INFINITY : s1[i];
+        if constexpr (SUBS == 2) s1[i] = off + 32 > lim ? -INFINITY : s1[i];
       }
     }
-    float ta = fmaxf(s0[0], s1[0]), tb = fmaxf(s0[1], s1[1]);
+    float ta = s0[0], tb = s0[1];
+    if constexpr (SUBS == 2) ta = fmaxf(ta, s1[0]), tb = fmaxf(tb, s1[1]);
 #pragma unroll
     for (int i = 2; i < 16; i += 2) {
-      ta = fmaxf(fmaxf(ta, s0[i]), s1[i]);
-      tb = fmaxf(fmaxf(tb, s0[i + 1]), s1[i + 1]);
+      ta = fmaxf(ta, s0[i]), tb = fmaxf(tb, s0[i + 1]);
+      if constexpr (SUBS == 2) ta = fmaxf(ta, s1[i]), tb = fmaxf(tb, s1[i + 1]);
     }
-    const float t_s = halves_max(fmaxf(ta, tb)) * a.scale_log2e;
+    const float t_s = halves_max(fmaxf(ta, tb)) * sc;  // (scales are positive)
     const float m_new = t_s > m_i + kRescale ? t_s : m_i;
     const float alpha = fast_exp2(m_i - m_new);
     m_i = m_new;
-    const f32x2 nm2 = {-m_new, -m_new};
+    const float base = m_new - kLift;
     u16x8 pf[2][2];
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2)
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const int i = 8 * s2 + 2 * w;
-        const f32x2 a0 = f32x2{s0[i], s0[i + 1]} * sc2 + nm2;
-        const f32x2 a1 = f32x2{s1[i], s1[i + 1]} * sc2 + nm2;
-        pf[0][s2].w[w] = pack_bf16x2(fast_exp2(a0.x), fast_exp2(a0.y));
-        pf[1][s2].w[w] = pack_bf16x2(fast_exp2(a1.x), fast_exp2(a1.y));
+        pf[0][s2].w[w] = pack_f16x2(fast_exp2(s0[i] * sc - base), fast_exp2(s0[i + 1] * sc - base));
+        if constexpr (SUBS == 2) pf[1][s2].w[w] = pack_f16x2(fast_exp2(s1[i] * sc - base), fast_exp2(s1[i + 1] * sc - base));
       }
-    if (__builtin_amdgcn_ballot_w64(alpha != 1.f)) {
+    // O's unit: the tile's vs, but for one that is as good as nothing beside it
+    const bool no_v = vs_tile < vs_unit * 0x1p-80f;
+    float unit = 1.f;
+    if (!no_v && vs_tile != vs_unit) {
+      unit = vs_unit / vs_tile;
+      vs_unit = vs_tile;
+    }
+    if (unit != 1.f || __builtin_amdgcn_ballot_w64(alpha != 1.f)) {
+      const float both = alpha * unit;
 #pragma unroll
-      for (int dt = 0; dt < 4; ++dt) o_acc[dt] *= alpha;
+      for (int dt = 0; dt < 4; ++dt) o_acc[dt] *= both;
       l_acc *= alpha;
     }
-    const char* vb = kb + kTileBytes;
 #pragma unroll
-    for (int sub = 0; sub < 2; ++sub)
+    for (int sub = 0; sub < SUBS; ++sub)
       if (sub == 0 || live1) {
+        if (no_v) {
 #pragma unroll
-        for (int i = 8 * sub; i < 8 * sub + 8; ++i) {
-          const bf16x8_t p = __builtin_bit_cast(bf16x8_t, pf[sub][(i >> 2) & 1]);
-          o_acc[i & 3] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vread(vb, i), p, o_acc[i & 3], 0, 0, 0);
-          if ((i & 3) == 3) l_acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kOnes, p, l_acc, 0, 0, 0);
+          for (int s2 = 0; s2 < 2; ++s2) l_acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kOnes, __builtin_bit_cast(f16x8, pf[sub][s2]), l_acc, 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int i = 8 * sub; i < 8 * sub + 8; ++i) {
+            const f16x8 p = __builtin_bit_cast(f16x8, pf[sub][(i >> 2) & 1]), x = vf[i % kAhead];
+            if (i + kAhead < 8 * SUBS) vf[i % kAhead] = vread(vb, i + kAhead);
+            o_acc[i & 3] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p, o_acc[i & 3], 0, 0, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            if (i + kAhead < 8 * SUBS) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+            if ((i & 3) == 3) l_acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kOnes, p, l_acc, 0, 0, 0);
+          }
         }
       }
   };
+  auto turn_over = [&]() __attribute__((always_inline)) {  // the tile that was on its way is the tile in use
+#pragma unroll
+    for (int g = 0; g < NG; ++g) ks_now[g] = ks_next[g];
+    vs_tile = top_scale(vs_next);
+  };
 
   if (n_tiles > 0) {
-    load(0);
-    store(smem);
+    store(smem, 0);
+    turn_over();
   }
   __syncthreads();
   for (int t = 0; t < n_tiles; ++t) {
     char *now = smem + (t & 1) * 2 * kTileBytes, *next = smem + ((t + 1) & 1) * 2 * kTileBytes;
     if (t + 1 < n_tiles) load(t + 1);
     compute(now, t);
-    if (t + 1 < n_tiles) store(next);
+    if (t + 1 < n_tiles) {
+      store(next, t + 1);
+      turn_over();
+    }
     __syncthreads();
   }
 
   // ---- lane (r, h) holds columns 32 dt + 8 g + 4 h .. + 3 of its row
-  const float l_i = l_acc[0];
-  if (place >= 0) {  // (the sums as they are; rows that are none hold zeros)
-    const int64_t row = ((int64_t)place * a.n_kv + kvh) * (BQ * NW) + BQ * wid + r;
+  float l_i = l_acc[0];
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt) o_acc[dt] *= vs_unit;
+  if constexpr (KW == 2) {  // the second half of the waves hands its sums to the first
+    float* so = reinterpret_cast<float*>(smem) + rw * (BQ * D);  // [64 lanes] x 64 values, a lane's apart by 64 so that a wave's lie together
+    float* sml = reinterpret_cast<float*>(smem + RW * BQ * D * 4) + rw * 128;
+    if (kw) {
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) so[(dt * 16 + i) * 64 + lane] = o_acc[dt][i];
+      sml[lane] = m_i, sml[64 + lane] = l_i;
+    }
+    __syncthreads();
+    if (kw) return;
+    const float m2 = sml[lane], l2 = sml[64 + lane], M = fmaxf(m_i, m2), e1 = fast_exp2(m_i - M), e2 = fast_exp2(m2 - M);
 #pragma unroll
     for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<f32x4*>(a.ws_o + row * D + 32 * dt + 8 * g + 4 * h) =
-            f32x4{o_acc[dt][4 * g], o_acc[dt][4 * g + 1], o_acc[dt][4 * g + 2], o_acc[dt][4 * g + 3]};
-    if (h == 0) *reinterpret_cast<f32x2*>(a.ws_ml + row * 2) = f32x2{m_i, l_i};
+      for (int i = 0; i < 16; ++i) o_acc[dt][i] = e1 * o_acc[dt][i] + e2 * so[(dt * 16 + i) * 64 + lane];
+    l_i = e1 * l_i + e2 * l2;
+    m_i = M;
+  }
+  if (place >= 0) {  // the sums as they are
+    const int64_t row = ((int64_t)place * a.n_kv + kvh) * a.tile + BQ * rw + r;
+    if (valid) {
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<f32x4*>(a.ws_o + row * D + 32 * dt + 8 * g + 4 * h) =
+              f32x4{o_acc[dt][4 * g], o_acc[dt][4 * g + 1], o_acc[dt][4 * g + 2], o_acc[dt][4 * g + 3]};
+      if (h == 0) *reinterpret_cast<f32x2*>(a.ws_ml + row * 2) = f32x2{m_i, l_i};
+    }
     return;
   }
   const float inv_l = l_i != 0.f ? 1.f / l_i : 0.f;
@@ -238,10 +368,219 @@ __global__ void __launch_bounds__(64 * NW, 2) block_prefill_kernel(const Prefill
     }
 }
 
-// one row a wave: its parts' sums under a common maximum, over their common sum
+// Few rows (16 CG of a key/value head at most) behind their keys: a decode step's kernel with more columns.  Bound by the cache's bytes: the
+// waves of a workgroup take chunks of 32 keys in turn, each for all rows, with K and V on their way a chunk ahead and no barrier between
+// them (the tiles above would leave waves without rows, and stage for 64 rows what 128 could use).  16 x 16 x 32 products: rows are the
+// columns of S^T = K Q^T and O^T = V^T P^T; ks is a factor of the scores, vs of the weights (a lane's eight keys lie in one block); V
+// goes through a wave's own image in LDS.
+constexpr int CH = 32;
+__device__ __forceinline__ int vimg_off(int row, int ch) { return row * 256 + 16 * (ch ^ (((row & 3) << 2) | ((row >> 2) & 3))); }
+
+template <int CODE, int CG>
+__global__ void __launch_bounds__(256, 2) block_rows_kernel(const PrefillArgs a) {
+  __shared__ __attribute__((aligned(16))) char image[4 * CH * D * 2];
+  __shared__ float st_m[4 * 16 * CG], st_l[4 * 16 * CG];
+  const int* item = a.work + (int64_t)blockIdx.y * kItem;
+  const int kvh = blockIdx.x, G = a.G;
+  const int seq = __builtin_amdgcn_readfirstlane(item[0]), key0 = __builtin_amdgcn_readfirstlane(item[2]), key1 = __builtin_amdgcn_readfirstlane(item[3]);
+  const int place = __builtin_amdgcn_readfirstlane(item[4]);
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, r = lane & 15;
+  const int q_start = __builtin_amdgcn_readfirstlane(a.cu[seq]), qlen = __builtin_amdgcn_readfirstlane(a.cu[seq + 1]) - q_start;
+  const int ctx = __builtin_amdgcn_readfirstlane((int)min((int64_t)a.ctx_lens[seq], (int64_t)a.bt_cols << a.bs_shift));
+  const int rows = min(qlen * G, 16 * CG), pos0 = ctx - qlen;
+  const int p0 = key0, p1 = min(key1, ctx);
+  char* vimg = image + wid * (CH * D * 2);
+
+  raw4 qf[CG][4];
+  int lim[CG];  // the last key a column sees (columns behind the rows hold the last row, and go nowhere)
+#pragma unroll
+  for (int c = 0; c < CG; ++c) {
+    const int f = max(min(16 * c + r, rows - 1), 0), tok = f / G, hq = f - tok * G;
+    lim[c] = a.causal ? pos0 + tok : ctx - 1;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) qf[c][s] = *reinterpret_cast<const raw4*>(a.q + (int64_t)(q_start + tok) * a.q_stride + (int64_t)(kvh * G + hq) * D + 8 * (4 * g + s));
+  }
+  const int first_lim = a.causal ? pos0 : ctx - 1;  // keys up to here are seen by every row
+
+  const int* bt = a.block_tables + (int64_t)seq * a.bt_stride;
+  const int last = max(ctx - 1, 0) >> a.bs_shift;
+  int first = p0 >> a.bs_shift, ids;
+  auto fetch = [&]() {
+    const int id = bt[min(first + lane, last)];
+    ids = (unsigned)id < (unsigned)a.num_blocks ? id : 0;
+  };
+  fetch();
+  auto block_at = [&](int i) {
+    if (i - first >= 64) {  // (chunks only go up)
+      first = i;
+      fetch();
+    }
+    return __builtin_amdgcn_readlane(ids, max(i - first, 0));
+  };
+
+  f32x4 oacc[CG][8];
+  float m_i[CG], l_i[CG];
+#pragma unroll
+  for (int c = 0; c < CG; ++c) {
+    m_i[c] = -1e30f, l_i[c] = 0.f;
+#pragma unroll
+    for (int db = 0; db < 8; ++db) oacc[c][db] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const int n_chunks = max(p1 - p0 + CH - 1, 0) / CH;
+  raw4 kf[2][2];
+  raw2 vr[8];
+  float ks_l, vs_l;
+  auto load = [&](int c) {
+    const int cb = p0 + c * CH;
+    const int cb1 = cb + 16 < p1 ? cb + 16 : cb;
+    const int64_t row0 = (int64_t)block_at(cb >> a.bs_shift) * a.n_kv + kvh, row1 = (int64_t)block_at(cb1 >> a.bs_shift) * a.n_kv + kvh;
+    const int in = (1 << a.bs_shift) - 1;
+    const int64_t base0 = ((row0 << a.bs_shift) + (cb & in)) * D, base1 = ((row1 << a.bs_shift) + (cb1 & in)) * D;
+    const int64_t srow = g < 2 ? row0 : row1;
+    ks_l = a.ks[srow];
+    vs_l = a.vs[srow];
+#pragma unroll
+    for (int bb = 0; bb < 2; ++bb) {
+      const int t = 8 * (r >> 2) + 4 * bb + (r & 3);
+      const uint8_t* p = a.k + (t < 16 ? base0 : base1) + (t & 15) * D + 32 * g;
+      kf[bb][0] = *reinterpret_cast<const raw4*>(p);
+      kf[bb][1] = *reinterpret_cast<const raw4*>(p + 16);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) vr[k] = *reinterpret_cast<const raw2*>(a.v + (k < 4 ? base0 : base1) + (4 * (k & 3) + g) * D + 8 * r);
+  };
+  auto step = [&](auto more_, int c) {
+    constexpr bool more = decltype(more_)::value;
+    const int cb = p0 + c * CH;
+    const bool ragged = cb + CH > p1, masked = ragged || cb + CH - 1 > first_lim;
+    f32x4 sacc[CG][2];
+#pragma unroll
+    for (int bb = 0; bb < 2; ++bb) {
+#pragma unroll
+      for (int cg = 0; cg < CG; ++cg) sacc[cg][bb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const raw2 lo = widen4_bf16<CODE, false>(kf[bb][s >> 1][2 * (s & 1)], 1.f), hi = widen4_bf16<CODE, false>(kf[bb][s >> 1][2 * (s & 1) + 1], 1.f);
+#pragma unroll
+        for (int cg = 0; cg < CG; ++cg)
+          sacc[cg][bb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, raw4{lo[0], lo[1], hi[0], hi[1]}),
+                                                                 __builtin_bit_cast(bf16x8_t, qf[cg][s]), sacc[cg][bb], 0, 0, 0);
+      }
+    }
+    if (ragged) {  // (weights of 0 meet zeros: whatever lies behind the context may be a NaN)
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (cb + 4 * k + g >= p1) vr[k] = raw2{0u, 0u};
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const raw2 lo = widen4_bf16<CODE, false>(vr[k][0], 1.f), hi = widen4_bf16<CODE, false>(vr[k][1], 1.f);
+      *reinterpret_cast<raw4*>(vimg + vimg_off(4 * k + g, r)) = raw4{lo[0], lo[1], hi[0], hi[1]};
+    }
+    const float kscale = ks_l * a.scale_log2e, vscale = vs_l;
+    if constexpr (more) load(c + 4);
+    raw4 pf[CG];
+#pragma unroll
+    for (int cg = 0; cg < CG; ++cg) {
+      float t[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) t[j] = sacc[cg][j >> 2][j & 3] * kscale;
+      if (masked) {
+        const int end = min(lim[cg], p1 - 1);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[j] = cb + 8 * g + j > end ? -INFINITY : t[j];
+      }
+      float cmax = fmaxf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), fmaxf(fmaxf(t[4], t[5]), fmaxf(t[6], t[7])));
+      cmax = over_row_pairs(halves_max(cmax), [](float x, float y) { return fmaxf(x, y); });
+      const float m_new = cmax > m_i[cg] + kRescale ? cmax : m_i[cg];
+      const float alpha = fast_exp2(m_i[cg] - m_new);
+      m_i[cg] = m_new;
+      float ps = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float x = fast_exp2(t[2 * w] - m_new), y = fast_exp2(t[2 * w + 1] - m_new);
+        ps += x + y;
+        pf[cg][w] = pack_bf16x2(x * vscale, y * vscale);
+      }
+      if (ragged) {  // (a scale behind the context may be anything)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          if (cb + 8 * g + 2 * w >= p1) pf[cg][w] &= 0xffff0000u;
+          if (cb + 8 * g + 2 * w + 1 >= p1) pf[cg][w] &= 0x0000ffffu;
+        }
+      }
+      l_i[cg] = l_i[cg] * alpha + ps;
+      if (__builtin_amdgcn_ballot_w64(alpha != 1.f)) {
+#pragma unroll
+        for (int db = 0; db < 8; ++db) oacc[cg][db] *= alpha;
+      }
+    }
+#pragma unroll
+    for (int db = 0; db < 8; ++db) {
+      const int qq = r >> 2, pp = r & 3;
+      const i16x4 lo = read_tr16((const lds_i16x4*)(vimg + vimg_off(8 * g + qq, 2 * db + (pp >> 1)) + 8 * (pp & 1)));
+      const i16x4 hi = read_tr16((const lds_i16x4*)(vimg + vimg_off(8 * g + 4 + qq, 2 * db + (pp >> 1)) + 8 * (pp & 1)));
+      const bf16x8_t v = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+#pragma unroll
+      for (int cg = 0; cg < CG; ++cg) oacc[cg][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8_t, pf[cg]), oacc[cg][db], 0, 0, 0);
+    }
+  };
+  int c = wid;
+  if (c < n_chunks) {
+    load(c);
+    for (; c + 4 < n_chunks; c += 4) step(std::true_type{}, c);
+    step(std::false_type{}, c);
+  }
+
+  // the waves' (O, m, l), 16 rows at a time, each in its own image; lane (g, r) holds columns 16 db + 4 g .. of a row
+#pragma unroll
+  for (int cg = 0; cg < CG; ++cg) {
+    const float l_tot = over_row_pairs(halves_sum(l_i[cg]), [](float x, float y) { return x + y; });
+    if (g == 0) st_m[(wid * CG + cg) * 16 + r] = m_i[cg], st_l[(wid * CG + cg) * 16 + r] = l_tot;
+  }
+#pragma unroll
+  for (int cg = 0; cg < CG; ++cg) {
+    if (16 * cg >= rows) break;
+    if (cg) __syncthreads();
+    float* so = reinterpret_cast<float*>(vimg) + r * D + 4 * g;
+#pragma unroll
+    for (int db = 0; db < 8; ++db) *reinterpret_cast<f32x4*>(so + 16 * db) = oacc[cg][db];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * D / 4; i += 256) {
+      const int in = i / (D / 4), d = 4 * (i % (D / 4)), f = 16 * cg + in;
+      if (f >= rows) break;
+      float m[4], M = -1e30f, den = 0.f;
+      f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) M = fmaxf(M, m[w] = st_m[(w * CG + cg) * 16 + in]);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float e = fast_exp2(m[w] - M);
+        sum += e * *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(image + w * (CH * D * 2)) + in * D + d);
+        den += e * st_l[(w * CG + cg) * 16 + in];
+      }
+      if (place >= 0) {
+        const int64_t row = ((int64_t)place * a.n_kv + kvh) * kFewRows + f;
+        *reinterpret_cast<f32x4*>(a.ws_o + row * D + d) = sum;
+        if (d == 0) *reinterpret_cast<f32x2*>(a.ws_ml + row * 2) = f32x2{M, den};
+      } else {
+        const float inv = den != 0.f ? 1.f / den : 0.f;
+        const int tok = f / G, hq = f - tok * G;
+        *reinterpret_cast<uint2*>(a.out + ((int64_t)(q_start + tok) * a.n_kv * G + kvh * G + hq) * D + d) =
+            uint2{pack_bf16x2(sum[0] * inv, sum[1] * inv), pack_bf16x2(sum[2] * inv, sum[3] * inv)};
+      }
+    }
+  }
+}
+
+// One row a workgroup: its parts' sums under a common maximum, over their common sum.  Eight groups of 32 lanes x 4 columns take every
+// eighth part, two of them on their way at once.
 __global__ void __launch_bounds__(256) block_prefill_join_kernel(bf16_t* __restrict__ out, const float* __restrict__ ws_o, const float* __restrict__ ws_ml,
                                                                  const int* __restrict__ joins, const int* __restrict__ cu, int n_kv, int G, int tile) {
-  const int lane = threadIdx.x & 63, in = blockIdx.x * 4 + (threadIdx.x >> 6), kvh = blockIdx.y;
+  __shared__ __attribute__((aligned(16))) f32x4 other[8][D / 4];
+  __shared__ float dens[8];
+  const int lane = threadIdx.x & 63, grp = threadIdx.x >> 5, col = threadIdx.x & 31, in = blockIdx.x, kvh = blockIdx.y;
   const int* item = joins + (int64_t)blockIdx.z * kJoin;
   const int seq = item[0], f = item[1] + in, place = item[2], n = item[3];
   const int q_start = cu[seq], rows = (cu[seq + 1] - q_start) * G;
@@ -249,34 +588,43 @@ __global__ void __launch_bounds__(256) block_prefill_join_kernel(bf16_t* __restr
   const int64_t step = (int64_t)n_kv * tile, row = ((int64_t)place * n_kv + kvh) * tile + in;
   float M = -1e30f;
   for (int p = lane; p < n; p += 64) M = fmaxf(M, ws_ml[(row + p * step) * 2]);
-  M = wave_reduce_max(M);
   float den = 0.f;
-  f32x2 sum = {0.f, 0.f};
-#pragma unroll 4
-  for (int p = 0; p < n; ++p) {
-    const f32x2 ml = *reinterpret_cast<const f32x2*>(ws_ml + (row + p * step) * 2);
-    const f32x2 x = *reinterpret_cast<const f32x2*>(ws_o + (row + p * step) * D + 2 * lane);
-    const float w = fast_exp2(ml.x - M);
-    den += w * ml.y;
-    sum += w * x;
+  f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+  M = wave_reduce_max(M);
+  for (int p = grp; p < n; p += 16) {
+    const int p2 = min(p + 8, n - 1);
+    const f32x2 ml = *reinterpret_cast<const f32x2*>(ws_ml + (row + p * step) * 2), ml2 = *reinterpret_cast<const f32x2*>(ws_ml + (row + p2 * step) * 2);
+    const f32x4 x = *reinterpret_cast<const f32x4*>(ws_o + (row + p * step) * D + 4 * col), x2 = *reinterpret_cast<const f32x4*>(ws_o + (row + p2 * step) * D + 4 * col);
+    const float w = fast_exp2(ml.x - M), w2 = p + 8 < n ? fast_exp2(ml2.x - M) : 0.f;
+    den += w * ml.y + w2 * ml2.y;
+    sum += w * x + w2 * x2;
   }
+  other[grp][col] = sum;
+  if (col == 0) dens[grp] = den;
+  __syncthreads();
+  if (grp) return;
+#pragma unroll
+  for (int k = 1; k < 8; ++k) sum += other[k][col], den += dens[k];
   const float inv = den != 0.f ? 1.f / den : 0.f;
   const int tok = f / G, hq = f - tok * G;
-  reinterpret_cast<uint32_t*>(out + ((int64_t)(q_start + tok) * n_kv * G + kvh * G + hq) * D)[lane] = pack_bf16x2(sum.x * inv, sum.y * inv);
+  *reinterpret_cast<uint2*>(out + ((int64_t)(q_start + tok) * n_kv * G + kvh * G + hq) * D + 4 * col) =
+      uint2{pack_bf16x2(sum[0] * inv, sum[1] * inv), pack_bf16x2(sum[2] * inv, sum[3] * inv)};
 }
 
 }  // namespace
 
-// q [T, Hq, 128] rows q_stride apart (16-byte aligned); out [T, Hq, 128]; work [n_work][6], joins [n_joins][4] and the places of their
-// sums (ws_o [places, Hkv, 32 waves, 128], ws_ml [..., 2] fp32) as the plan says.  code: 0 int8, 1 e4m3fn.
-extern "C" int dx_block_prefill(void* out, float* ws_o, float* ws_ml, const void* q, int64_t q_stride, const void* k, const void* v, const float* ks,
-                                const float* vs, const int* block_tables, int bt_stride, int bt_cols, const int* cu, const int* ctx_lens,
-                                const int* work, int n_work, const int* joins, int n_joins, int waves, int n_q, int n_kv, int head_dim,
-                                int block_size, int num_blocks, float scale, int causal, int code, hipStream_t stream) {
+// q [T, Hq, 128] rows q_stride apart (16-byte aligned); out [T, Hq, 128]; work [n_work + n_few][6] (tiles, then sequences of few rows),
+// joins [n_joins + n_few_joins][4] and the places of their sums (ws_o [places, Hkv, tile, 128], ws_ml [..., 2] fp32; few: [places, Hkv,
+// 32, ...]) as the plan says; tile: rows of a work item (64, 128, 256); few_groups: 16s of rows (1, 2).  code: 0 int8, 1 e4m3fn.
+extern "C" int dx_block_prefill(void* out, float* ws_o, float* ws_ml, float* few_o, float* few_ml, const void* q, int64_t q_stride, const void* k,
+                                const void* v, const float* ks, const float* vs, const int* block_tables, int bt_stride, int bt_cols, const int* cu,
+                                const int* ctx_lens, const int* work, int n_work, int n_few, const int* joins, int n_joins, int n_few_joins, int tile,
+                                int few_groups, int n_q, int n_kv, int head_dim, int block_size, int num_blocks, float scale, int causal, int code,
+                                hipStream_t stream) {
   if (head_dim != D || block_size < 16 || (block_size & (block_size - 1)) || n_kv < 1 || n_kv > 65535 || n_q % n_kv || q_stride % 8 || bt_cols < 1 ||
-      (waves != 4 && waves != 8) || n_work > 65535 || n_joins > 65535)
+      (tile != 64 && tile != 128 && tile != 256) || (few_groups != 1 && few_groups != 2) || n_work > 65535 || n_few > 65535 || n_joins > 65535 ||
+      n_few_joins > 65535)
     return -1;
-  if (n_work == 0) return 0;
   PrefillArgs a{};
   a.out = (bf16_t*)out, a.ws_o = ws_o, a.ws_ml = ws_ml, a.q = (const bf16_t*)q;
   a.k = (const uint8_t*)k, a.v = (const uint8_t*)v, a.ks = ks, a.vs = vs;
@@ -284,16 +632,40 @@ extern "C" int dx_block_prefill(void* out, float* ws_o, float* ws_ml, const void
   a.q_stride = q_stride, a.bt_stride = bt_stride, a.bt_cols = bt_cols;
   a.n_kv = n_kv, a.G = n_q / n_kv, a.bs_shift = __builtin_ctz((unsigned)block_size), a.num_blocks = num_blocks, a.causal = causal;
   a.scale_log2e = scale * 1.4426950408889634f;
-  const dim3 grid(n_kv, n_work);
-#define DX_BP(C)                                                                       \
-  do {                                                                                 \
-    if (waves == 8) block_prefill_kernel<C, 8><<<grid, 512, 0, stream>>>(a);           \
-    else block_prefill_kernel<C, 4><<<grid, 256, 0, stream>>>(a);                      \
+  if (n_work) {
+    const dim3 grid(n_kv, n_work);
+    a.tile = tile;
+#define DX_BPT(C, ONE)                                                                         \
+  do {                                                                                         \
+    if (tile == 256) block_prefill_kernel<C, 8, 1, ONE><<<grid, 512, 0, stream>>>(a);          \
+    else if (tile == 128) block_prefill_kernel<C, 4, 1, ONE><<<grid, 256, 0, stream>>>(a);     \
+    else block_prefill_kernel<C, 2, 2, ONE><<<grid, 256, 0, stream>>>(a);                      \
   } while (0)
-  if (code == kE4m3) DX_BP(kE4m3);
-  else DX_BP(kInt8);
+#define DX_BP(C)                              \
+  do {                                        \
+    if (block_size >= BKV) DX_BPT(C, true);   \
+    else DX_BPT(C, false);                    \
+  } while (0)
+    if (code == kE4m3) DX_BP(kE4m3);
+    else DX_BP(kInt8);
 #undef DX_BP
-  if (n_joins)
-    block_prefill_join_kernel<<<dim3(8 * waves, n_kv, n_joins), 256, 0, stream>>>((bf16_t*)out, ws_o, ws_ml, joins, cu, n_kv, n_q / n_kv, 32 * waves);
+#undef DX_BPT
+    if (n_joins) block_prefill_join_kernel<<<dim3(tile, n_kv, n_joins), 256, 0, stream>>>(a.out, ws_o, ws_ml, joins, cu, n_kv, a.G, tile);
+  }
+  if (n_few) {
+    a.work = work + kItem * n_work, a.ws_o = few_o, a.ws_ml = few_ml;
+    const dim3 grid(n_kv, n_few);
+#define DX_BR(C)                                                                       \
+  do {                                                                                 \
+    if (few_groups == 1) block_rows_kernel<C, 1><<<grid, 256, 0, stream>>>(a);         \
+    else block_rows_kernel<C, 2><<<grid, 256, 0, stream>>>(a);                         \
+  } while (0)
+    if (code == kE4m3) DX_BR(kE4m3);
+    else DX_BR(kInt8);
+#undef DX_BR
+    if (n_few_joins)
+      block_prefill_join_kernel<<<dim3(16 * few_groups, n_kv, n_few_joins), 256, 0, stream>>>(a.out, few_o, few_ml, joins + kJoin * n_joins, cu, n_kv, a.G,
+                                                                                              kFewRows);
+  }
   return (int)hipGetLastError();
 }

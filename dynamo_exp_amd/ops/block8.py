@@ -210,11 +210,15 @@ def decode_parts(batch: int, n_kv: int, max_ctx: int) -> int:
 
 class PrefillPlan(NamedTuple):
     """What a step's prompt rows are cut into, for all of its layers (:func:`prefill_plan`)."""
-    work: torch.Tensor  # int32: n_work items of 6, then n_joins of 4
+    work: torch.Tensor  # int32: n_work + n_few items of 6, then n_joins + n_few_joins of 4
     n_work: int
+    n_few: int
     n_joins: int
+    n_few_joins: int
     places: int  # tiles of sums in the workspace
-    waves: int
+    few_places: int
+    tile: int  # rows of a work item
+    few_groups: int  # 16s of rows that the sequences of few rows have at most
     rows: int
     sequences: int
     n_q: int
@@ -223,44 +227,58 @@ class PrefillPlan(NamedTuple):
 
 
 PREFILL_WGS, PREFILL_TILES = 512, 4
+FEW_ROWS, FEW_WGS, FEW_KEYS = 32, 256, 256
 
 
 def prefill_plan(q_lens: list[int], ctx_lens: list[int], n_q: int, n_kv: int, device="cuda", causal: bool = True) -> PrefillPlan:
     """Cuts prompt chunks (q_lens new tokens each, the last of ctx_lens tokens) into work items for ``prefill_attention`` over a
-    block-scaled cache: tiles of query rows, heaviest first, and where those are too few for the chip, parts of their keys."""
+    block-scaled cache: tiles of query rows, heaviest first, and where those are too few for the chip, parts of their keys.  Sequences of
+    at most 32 rows a key/value head (new tokens times query heads per key/value head) go to a kernel of their own."""
     if len(q_lens) != len(ctx_lens) or any(q < 0 or c < q for q, c in zip(q_lens, ctx_lens)):
         raise ValueError(f"prefill_plan: {list(q_lens)} new tokens of {list(ctx_lens)}")
     if n_kv < 1 or n_q % n_kv:
         raise ValueError(f"prefill_plan: {n_q} query heads, {n_kv} key/value heads")
     g = n_q // n_kv
-    waves = 8 if n_kv * sum(-(-q * g // 256) for q in q_lens) >= PREFILL_WGS else 4
-    tile = 32 * waves
+    few = [s for s, ql in enumerate(q_lens) if 0 < ql * g <= FEW_ROWS]
+    many = [s for s, ql in enumerate(q_lens) if ql * g > FEW_ROWS]
+    count = lambda tile: n_kv * sum(-(-q_lens[s] * g // tile) for s in many)  # noqa: E731
+    tile = 256 if count(256) >= PREFILL_WGS else 128 if any(q_lens[s] * g > 64 for s in many) else 64
+
+    def cut(items, unit, per):
+        """items (units of keys, sequence, first row) -> work and joins: those of over 1.5 `per` units in parts of about `per`."""
+        work, joins, places = [], [], 0
+        for n, s, r0 in items:
+            parts = -(-n // per) if 2 * n > 3 * per else 1
+            each = -(-n // parts)
+            parts = -(-n // each)
+            if parts == 1:
+                work.append((n, [s, r0, 0, unit * n, -1, 0]))
+                continue
+            joins += [s, r0, places, parts]
+            for p in range(parts):
+                end = min((p + 1) * each, n)
+                work.append((end - p * each, [s, r0, unit * p * each, unit * end, places + p, 0]))
+            places += parts
+        if len(work) > 65535:
+            raise ValueError(f"prefill_plan: {len(work)} work items, at most 65535")
+        work.sort(key=lambda w: -w[0])
+        return [x for _, w in work for x in w], joins, places
+
     items = []  # key tiles, sequence, first row
-    for s, (ql, cl) in enumerate(zip(q_lens, ctx_lens)):
+    for s in many:
+        ql, cl = q_lens[s], ctx_lens[s]
         for r0 in range(0, ql * g, tile):
             seen = cl - ql + (min(r0 + tile, ql * g) - 1) // g + 1 if causal else cl
             items.append((-(-seen // 64), s, r0))
     total = sum(i[0] for i in items)
-    per = max(PREFILL_TILES, -(-total * n_kv // PREFILL_WGS)) if len(items) * n_kv < PREFILL_WGS else 1 << 30
-    work, joins, places = [], [], 0
-    for n, s, r0 in items:
-        parts = -(-n // per) if 2 * n > 3 * per else 1
-        each = -(-n // parts)
-        parts = -(-n // each)
-        if parts == 1:
-            work.append((n, [s, r0, 0, 64 * n, -1, 0]))
-            continue
-        joins += [s, r0, places, parts]
-        for p in range(parts):
-            end = min((p + 1) * each, n)
-            work.append((end - p * each, [s, r0, 64 * p * each, 64 * end, places + p, 0]))
-        places += parts
-    if len(work) > 65535:
-        raise ValueError(f"prefill_plan: {len(work)} work items, at most 65535")
-    work.sort(key=lambda w: -w[0])
-    flat = [x for _, w in work for x in w] + joins
-    return PrefillPlan(torch.tensor(flat or [0], dtype=torch.int32).to(device), len(work), len(joins) // 4, places, waves, sum(q_lens), len(q_lens), n_q, n_kv,
-                       causal)
+    work, joins, places = cut(items, 64, max(PREFILL_TILES, -(-total * n_kv // PREFILL_WGS)) if len(items) * n_kv < PREFILL_WGS else 1 << 30)
+    items = [(-(-ctx_lens[s] // 128), s, 0) for s in few]
+    total = sum(i[0] for i in items)
+    few_work, few_joins, few_places = cut(items, 128, max(FEW_KEYS // 128, -(-total * n_kv // FEW_WGS)))
+    flat = work + few_work + joins + few_joins
+    most = max([q_lens[s] * g for s in few], default=0)
+    return PrefillPlan(torch.tensor(flat or [0], dtype=torch.int32).to(device), len(work) // 6, len(few_work) // 6, len(joins) // 4, len(few_joins) // 4,
+                       places, few_places, tile, 1 if most <= 16 else 2, sum(q_lens), len(q_lens), n_q, n_kv, causal)
 
 
 def prefill(q, k_cache, v_cache, block_tables, cu_seqlens_q, ctx_lens, scale, out, plan, kv_scales, causal):
@@ -279,15 +297,18 @@ def prefill(q, k_cache, v_cache, block_tables, cu_seqlens_q, ctx_lens, scale, ou
         raise ValueError(f"prefill_attention: a plan of {plan.rows} rows, {plan.sequences} sequences, {plan.n_q} / {plan.n_kv} heads, causal "
                          f"{plan.causal} for {T}, {n}, {hq} / {hkv}, {causal}")
     _check_on(q.device, cu_seqlens_q=cu_seqlens_q, work=plan.work)
-    o = ml = 0
-    if plan.places:
-        sums = plan.places * hkv * 32 * plan.waves
-        ws = torch.empty(sums * (d + 2), dtype=torch.float32, device=q.device)
+    o = ml = few_o = few_ml = 0
+    tiles, few = plan.places * hkv * plan.tile, plan.few_places * hkv * FEW_ROWS
+    if tiles or few:
+        ws = torch.empty((tiles + few) * (d + 2), dtype=torch.float32, device=q.device)
         o = ws.data_ptr()
-        ml = o + 4 * sums * d
+        few_o = o + 4 * tiles * d
+        ml = few_o + 4 * few * d
+        few_ml = ml + 8 * tiles
     work = plan.work.data_ptr()
-    _native.kernels().block_prefill(out.data_ptr(), o, ml, q.data_ptr(), q.stride(0) if T > 1 else 0, k_cache.data_ptr(), v_cache.data_ptr(),
-                                    kv_scales[0].data_ptr(), kv_scales[1].data_ptr(), block_tables.data_ptr(), block_tables.stride(0),
-                                    block_tables.shape[1], cu_seqlens_q.data_ptr(), ctx_lens.data_ptr(), work, plan.n_work, work + 24 * plan.n_work,
-                                    plan.n_joins, plan.waves, hq, hkv, d, bs, nb, float(scale), int(causal), CODES[k_cache.dtype], _stream(q))
+    _native.kernels().block_prefill(out.data_ptr(), o, ml, few_o, few_ml, q.data_ptr(), q.stride(0) if T > 1 else 0, k_cache.data_ptr(),
+                                    v_cache.data_ptr(), kv_scales[0].data_ptr(), kv_scales[1].data_ptr(), block_tables.data_ptr(),
+                                    block_tables.stride(0), block_tables.shape[1], cu_seqlens_q.data_ptr(), ctx_lens.data_ptr(), work, plan.n_work,
+                                    plan.n_few, work + 24 * (plan.n_work + plan.n_few), plan.n_joins, plan.n_few_joins, plan.tile, plan.few_groups,
+                                    hq, hkv, d, bs, nb, float(scale), int(causal), CODES[k_cache.dtype], _stream(q))
     return out

@@ -267,10 +267,16 @@ def attention64(q, k8, v8, ks, vs, table, new, ctx, causal=True):
     return out, size
 
 
-def near(got, want, size, roundings):
+def fp16_floor(ctx, v8, vs):
+    """What weights that fp16 holds to 2^-32 of the largest may cost a row: each key's, times the largest value (read or not)."""
+    return 2.0 ** -32 * max(ctx) * float((v8.view(torch.uint8).view(v8.dtype).float().nan_to_num(0.0).abs().amax((1, 2, 3)) * vs.nan_to_num(0.0, 0.0, 0.0).amax(1)).max())
+
+
+def near(got, want, size, roundings, floor=0.0):
     """Weights rounded to bf16 `roundings` times (in the sum, and where the row sum is of the rounded ones), the result once; scores of
-    128 products in fp32, of size 30 at most here: 128 2^-24 30 < 2^-12 of a weight, twice."""
-    tol = (roundings * 2 ** -8 + 2 ** -11) * size + 2 ** -8 * want.abs() * 1.01
+    128 products in fp32, of size 30 at most here: 128 2^-24 30 < 2^-12 of a weight, twice.  Weights under 2^-126 are no normal numbers
+    and may be 0: at most 2^14 of them meet values of at most 2^11 here, 2^-101 in all."""
+    tol = (roundings * 2 ** -8 + 2 ** -11) * size + 2 ** -8 * want.abs() * 1.01 + 2 ** -101 + floor
     err = (got.double() - want).abs()
     assert bool((err <= tol).all()), float((err / tol.clamp(min=1e-300)).max())
 
@@ -388,13 +394,8 @@ def run_prefill(codes, nq, nkv, bs, new, ctx, seed=0, causal=True, planned=True,
     out = torch.full((T, nq, D), NAN, dtype=torch.bfloat16, device="cuda")
     r = ops.prefill_attention(*dev, SCALE, out, work=plan, kv_scales=tuple(on_gpu(ks, vs)), causal=causal)
     assert r is out
-    vals = (k8, v8, ks, vs)
-    if not pow2:  # the kernel's values are rounded to bf16
-        vals = [bits(c).view(c.dtype) for c in (k8, v8)] + [ks, vs]
-        kb, vb = ref.block_values(k8, ks).bfloat16(), ref.block_values(v8, vs).bfloat16()
-        vals = (kb, vb, torch.ones_like(ks), torch.ones_like(vs))
-    want, size = attention64(q, *vals, table, new, ctx, causal)
-    near(out.cpu(), want, size, 2)
+    want, size = attention64(q, k8, v8, ks, vs, table, new, ctx, causal)
+    near(out.cpu(), want, size, 2, fp16_floor(ctx, v8, vs))
     return plan
 
 
@@ -417,7 +418,7 @@ def test_prefill_heads(codes, nq, nkv):
 @both
 def test_prefill_tiles_of_eight_waves(codes):
     plan = run_prefill(codes, 32, 8, 64, [1100, 900, 1300, 1000], [1100, 1000, 1300, 1001], seed=4)
-    assert plan.waves == 8 and plan.places == 0
+    assert plan.tile == 256 and plan.places == 0
 
 
 @pytest.mark.gpu
@@ -440,6 +441,51 @@ def test_prefill_bidirectional_and_unplanned(codes):
 @both
 def test_prefill_scales_that_are_no_powers(codes):
     run_prefill(codes, 8, 2, 32, [90, 5], [90, 500], seed=7, pow2=False)
+
+
+@pytest.mark.gpu
+@both
+@pytest.mark.parametrize("bs", [16, 32, 64, 128])
+@pytest.mark.parametrize("new,ctx", [([200, 30], [700, 300]), ([8], [600])])
+def test_prefill_unlike_scales(codes, bs, new, ctx):
+    """Value scales up to 2^20 apart, from block to block and (small blocks) within a tile of keys; a block of zeros, whose scale is 0."""
+    nq, nkv = 8, 2
+    table, k8, v8, ks, vs = cache_of(codes, nkv, bs, ctx, 5, junk=False)
+    vs *= 2.0 ** torch.randint(-10, 11, vs.shape, generator=torch.Generator().manual_seed(1))
+    ks *= 2.0 ** torch.randint(-3, 2, ks.shape, generator=torch.Generator().manual_seed(2))
+    zero = int(table[0, 1])
+    bits(v8)[zero] = 0
+    vs[zero] = 0
+    T = sum(new)
+    q = torch.randn((T, nq, D), generator=torch.Generator().manual_seed(3)).bfloat16()
+    cu = torch.tensor([sum(new[:i]) for i in range(len(new) + 1)], dtype=torch.int32)
+    out = torch.empty((T, nq, D), dtype=torch.bfloat16, device="cuda")
+    dev = on_gpu(q, k8, v8, table, cu, torch.tensor(ctx, dtype=torch.int32))
+    ops.prefill_attention(*dev, SCALE, out, work=ops.prefill_plan(new, ctx, nq, nkv), kv_scales=tuple(on_gpu(ks, vs)))
+    near(out.cpu(), *attention64(q, k8, v8, ks, vs, table, new, ctx), 2, fp16_floor(ctx, v8, vs))
+
+
+@pytest.mark.gpu
+def test_long_flat_weights():
+    """40000 keys whose weights are alike but for one that is 2^15 times theirs: together the small ones are worth as much.  (Weights of
+    2^-15 are no normal numbers in fp16.)"""
+    nq, nkv, bs, ctx = 4, 1, 64, [40000]
+    table, k8, v8, ks, vs = cache_of("int8", nkv, bs, ctx, 5)
+    bits(k8)[:] = 0
+    ks[:] = 1.0
+    k8[int(table[0, 3]), 0, 5] = 1
+    for new in ([1], [12], [30]):
+        T = new[0]
+        q = torch.full((T, nq, D), 15 * math.log(2) / (D * SCALE), dtype=torch.float32).bfloat16()
+        cu = torch.tensor([0, T], dtype=torch.int32)
+        out = torch.empty((T, nq, D), dtype=torch.bfloat16, device="cuda")
+        dev = on_gpu(q, k8, v8, table, cu, torch.tensor(ctx, dtype=torch.int32))
+        scales = tuple(on_gpu(ks, vs))
+        ops.prefill_attention(*dev, SCALE, out, work=ops.prefill_plan(new, ctx, nq, nkv), kv_scales=scales)
+        near(out.cpu(), *attention64(q, k8, v8, ks, vs, table, new, ctx), 2)
+        if T == 1:
+            ops.decode_attention(dev[0], dev[1], dev[2], dev[3], dev[5], SCALE, out, None, kv_scales=scales)
+            near(out.cpu(), *attention64(q, k8, v8, ks, vs, table, new, ctx), 2)
 
 
 # ---------------------------------------------------------------- together
@@ -645,21 +691,39 @@ def test_plan_covers_every_row_and_key():
             new = torch.randint(0, 700, (n,), generator=g).tolist()
             ctx = [a + b for a, b in zip(new, torch.randint(0, 9000, (n,), generator=g).tolist())]
             p = ops.prefill_plan(new, ctx, nq, nkv, "cpu")
-            flat, G, tile = p.work.tolist(), nq // nkv, 32 * p.waves
-            items = [flat[6 * i:6 * i + 6] for i in range(p.n_work)]
-            joins = [flat[6 * p.n_work + 4 * i:][:4] for i in range(p.n_joins)]
-            places = sorted(w[4] for w in items if w[4] >= 0)
-            assert places == list(range(p.places)) and sum(j[3] for j in joins) == p.places
+            flat, G, tile = p.work.tolist(), nq // nkv, p.tile
+            n_items, n_joins = p.n_work + p.n_few, p.n_joins + p.n_few_joins
+            items = [flat[6 * i:6 * i + 6] for i in range(n_items)]
+            joins = [flat[6 * n_items + 4 * i:][:4] for i in range(n_joins)]
+            assert len(flat) == max(1, 6 * n_items + 4 * n_joins)
+            for w, j, places in ((items[:p.n_work], joins[:p.n_joins], p.places), (items[p.n_work:], joins[p.n_joins:], p.few_places)):
+                assert sorted(x[4] for x in w if x[4] >= 0) == list(range(places)) and sum(x[3] for x in j) == places
             for s, (ql, cl) in enumerate(zip(new, ctx)):
-                for r0 in range(0, ql * G, tile):
-                    mine = sorted(w[2:5] for w in items if w[0] == s and w[1] == r0)
-                    assert mine[0][0] == 0 and all(a[1] == b[0] and a[1] % 64 == 0 for a, b in zip(mine, mine[1:]))
-                    assert mine[-1][1] > cl - ql + (min(r0 + tile, ql * G) - 1) // G
+                few = 0 < ql * G <= block8.FEW_ROWS
+                assert not few or ql * G <= 16 * p.few_groups
+                w, j, step = (items[p.n_work:], joins[p.n_joins:], block8.FEW_ROWS) if few else (items[:p.n_work], joins[:p.n_joins], tile)
+                assert sum(x[0] == s for x in items) == sum(x[0] == s for x in w)
+                for r0 in range(0, ql * G, step):
+                    mine = sorted(x[2:5] for x in w if x[0] == s and x[1] == r0)
+                    assert mine[0][0] == 0 and all(x[1] == y[0] and x[1] % 64 == 0 for x, y in zip(mine, mine[1:]))
+                    assert mine[-1][1] > cl - ql + (min(r0 + step, ql * G) - 1) // G
                     if len(mine) > 1:
-                        j = [j for j in joins if j[:2] == [s, r0]]
-                        assert len(j) == 1 and [m[2] for m in mine] == list(range(j[0][2], j[0][2] + j[0][3]))
+                        k = [x for x in j if x[:2] == [s, r0]]
+                        assert len(k) == 1 and [m[2] for m in mine] == list(range(k[0][2], k[0][2] + k[0][3]))
                     else:
                         assert mine[0][2] == -1
+
+
+@pytest.mark.gpu
+@both
+@pytest.mark.parametrize("nq,nkv", [(8, 2), (14, 2), (32, 8), (48, 1), (3, 3)])
+@pytest.mark.parametrize("bs", [16, 64])
+def test_prefill_few_rows(codes, nq, nkv, bs):
+    """Sequences of 1 to 64 rows a key/value head (few, or a tile of 64), in one part and in many, beside one of many rows."""
+    for new, ctx in (([1, 2, 5], [1, 3, 400]), ([16, 1, 100, 3], [2100, 900, 300, 70]), ([4], [9000])):
+        plan = run_prefill(codes, nq, nkv, bs, new, ctx, seed=nq + bs)
+        assert bool(plan.n_few) == any(0 < n * nq // nkv <= block8.FEW_ROWS for n in new)
+    run_prefill(codes, nq, nkv, bs, [3, 1], [777, 1], seed=2, causal=False)
 
 
 @pytest.mark.gpu
