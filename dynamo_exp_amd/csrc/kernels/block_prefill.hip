@@ -13,9 +13,10 @@
 // moves when a tile's exceeds it by 2^8, and weights are held as 2^7 times themselves, 2^15 at most: fp16 rounds those over 2^-21 (of the
 // running maximum's) to 2^-11 of themselves, smaller ones to 2^-32.  Q is brought under 2 by a power of two a row (what lies 2^14 under the row's largest value loses digits).
 //
-// Scales stay out of the products: ks is a factor of the scores, and O is held in units of the tile's vs, changed when that changes.  In
-// blocks of 16 and 32 a tile has several: the scores take theirs group by group, V is widened in units of the tile's largest (fp16 holds a
-// code 2^-24 times that exactly).  A tile whose vs is 2^-80 of the unit in use adds nothing that fp32 would see, and is left out.
+// Scales stay out of the products and cost no instruction a score: ks is a factor of the scores, O is held in units of a vs that the
+// tiles agree on, and what a tile's vs is of the unit (1 to 2^-8) is added to its exponents; the row sum's ones are its inverse.  The unit
+// follows the largest vs up, and down by 2^8 steps; a block whose vs is less than 2^-8 of the unit (blocks of 16 and 32 keys, next to
+// larger ones of their tile) is widened to fp16 as so much less, exact to 2^-24 of a code.
 //
 // Few rows behind many keys are split over the keys (the plan says where), each part leaves its sums in fp32, and a second kernel
 // joins them.
@@ -54,6 +55,7 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
   constexpr int NW = RW * KW, PIECES = 8 / NW;  // pieces of 8 rows of a tile that a wave brings
   constexpr int SUBS = 2 / KW;                  // 32-key pieces of a tile that a wave multiplies
   constexpr int NG = ONE ? 1 : 4;               // scales of a tile
+  constexpr bool kRaised = NW == 8;
   __shared__ __attribute__((aligned(16))) char smem[2 * 2 * kTileBytes];
   const int* item = a.work + (int64_t)blockIdx.y * kItem;
   const int kvh = blockIdx.x, G = a.G;
@@ -100,6 +102,8 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
   // ---- a tile's codes: piece p of this wave is rows 8 (PIECES wid + p) .. + 7, a lane 16 columns of one of them
   raw4 kr[PIECES], vr[PIECES];
   float ks_next[NG], vs_next[NG];  // the scales of the tile on its way
+  float unit = 0x1p-126f, most = 0.f;  // what O is in, from that tile on; the largest vs so far
+  float vs_part[NG];                   // its values' scales in units of that
   auto load = [&](int t) __attribute__((always_inline)) {
     const int j0 = key0 + t * BKV;
     if (min((j0 + BKV - 1) >> a.bs_shift, last) - first >= 64) {
@@ -123,9 +127,15 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
       vs_next[g] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs_l), i));
     }
   };
-  auto top_scale = [&](const float (&vs)[NG]) {
-    if constexpr (ONE) return vs[0];
-    else return fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+  auto agree = [&]() __attribute__((always_inline)) {
+    float top = vs_next[0];
+#pragma unroll
+    for (int g = 1; g < NG; ++g) top = fmaxf(top, vs_next[g]);
+    // (never 2^60 under the largest: O stays a number, and what is less would hardly be seen beside it; a block of zeros may have scale 0)
+    most = fmaxf(most, top);
+    if (top > unit || (top < unit * 0x1p-8f && top > most * 0x1p-60f)) unit = top;
+#pragma unroll
+    for (int g = 0; g < NG; ++g) vs_part[g] = vs_next[g] * __builtin_amdgcn_rcpf(unit);  // (of a power of two: exact)
   };
   auto store = [&](char* kb, int t) __attribute__((always_inline)) {
     const int j0 = key0 + t * BKV;
@@ -141,14 +151,10 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
       widen16_f16<CODE, false>(kr[p], 1.f, o);
       *reinterpret_cast<raw4*>(kb + to) = o[0];
       *reinterpret_cast<raw4*>(kb + to1) = o[1];
-      if constexpr (ONE) {
-        widen16_f16<CODE, false>(vr[p], 1.f, o);
-      } else {
-        const int g = (PIECES * wid + p) >> 1;
-        const float mine = g == 0 ? vs_next[0] : g == 1 ? vs_next[NG > 1 ? 1 : 0] : g == 2 ? vs_next[NG > 2 ? 2 : 0] : vs_next[NG > 3 ? 3 : 0];
-        const float top = top_scale(vs_next);
-        widen16_f16<CODE, true>(vr[p], top > 0.f ? mine / top : 0.f, o);
-      }
+      const int g = ONE ? 0 : (PIECES * wid + p) >> 1;
+      const float part = g == 0 ? vs_part[0] : g == 1 ? vs_part[NG > 1 ? 1 : 0] : g == 2 ? vs_part[NG > 2 ? 2 : 0] : vs_part[NG > 3 ? 3 : 0];
+      if (part < 0x1p-8f) widen16_f16<CODE, true>(vr[p], part * 0x1p8f, o);
+      else widen16_f16<CODE, false>(vr[p], 1.f, o);
       *reinterpret_cast<raw4*>(kb + kTileBytes + to) = o[0];
       *reinterpret_cast<raw4*>(kb + kTileBytes + to1) = o[1];
     }
@@ -178,8 +184,8 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
 #pragma unroll
   for (int i = 0; i < 4; ++i) o_acc[i] = f32x16{};
   float m_i = -1e30f;
-  float ks_now[NG], vs_tile = 1.f, vs_unit = n_tiles > 0 ? top_scale(vs_next) : 1.f;
-  const f16x8 kOnes = __builtin_bit_cast(f16x8, u16x8{{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u}});
+  float ks_now[NG], part_log[NG], unit_now = 1.f, unit_o = 0.f;  // of the tile in use; what this wave's O is in
+  uint32_t ones[NG];                                             // fp16 pairs
   auto vread = [&](const char* vb, int i) __attribute__((always_inline)) {  // columns 32 (i % 4) .. + 31 of keys 16 (i / 4) .. + 15
     const i16x4 lo = read_tr16((const lds_i16x4*)(vb + i / 4 * 4096 + voff[i % 4][0]));
     const i16x4 hi = read_tr16((const lds_i16x4*)(vb + i / 4 * 4096 + voff[i % 4][1]));
@@ -218,17 +224,6 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
     const char* vb = tile + kTileBytes + 8192 * SUBS * kw;
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) vf[i] = vread(vb, i);
-    // a score's worth: one factor a tile, or one each 16 keys
-    float sc = q_unit * ks_now[0];
-    if constexpr (!ONE) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float g0 = KW == 2 ? (kw ? ks_now[NG > 2 ? 2 + (i >> 3) : 0] : ks_now[NG > 1 ? i >> 3 : 0]) : ks_now[NG > 1 ? i >> 3 : 0];
-        s0[i] *= q_unit * g0;
-        if constexpr (SUBS == 2) s1[i] *= q_unit * ks_now[NG > 2 ? 2 + (i >> 3) : 0];
-      }
-      sc = 1.f;
-    }
     if (j0 + 32 * SUBS - 1 > wave_min || j0 + 32 * SUBS > ctx) {  // the diagonal, or the context's end
       const int lim = min(my_pos, ctx - 1) - j0 - 4 * h;
 #pragma unroll
@@ -238,66 +233,104 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
         if constexpr (SUBS == 2) s1[i] = off + 32 > lim ? -INFINITY : s1[i];
       }
     }
-    float ta = s0[0], tb = s0[1];
-    if constexpr (SUBS == 2) ta = fmaxf(ta, s1[0]), tb = fmaxf(tb, s1[1]);
+    // a score's factor, and what its exponent is short of: one of a tile, or one each 16 keys (group 2 sub + s2 of this wave's)
+    float sc[2][2], lg[2][2];
+    uint32_t one[2][2];
 #pragma unroll
-    for (int i = 2; i < 16; i += 2) {
-      ta = fmaxf(ta, s0[i]), tb = fmaxf(tb, s0[i + 1]);
-      if constexpr (SUBS == 2) ta = fmaxf(ta, s1[i]), tb = fmaxf(tb, s1[i + 1]);
+    for (int sub = 0; sub < SUBS; ++sub)
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2) {
+        if constexpr (ONE) {
+          sc[sub][s2] = q_unit * ks_now[0], lg[sub][s2] = part_log[0], one[sub][s2] = ones[0];
+        } else if constexpr (KW == 1) {
+          sc[sub][s2] = q_unit * ks_now[NG > 1 ? 2 * sub + s2 : 0], lg[sub][s2] = part_log[NG > 1 ? 2 * sub + s2 : 0], one[sub][s2] = ones[NG > 1 ? 2 * sub + s2 : 0];
+        } else {
+          constexpr int kHi = NG > 2 ? 2 : 0;
+          sc[sub][s2] = q_unit * (kw ? ks_now[kHi + (NG > 1 ? s2 : 0)] : ks_now[NG > 1 ? s2 : 0]);
+          lg[sub][s2] = kw ? part_log[kHi + (NG > 1 ? s2 : 0)] : part_log[NG > 1 ? s2 : 0];
+          one[sub][s2] = kw ? ones[kHi + (NG > 1 ? s2 : 0)] : ones[NG > 1 ? s2 : 0];
+        }
+      }
+    float t_s;
+    if constexpr (ONE) {
+      float ta = s0[0], tb = s0[1];
+      if constexpr (SUBS == 2) ta = fmaxf(ta, s1[0]), tb = fmaxf(tb, s1[1]);
+#pragma unroll
+      for (int i = 2; i < 16; i += 2) {
+        ta = fmaxf(ta, s0[i]), tb = fmaxf(tb, s0[i + 1]);
+        if constexpr (SUBS == 2) ta = fmaxf(ta, s1[i]), tb = fmaxf(tb, s1[i + 1]);
+      }
+      t_s = halves_max(fmaxf(ta, tb)) * sc[0][0];  // (scales are positive)
+    } else {
+      t_s = -INFINITY;
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2) {
+        float ta = s0[8 * s2], tb = SUBS == 2 ? s1[8 * s2] : -INFINITY;
+#pragma unroll
+        for (int i = 8 * s2 + 1; i < 8 * s2 + 8; ++i) {
+          ta = fmaxf(ta, s0[i]);
+          if constexpr (SUBS == 2) tb = fmaxf(tb, s1[i]);
+        }
+        t_s = fmaxf(t_s, ta * sc[0][s2]);
+        if constexpr (SUBS == 2) t_s = fmaxf(t_s, tb * sc[1][s2]);
+      }
+      t_s = halves_max(t_s);
     }
-    const float t_s = halves_max(fmaxf(ta, tb)) * sc;  // (scales are positive)
     const float m_new = t_s > m_i + kRescale ? t_s : m_i;
     const float alpha = fast_exp2(m_i - m_new);
     m_i = m_new;
-    const float base = m_new - kLift;
     u16x8 pf[2][2];
 #pragma unroll
-    for (int s2 = 0; s2 < 2; ++s2)
+    for (int s2 = 0; s2 < 2; ++s2) {
+      const float b0 = m_new - (kLift + lg[0][s2]), b1 = SUBS == 2 ? m_new - (kLift + lg[SUBS - 1][s2]) : 0.f;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const int i = 8 * s2 + 2 * w;
-        pf[0][s2].w[w] = pack_f16x2(fast_exp2(s0[i] * sc - base), fast_exp2(s0[i + 1] * sc - base));
-        if constexpr (SUBS == 2) pf[1][s2].w[w] = pack_f16x2(fast_exp2(s1[i] * sc - base), fast_exp2(s1[i + 1] * sc - base));
+        pf[0][s2].w[w] = pack_f16x2(fast_exp2(s0[i] * sc[0][s2] - b0), fast_exp2(s0[i + 1] * sc[0][s2] - b0));
+        if constexpr (SUBS == 2) pf[1][s2].w[w] = pack_f16x2(fast_exp2(s1[i] * sc[1][s2] - b1), fast_exp2(s1[i + 1] * sc[1][s2] - b1));
       }
-    // O's unit: the tile's vs, but for one that is as good as nothing beside it
-    const bool no_v = vs_tile < vs_unit * 0x1p-80f;
-    float unit = 1.f;
-    if (!no_v && vs_tile != vs_unit) {
-      unit = vs_unit / vs_tile;
-      vs_unit = vs_tile;
     }
-    if (unit != 1.f || __builtin_amdgcn_ballot_w64(alpha != 1.f)) {
-      const float both = alpha * unit;
+    const bool other = unit_o != unit_now;
+    if (other || __builtin_amdgcn_ballot_w64(alpha != 1.f)) {
+      const float both = alpha * (unit_o * __builtin_amdgcn_rcpf(unit_now));
+      unit_o = unit_now;
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt) o_acc[dt] *= both;
       l_acc *= alpha;
     }
+    if constexpr (kRaised) __builtin_amdgcn_s_setprio(0);
 #pragma unroll
     for (int sub = 0; sub < SUBS; ++sub)
       if (sub == 0 || live1) {
-        if (no_v) {
 #pragma unroll
-          for (int s2 = 0; s2 < 2; ++s2) l_acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kOnes, __builtin_bit_cast(f16x8, pf[sub][s2]), l_acc, 0, 0, 0);
-        } else {
-#pragma unroll
-          for (int i = 8 * sub; i < 8 * sub + 8; ++i) {
-            const f16x8 p = __builtin_bit_cast(f16x8, pf[sub][(i >> 2) & 1]), x = vf[i % kAhead];
-            if (i + kAhead < 8 * SUBS) vf[i % kAhead] = vread(vb, i + kAhead);
-            o_acc[i & 3] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p, o_acc[i & 3], 0, 0, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            if (i + kAhead < 8 * SUBS) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-            if ((i & 3) == 3) l_acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(kOnes, p, l_acc, 0, 0, 0);
+        for (int i = 8 * sub; i < 8 * sub + 8; ++i) {
+          const int s2 = (i >> 2) & 1;
+          const f16x8 p = __builtin_bit_cast(f16x8, pf[sub][s2]), x = vf[i % kAhead];
+          if (i + kAhead < 8 * SUBS) vf[i % kAhead] = vread(vb, i + kAhead);
+          o_acc[i & 3] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p, o_acc[i & 3], 0, 0, 0);
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          if (i + kAhead < 8 * SUBS) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+          if ((i & 3) == 3) {
+            const uint32_t k1 = one[sub][s2];
+            l_acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, raw4{k1, k1, k1, k1}), p, l_acc, 0, 0, 0);
           }
         }
       }
+    if constexpr (kRaised) __builtin_amdgcn_s_setprio(1);
   };
   auto turn_over = [&]() __attribute__((always_inline)) {  // the tile that was on its way is the tile in use
+    unit_now = unit;
 #pragma unroll
-    for (int g = 0; g < NG; ++g) ks_now[g] = ks_next[g];
-    vs_tile = top_scale(vs_next);
+    for (int g = 0; g < NG; ++g) {
+      const float part = fmaxf(vs_part[g], 0x1p-8f);
+      ks_now[g] = ks_next[g];
+      part_log[g] = __builtin_amdgcn_logf(part);
+      ones[g] = pack_f16x2(__builtin_amdgcn_rcpf(part), __builtin_amdgcn_rcpf(part));
+    }
   };
 
   if (n_tiles > 0) {
+    agree();
     store(smem, 0);
     turn_over();
   }
@@ -307,6 +340,7 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
     if (t + 1 < n_tiles) load(t + 1);
     compute(now, t);
     if (t + 1 < n_tiles) {
+      agree();
       store(next, t + 1);
       turn_over();
     }
@@ -316,7 +350,7 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
   // ---- lane (r, h) holds columns 32 dt + 8 g + 4 h .. + 3 of its row
   float l_i = l_acc[0];
 #pragma unroll
-  for (int dt = 0; dt < 4; ++dt) o_acc[dt] *= vs_unit;
+  for (int dt = 0; dt < 4; ++dt) o_acc[dt] *= unit_o;
   if constexpr (KW == 2) {  // the second half of the waves hands its sums to the first
     float* so = reinterpret_cast<float*>(smem) + rw * (BQ * D);  // [64 lanes] x 64 values, a lane's apart by 64 so that a wave's lie together
     float* sml = reinterpret_cast<float*>(smem + RW * BQ * D * 4) + rw * 128;
