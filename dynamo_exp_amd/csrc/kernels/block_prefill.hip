@@ -9,7 +9,7 @@
 // bytes a lane, and become fp16 in a swizzled double-buffered LDS image behind the tile's products (a workgroup widens a code once
 // for all its rows, by 0.5 or 1.25 instructions).  S^T = K Q^T and O^T = V^T P^T on 32 x 32 x 16 products: a lane's scores are one
 // row's, the softmax is lane-local but for one exchange between the halves, the weights are the second product's operand as they are, V
-// is read transposed, and the row sum is a product with ones (of the fp16 weights that the second product sees).  The running maximum
+// is read transposed, and the row sum is taken of the fp16 weights that the second product sees, two by an instruction.  The running maximum
 // moves when a tile's exceeds it by 2^8, and weights are held as 2^7 times themselves, 2^15 at most: fp16 rounds those over 2^-21 (of the
 // running maximum's) to 2^-11 of themselves, smaller ones to 2^-32.  Q is brought under 2 by a power of two a row (what lies 2^14 under the row's largest value loses digits).
 //
@@ -48,6 +48,11 @@ struct PrefillArgs {
   int bt_stride, bt_cols, n_kv, G, bs_shift, num_blocks, causal, tile;  // tile: rows of a place of sums
   float scale_log2e;
 };
+
+// a pair of fp16 times another, added to a sum in fp32
+__device__ __forceinline__ float sum2(uint32_t a, uint32_t b, float c) {
+  return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, a), __builtin_bit_cast(f16x2, b), c, false);
+}
 
 // RW: row waves of 32 rows; KW: waves that share a tile's keys (1, or 2: 32 each); ONE: a tile's keys lie in one block
 template <int CODE, int RW, int KW, bool ONE>
@@ -127,15 +132,17 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
       vs_next[g] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs_l), i));
     }
   };
+  // (what is the same in all lanes, in scalar registers)
+  auto uni = [](float x) __attribute__((always_inline)) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); };
   auto agree = [&]() __attribute__((always_inline)) {
     float top = vs_next[0];
 #pragma unroll
     for (int g = 1; g < NG; ++g) top = fmaxf(top, vs_next[g]);
     // (never 2^60 under the largest: O stays a number, and what is less would hardly be seen beside it; a block of zeros may have scale 0)
-    most = fmaxf(most, top);
-    if (top > unit || (top < unit * 0x1p-8f && top > most * 0x1p-60f)) unit = top;
+    most = uni(fmaxf(most, top));
+    if (top > unit || (top < unit * 0x1p-8f && top > most * 0x1p-60f)) unit = uni(top);
 #pragma unroll
-    for (int g = 0; g < NG; ++g) vs_part[g] = vs_next[g] * __builtin_amdgcn_rcpf(unit);  // (of a power of two: exact)
+    for (int g = 0; g < NG; ++g) vs_part[g] = uni(vs_next[g] * __builtin_amdgcn_rcpf(unit));  // (of a power of two: exact)
   };
   auto store = [&](char* kb, int t) __attribute__((always_inline)) {
     const int j0 = key0 + t * BKV;
@@ -180,10 +187,10 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
       for (int w = 0; w < 4; ++w) qf[s].w[w] = pack_f16x2(bf16lo(qf[s].w[w]) * unit, bf16hi(qf[s].w[w]) * unit);
     q_unit = a.scale_log2e / unit;
   }
-  f32x16 o_acc[4], l_acc = f32x16{};
+  f32x16 o_acc[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) o_acc[i] = f32x16{};
-  float m_i = -1e30f;
+  float m_i = -1e30f, l_i = 0.f;  // (l: of this lane's keys)
   float ks_now[NG], part_log[NG], unit_now = 1.f, unit_o = 0.f;  // of the tile in use; what this wave's O is in
   uint32_t ones[NG];                                             // fp16 pairs
   auto vread = [&](const char* vb, int i) __attribute__((always_inline)) {  // columns 32 (i % 4) .. + 31 of keys 16 (i / 4) .. + 15
@@ -290,13 +297,19 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
         if constexpr (SUBS == 2) pf[1][s2].w[w] = pack_f16x2(fast_exp2(s1[i] * sc[1][s2] - b1), fast_exp2(s1[i + 1] * sc[1][s2] - b1));
       }
     }
+    l_i *= alpha;
+#pragma unroll
+    for (int sub = 0; sub < SUBS; ++sub)
+#pragma unroll
+      for (int s2 = 0; s2 < 2; ++s2)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) l_i = sum2(pf[sub][s2].w[w], one[sub][s2], l_i);
     const bool other = unit_o != unit_now;
     if (other || __builtin_amdgcn_ballot_w64(alpha != 1.f)) {
       const float both = alpha * (unit_o * __builtin_amdgcn_rcpf(unit_now));
       unit_o = unit_now;
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt) o_acc[dt] *= both;
-      l_acc *= alpha;
     }
     if constexpr (kRaised) __builtin_amdgcn_s_setprio(0);
 #pragma unroll
@@ -310,10 +323,6 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
           o_acc[i & 3] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p, o_acc[i & 3], 0, 0, 0);
           __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
           if (i + kAhead < 8 * SUBS) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-          if ((i & 3) == 3) {
-            const uint32_t k1 = one[sub][s2];
-            l_acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, raw4{k1, k1, k1, k1}), p, l_acc, 0, 0, 0);
-          }
         }
       }
     if constexpr (kRaised) __builtin_amdgcn_s_setprio(1);
@@ -324,8 +333,8 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
     for (int g = 0; g < NG; ++g) {
       const float part = fmaxf(vs_part[g], 0x1p-8f);
       ks_now[g] = ks_next[g];
-      part_log[g] = __builtin_amdgcn_logf(part);
-      ones[g] = pack_f16x2(__builtin_amdgcn_rcpf(part), __builtin_amdgcn_rcpf(part));
+      part_log[g] = uni(__builtin_amdgcn_logf(part));
+      ones[g] = __builtin_amdgcn_readfirstlane(pack_f16x2(__builtin_amdgcn_rcpf(part), __builtin_amdgcn_rcpf(part)));
     }
   };
 
@@ -348,7 +357,7 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
   }
 
   // ---- lane (r, h) holds columns 32 dt + 8 g + 4 h .. + 3 of its row
-  float l_i = l_acc[0];
+  l_i = halves_sum(l_i);
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt) o_acc[dt] *= unit_o;
   if constexpr (KW == 2) {  // the second half of the waves hands its sums to the first
