@@ -226,7 +226,7 @@ class PrefillPlan(NamedTuple):
     causal: bool
 
 
-PREFILL_WGS, PREFILL_TILES = 512, 4
+PREFILL_WGS, SPLIT_WGS, PREFILL_TILES = 512, 256, 4
 FEW_ROWS, FEW_WGS, FEW_KEYS = 32, 256, 256
 
 
@@ -271,7 +271,7 @@ def prefill_plan(q_lens: list[int], ctx_lens: list[int], n_q: int, n_kv: int, de
             seen = cl - ql + (min(r0 + tile, ql * g) - 1) // g + 1 if causal else cl
             items.append((-(-seen // 64), s, r0))
     total = sum(i[0] for i in items)
-    work, joins, places = cut(items, 64, max(PREFILL_TILES, -(-total * n_kv // PREFILL_WGS)) if len(items) * n_kv < PREFILL_WGS else 1 << 30)
+    work, joins, places = cut(items, 64, max(PREFILL_TILES, -(-total * n_kv // SPLIT_WGS)) if len(items) * n_kv < SPLIT_WGS else 1 << 30)
     items = [(-(-ctx_lens[s] // 128), s, 0) for s in few]
     total = sum(i[0] for i in items)
     few_work, few_joins, few_places = cut(items, 128, max(FEW_KEYS // 128, -(-total * n_kv // FEW_WGS)))
