@@ -5,7 +5,9 @@
 //
 // Bound by HBM: a (token, head) row of codes is read once, 2 x 128 bytes, and serves the G query heads of its group, which are
 // columns of the matrix products.  Balanced parts of a context, joined by a second kernel, as in the bf16 form
-// (decode_join.h); a workgroup's four waves take chunks of 32 tokens in turn, their K and V on their way a chunk ahead.
+// (decode_join.h); a workgroup's waves take chunks of 32 tokens in turn, their K and V on their way a chunk ahead.  Four waves, or eight
+// where contexts are short and few enough to be left whole (at most 768 tokens, a workgroup a CU): the join, a launch of its own, costs
+// more than two chunks more.
 //
 // Codes widen to bf16 exactly, so the products see them without their scales: ks is a factor of a lane's scores (a lane's eight
 // tokens lie in one half of a chunk, thus in one block of 16 or more), and vs one of its weights before they are rounded to bf16
@@ -22,7 +24,7 @@
 
 namespace {
 
-constexpr int D = kHeadDim, kThreads = 256, CH = 32;
+constexpr int D = kHeadDim, CH = 32;
 
 __device__ __forceinline__ int vimg_off(int row, int ch) {  // byte offset of 16-B chunk ch of row in a wave's image
   return row * 256 + 16 * (ch ^ (((row & 3) << 2) | ((row >> 2) & 3)));
@@ -41,16 +43,24 @@ struct DecodeArgs {
   float scale_log2e;
 };
 
-template <int CODE>
-__global__ void __launch_bounds__(kThreads, 3) block_decode_kernel(const DecodeArgs a) {
+template <int CODE, int NW>
+__global__ void __launch_bounds__(64 * NW, NW == 4 ? 3 : 2) block_decode_kernel(const DecodeArgs a) {
+  constexpr int kThreads = 64 * NW;
   constexpr float kRescale = 8.0f;  // the running maximum moves when a chunk's exceeds it by 2^8
-  __shared__ __attribute__((aligned(16))) char image[4 * CH * D * 2];
-  __shared__ float st_m[4 * 16], st_l[4 * 16];
+  __shared__ __attribute__((aligned(16))) char image[NW * CH * D * 2];
+  __shared__ float st_m[NW * 16], st_l[NW * 16];
   const int pid = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z, n_parts = gridDim.x, G = a.G;
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, r = lane & 15;
   const int64_t qh0 = ((int64_t)b * a.n_kv + kvh) * G;
-  // (a table's columns are all that may be read of it)
+  // the part's blocks, 64 at a time, a lane each; the first 64 of the context are asked for beside its length, not behind it (a table's
+  // columns are all that may be read of it)
+  const int* bt = a.block_tables + (int64_t)b * a.bt_stride;
+  int first = 0, ids = bt[min(lane, a.bt_cols - 1)];
+  raw4 qf[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s)  // (columns behind the heads hold the last one's, and go nowhere)
+    qf[s] = *reinterpret_cast<const raw4*>(a.q + b * a.q_stride + (int64_t)(kvh * G + min(r, G - 1)) * D + 8 * (4 * g + s));
   const int ctx = __builtin_amdgcn_readfirstlane((int)min((int64_t)a.ctx_lens[b], (int64_t)a.bt_cols << a.bs_shift));
   if (ctx <= 0) {
     if (n_parts == 1)
@@ -63,26 +73,19 @@ __global__ void __launch_bounds__(kThreads, 3) block_decode_kernel(const DecodeA
   const int p1 = min(p0 + part, ctx);
   char* vimg = image + wid * (CH * D * 2);
 
-  raw4 qf[4];
-#pragma unroll
-  for (int s = 0; s < 4; ++s)  // (columns behind the heads hold the last one's, and go nowhere)
-    qf[s] = *reinterpret_cast<const raw4*>(a.q + b * a.q_stride + (int64_t)(kvh * G + min(r, G - 1)) * D + 8 * (4 * g + s));
-
-  // the part's blocks, 64 at a time, a lane each
-  const int* bt = a.block_tables + (int64_t)b * a.bt_stride;
   const int last = (ctx - 1) >> a.bs_shift;
-  int first = p0 >> a.bs_shift, ids;
-  auto fetch = [&]() {
-    const int id = bt[min(first + lane, last)];
-    ids = (unsigned)id < (unsigned)a.num_blocks ? id : 0;
-  };
-  fetch();
+  auto fetch = [&]() { ids = bt[min(first + lane, last)]; };
+  if ((p1 - 1) >> a.bs_shift >= 64) {
+    first = p0 >> a.bs_shift;
+    fetch();
+  }
   auto block_at = [&](int i) {
     if (i - first >= 64) {  // (chunks only go up)
       first = i;
       fetch();
     }
-    return __builtin_amdgcn_readlane(ids, max(i - first, 0));
+    const int id = __builtin_amdgcn_readlane(ids, max(i - first, 0));
+    return (unsigned)id < (unsigned)a.num_blocks ? id : 0;
   };
 
   f32x4 oacc[8];
@@ -141,7 +144,7 @@ __global__ void __launch_bounds__(kThreads, 3) block_decode_kernel(const DecodeA
       *reinterpret_cast<raw4*>(vimg + vimg_off(4 * k + g, r)) = raw4{lo[0], lo[1], hi[0], hi[1]};
     }
     const float kscale = ks_l * a.scale_log2e, vscale = vs_l;
-    if constexpr (more) load(c + 4);
+    if constexpr (more) load(c + NW);
     float t[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) t[j] = sacc[j >> 2][j & 3] * kscale;
@@ -187,7 +190,7 @@ __global__ void __launch_bounds__(kThreads, 3) block_decode_kernel(const DecodeA
   int c = wid;
   if (c < n_chunks) {
     load(c);
-    for (; c + 4 < n_chunks; c += 4) step(std::true_type{}, c);
+    for (; c + NW < n_chunks; c += NW) step(std::true_type{}, c);
     step(std::false_type{}, c);
   }
 
@@ -202,18 +205,18 @@ __global__ void __launch_bounds__(kThreads, 3) block_decode_kernel(const DecodeA
   __syncthreads();
   for (int i = threadIdx.x; i < G * D / 4; i += kThreads) {
     const int h = i / (D / 4), d = 4 * (i % (D / 4));
-    float m[4], l[4];
-    f32x4 o[4];
+    float m[NW], l[NW], M = -1e30f;
+    f32x4 o[NW];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < NW; ++w) {
       m[w] = st_m[w * 16 + h], l[w] = st_l[w * 16 + h];
       o[w] = *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(image + w * (CH * D * 2)) + h * D + d);
+      M = fmaxf(M, m[w]);
     }
-    const float M = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
     float den = 0.f;
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < NW; ++w) {
       const float f = exp2f(m[w] - M);
       sum += f * o[w];
       den += f * l[w];
@@ -251,8 +254,15 @@ extern "C" int dx_block_decode(void* out, float* tmp_out, float* tmp_ml, const v
   a.n_kv = n_kv, a.G = n_q / n_kv, a.bs_shift = __builtin_ctz((unsigned)block_size), a.num_blocks = num_blocks;
   a.scale_log2e = scale * 1.4426950408889634f;
   const dim3 grid(n_parts, n_kv, batch);
-  if (code == kE4m3) block_decode_kernel<kE4m3><<<grid, kThreads, 0, stream>>>(a);
-  else block_decode_kernel<kInt8><<<grid, kThreads, 0, stream>>>(a);
+  const bool eight = n_parts == 1 && (int64_t)batch * n_kv <= 256;
+#define DX_BD(C)                                                               \
+  do {                                                                         \
+    if (eight) block_decode_kernel<C, 8><<<grid, 512, 0, stream>>>(a);         \
+    else block_decode_kernel<C, 4><<<grid, 256, 0, stream>>>(a);               \
+  } while (0)
+  if (code == kE4m3) DX_BD(kE4m3);
+  else DX_BD(kInt8);
+#undef DX_BD
   if (n_parts > 1) join(a.out, tmp_out, tmp_ml, ctx_lens, n_q, batch, n_parts, 4 * CH, stream,
                         (int)min((int64_t)bt_cols * block_size, (int64_t)0x7fffffff));
   return (int)hipGetLastError();

@@ -724,6 +724,8 @@ def kv_dequant_scratch(k_cache, v_cache, block_tables, ctx_lens, kv_scales=(1.0,
     nseq x padded max_blocks); without it (direct calls in tests) the
     dense table i * max_blocks + j.  kv_scales tensors: a block-scaled cache
     (block8)."""
+    if block8.blocked(kv_scales):
+        return block8.read_back(k_cache, v_cache, kv_scales, block_tables, ctx_lens, scratch, _KV_SCRATCH)
     nseq, maxb = block_tables.shape
     _, H, BS, D = k_cache.shape
     n = scratch[1] if scratch is not None else nseq * maxb
@@ -735,13 +737,10 @@ def kv_dequant_scratch(k_cache, v_cache, block_tables, ctx_lens, kv_scales=(1.0,
               torch.empty((cap, H, BS, D), dtype=torch.bfloat16, device=k_cache.device),
               torch.arange(cap, dtype=torch.int32, device=k_cache.device))
         _KV_SCRATCH[key] = ws
-    ks, vs = (ws[0], ws[1]) if ws[0].shape[0] == n else (ws[0][:max(n, 1)], ws[1][:max(n, 1)])
+    ks, vs = ws[0][:max(n, 1)], ws[1][:max(n, 1)]
     table = scratch[0] if scratch is not None else ws[2][:n].view(nseq, maxb)
     assert block_tables.dtype == torch.int32 and ctx_lens.dtype == torch.int32 and table.dtype == torch.int32
     assert table.shape == (nseq, maxb) and table.is_contiguous()
-    if block8.blocked(kv_scales):
-        block8.dequant(k_cache, v_cache, kv_scales, block_tables, ctx_lens, ks, vs, table)
-        return ks, vs, table
     _k().kv_dequant(k_cache.data_ptr(), v_cache.data_ptr(), ks.data_ptr(), vs.data_ptr(), block_tables.data_ptr(),
                     block_tables.stride(0), ctx_lens.data_ptr(), table.data_ptr(), nseq, maxb, H, BS, D,
                     float(kv_scales[0]), float(kv_scales[1]), _stream())

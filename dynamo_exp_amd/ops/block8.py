@@ -11,6 +11,7 @@ scale anew.
 """
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple
 
 import torch
@@ -135,19 +136,36 @@ def append_rows(qp, kp, vp, T, stride, nq, hkv, qop, q_out_stride, positions, co
         _stream(k_cache))
 
 
-def dequant(k_cache, v_cache, kv_scales, block_tables, ctx_lens, k_out, v_out, table):
-    """The blocks of `block_tables` [n, columns] that hold ctx_lens [n] tokens, as bf16, into blocks `table` [n, columns] of k_out and v_out."""
+def read_back(k_cache, v_cache, kv_scales, block_tables, ctx_lens, scratch, workspaces):
+    """ops.kv_dequant_scratch of a block-scaled cache."""
     _check_cache(k_cache, v_cache, kv_scales)
     nb, hkv, bs, d = k_cache.shape
     n, cols = block_tables.shape
-    if block_tables.dtype != torch.int32 or ctx_lens.dtype != torch.int32 or table.dtype != torch.int32:
+    if block_tables.dtype != torch.int32 or ctx_lens.dtype != torch.int32:
         raise TypeError("kv_dequant_scratch: tables and lengths are int32")
-    if block_tables.stride(1) != 1 and cols > 1 or ctx_lens.shape != (n,) or table.shape != (n, cols) or not (table.is_contiguous() and ctx_lens.is_contiguous()):
-        raise ValueError("kv_dequant_scratch: block_tables [n, columns], ctx_lens [n], table [n, columns]")
-    _check_on(k_cache.device, block_tables=block_tables, ctx_lens=ctx_lens, table=table)
-    _native.kernels().block_dequant(k_cache.data_ptr(), v_cache.data_ptr(), kv_scales[0].data_ptr(), kv_scales[1].data_ptr(), k_out.data_ptr(),
-                                    v_out.data_ptr(), block_tables.data_ptr(), block_tables.stride(0), ctx_lens.data_ptr(), table.data_ptr(), n, cols,
-                                    nb, k_out.shape[0], hkv, bs, d, CODES[k_cache.dtype], _stream(k_cache))
+    if (cols > 1 and block_tables.stride(1) != 1) or ctx_lens.dim() != 1 or ctx_lens.shape[0] != n or not ctx_lens.is_contiguous():
+        raise ValueError(f"kv_dequant_scratch: block_tables {tuple(block_tables.shape)}, ctx_lens {tuple(ctx_lens.shape)}")
+    dev = k_cache.device
+    if block_tables.device != dev or ctx_lens.device != dev:
+        raise ValueError(f"kv_dequant_scratch: tables on {block_tables.device}, lengths on {ctx_lens.device}, the cache on {dev}")
+    stream = _stream(k_cache)
+    need = n * cols if scratch is None else scratch[1]
+    ws = workspaces.get((dev, stream))
+    if ws is None or ws[0].shape[0] < need or ws[0].shape[1:] != k_cache.shape[1:]:
+        cap = max(need, 64)
+        ws = (*(torch.empty((cap, hkv, bs, d), dtype=torch.bfloat16, device=dev) for _ in range(2)), torch.arange(cap, dtype=torch.int32, device=dev))
+        workspaces[(dev, stream)] = ws
+    ks, vs = (ws[0], ws[1]) if ws[0].shape[0] == need else (ws[0][:max(need, 1)], ws[1][:max(need, 1)])
+    if scratch is None:
+        table = ws[2].as_strided((n, cols), (cols, 1))
+    else:
+        table = scratch[0]
+        if table.dtype != torch.int32 or table.shape != (n, cols) or not table.is_contiguous() or table.device != dev:
+            raise ValueError(f"kv_dequant_scratch: the scratch's table is [{n}, {cols}] int32, contiguous, on {dev}")
+    _native.kernels().block_dequant(k_cache.data_ptr(), v_cache.data_ptr(), kv_scales[0].data_ptr(), kv_scales[1].data_ptr(), ks.data_ptr(),
+                                    vs.data_ptr(), block_tables.data_ptr(), block_tables.stride(0), ctx_lens.data_ptr(), table.data_ptr(), n, cols,
+                                    nb, ks.shape[0], hkv, bs, d, CODES[k_cache.dtype], stream)
+    return ks, vs, table
 
 
 def _check_reader(q, out, k_cache, v_cache, kv_scales, block_tables, ctx_lens, n):
@@ -158,14 +176,20 @@ def _check_reader(q, out, k_cache, v_cache, kv_scales, block_tables, ctx_lens, n
         raise TypeError("attention over a block-scaled cache: q and out are bfloat16")
     if d != HEAD_DIM or hq % hkv or out.shape != q.shape or not out.is_contiguous():
         raise ValueError(f"attention over a block-scaled cache: q {tuple(q.shape)}, out {tuple(out.shape)}, {hkv} key/value heads")
-    if T and (q.stride(2) != 1 or (hq > 1 and q.stride(1) != d) or (T > 1 and q.stride(0) % 8) or q.data_ptr() % 16 or out.data_ptr() % 16):
-        raise ValueError("attention over a block-scaled cache: q's heads behind one another, its rows and out 16-byte aligned")
+    if T:
+        rows, heads, cols = q.stride()
+        if cols != 1 or (hq > 1 and heads != d) or (T > 1 and rows % 8) or (q.data_ptr() | out.data_ptr()) % 16:
+            raise ValueError("attention over a block-scaled cache: q's heads behind one another, its rows and out 16-byte aligned")
     if block_tables.dtype != torch.int32 or ctx_lens.dtype != torch.int32:
         raise TypeError("attention over a block-scaled cache: tables and lengths are int32")
-    if (block_tables.dim() != 2 or block_tables.shape[0] != n or block_tables.shape[1] < 1 or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1)
-            or ctx_lens.shape != (n,) or not ctx_lens.is_contiguous()):
-        raise ValueError(f"attention over a block-scaled cache: block_tables {tuple(block_tables.shape)}, ctx_lens {tuple(ctx_lens.shape)}, {n} sequences")
-    _check_on(k_cache.device, q=q, out=out, block_tables=block_tables, ctx_lens=ctx_lens)
+    table = block_tables.shape
+    if (len(table) != 2 or table[0] != n or table[1] < 1 or (table[1] > 1 and block_tables.stride(1) != 1) or ctx_lens.dim() != 1 or
+            ctx_lens.shape[0] != n or not ctx_lens.is_contiguous()):
+        raise ValueError(f"attention over a block-scaled cache: block_tables {tuple(table)}, ctx_lens {tuple(ctx_lens.shape)}, {n} sequences")
+    dev = k_cache.device
+    if q.device != dev or out.device != dev or block_tables.device != dev or ctx_lens.device != dev:
+        raise ValueError(f"attention over a block-scaled cache: q on {q.device}, out on {out.device}, block_tables on {block_tables.device}, "
+                         f"ctx_lens on {ctx_lens.device}, the cache on {dev}")
 
 
 def decode(q, k_cache, v_cache, block_tables, ctx_lens, scale, out, n_parts, workspace, kv_scales):
@@ -199,13 +223,28 @@ def decode(q, k_cache, v_cache, block_tables, ctx_lens, scale, out, n_parts, wor
     return out
 
 
-DECODE_WGS, DECODE_PART = 512, 256
+CUS = 256
+# Tokens that eight waves take whole where a CU has one workgroup at most.  us on the GPU, whole and in the best number of parts with their
+# join: 30 sequences of 700 tokens, 8 key/value heads 11.5 and 14.6, 30 of 300 7.6 and 11.0, one of 400 7.2 and 7.0, one of 700 8.9 and
+# 7.3; a second launch costs the host 4 us more where launches are not captured.
+WHOLE = 768
 
 
+@functools.lru_cache(maxsize=4096)
 def decode_parts(batch: int, n_kv: int, max_ctx: int) -> int:
-    """Parts of a context for a decode launch over the 8-bit cache."""
-    want = -(-DECODE_WGS // max(1, batch * n_kv))
-    return max(1, min(want, -(-max(1, max_ctx) // DECODE_PART)))
+    """Parts of a context for a decode launch over the 8-bit cache of `batch` contexts of at most `max_ctx` tokens: a CU's share of the
+    workgroups, times a part's tokens and the 64 tokens' time that a part takes without any, is least, and a CU with one workgroup is a
+    tenth slower.  us, this and the parts next to it, 8 key/value heads: 40 sequences of 3000 tokens 4 parts 46.1 (2 50.5, 5 48.7), 3 of
+    60000 32 63.3 (22 81, 48 69), one of 700 6 7.3 (3 8.4), one of 4000 32 8.1 (16 8.8), 96 of 3150 1 92 (2 94)."""
+    heads = batch * n_kv
+    if heads <= CUS and max_ctx <= WHOLE:
+        return 1
+
+    def cost(p):
+        wgs = -(-heads * p // CUS)
+        return (wgs if wgs > 1 else 1.1) * (-(-max_ctx // (32 * p)) * 32 + 64)
+
+    return min(range(1, max(1, min(64, max_ctx // 96)) + 1), key=cost)
 
 
 class PrefillPlan(NamedTuple):
