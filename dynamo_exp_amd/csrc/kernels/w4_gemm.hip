@@ -13,7 +13,12 @@
 // 128 columns.  Scales [N / 16][K / 128][row][group] bf16, zeros (128 + z) the same in bytes: a lane's products are all of one row.
 // The K axis is split over the waves of a workgroup, whose sums are added in LDS in the waves' order, and over workgroups where rows
 // are few (their sums in fp32, added by a second kernel).  x rows come from L2 once for RT tiles.
+//
+// More than 16 rows (w4_wide_kernel): x would come from L2 more often than the weights from HBM (64 rows of 28672 x 4096 took 89 us that
+// way), so a workgroup's eight waves, four tile pairs by two halves of 256 columns, read it from LDS, staged a step ahead.
 #include "block8.h"
+
+#include <type_traits>
 
 namespace {
 
@@ -178,6 +183,153 @@ __global__ void __launch_bounds__(512) w4_kernel(const W4Args a) {
   }
 }
 
+// 16 T rows of x; waves: four pairs of 16-row weight tiles by the two chunks of a step of 256 columns
+template <int T, int GS, bool ZERO>
+__global__ void __launch_bounds__(512) w4_wide_kernel(const W4Args a) {
+  constexpr int RT = 2, GC = 4 / GS, XN = T;  // 16-byte pieces of x a thread stages in a step
+  __shared__ __attribute__((aligned(16))) raw4 img[2][16 * T * 32];  // [row][piece ^ row % 16]: a wave's reads meet all banks
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, q = lane >> 4, half = wid >> 2;
+  const int tiles = (a.N + 15) >> 4, nt0 = (blockIdx.x * 4 + (wid & 3)) * RT, m0 = blockIdx.y * (16 * T);
+  uint32_t base = 0x43004300u;
+  asm("" : "+v"(base));
+  const raw4 kOnes = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+  f32x4 acc[RT][T];
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int t = 0; t < T; ++t) acc[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  struct Chunk {
+    raw4 w[RT];
+    uint32_t s[RT][(GC + 1) / 2], z[RT];
+  };
+  int64_t tile_at[RT];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) tile_at[i] = (int64_t)min(nt0 + i, tiles - 1) * a.chunks;
+  const int pairs = (a.chunks + 1) >> 1, first = blockIdx.z, step = gridDim.z;
+  const int n = pairs > first ? (pairs - first + step - 1) / step : 0;
+  const bf16_t* xp[XN];
+  int col[XN], to[XN];
+#pragma unroll
+  for (int i = 0; i < XN; ++i) {
+    const int at = threadIdx.x + 512 * i, row = at >> 5, piece = at & 31;
+    xp[i] = a.x + (int64_t)min(m0 + row, a.M - 1) * a.ldx;
+    col[i] = 8 * piece;
+    to[i] = row * 32 + (piece ^ (row & 15));
+  }
+  raw4 xr[XN];
+  auto load = [&](int j, Chunk& c) __attribute__((always_inline)) {
+    const int pair = first + min(j, n - 1) * step;
+    const int kc = min(2 * pair + half, a.chunks - 1);
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const int64_t at = tile_at[i] + kc;
+      c.w[i] = __builtin_nontemporal_load(a.w + at * 64 + lane);
+      const uint16_t* s = a.s + (at * 16 + r) * GC;
+      const uint8_t* z = a.z + (at * 16 + r) * GC;
+      if constexpr (GC == 1) {
+        c.s[i][0] = *s;
+        if constexpr (ZERO) c.z[i] = *z;
+      } else if constexpr (GC == 2) {
+        c.s[i][0] = *reinterpret_cast<const uint32_t*>(s);
+        if constexpr (ZERO) c.z[i] = *reinterpret_cast<const uint16_t*>(z);
+      } else {
+        const raw2 v = *reinterpret_cast<const raw2*>(s);
+        c.s[i][0] = v[0], c.s[i][1] = v[1];
+        if constexpr (ZERO) c.z[i] = *reinterpret_cast<const uint32_t*>(z);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < XN; ++i) {
+      const int k = 256 * pair + col[i];
+      xr[i] = *reinterpret_cast<const raw4*>(xp[i] + (k < a.K ? k : 0));  // (behind the columns, whose scales are 0, any x of the row will do)
+    }
+  };
+  auto store = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < XN; ++i) img[buf][to[i]] = xr[i];
+  };
+  auto compute = [&](const Chunk& c, const raw4* x) __attribute__((always_inline)) {
+#pragma unroll
+    for (int g = 0; g < GC; ++g) {
+      f32x4 xs[T], part[RT][T];
+#pragma unroll
+      for (int t = 0; t < T; ++t) {
+        xs[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < RT; ++i) part[i][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+#pragma unroll
+      for (int s = g * GS; s < (g + 1) * GS; ++s) {
+        bf16x8_t w[RT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) w[i] = codes_bf16(c.w[i][s], base);
+#pragma unroll
+        for (int t = 0; t < T; ++t) {
+          const bf16x8_t f = __builtin_bit_cast(bf16x8_t, x[(16 * t + r) * 32 + ((16 * half + 4 * s + q) ^ r)]);
+          xs[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, __builtin_bit_cast(bf16x8_t, kOnes), xs[t], 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < RT; ++i) part[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f, w[i], part[i][t], 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        const float sc = g & 1 ? bf16hi(c.s[i][g >> 1]) : bf16lo(c.s[i][g >> 1]);
+        const float zc = ZERO ? (float)((c.z[i] >> (8 * g)) & 0xffu) : 136.f;
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[i][t][e] += sc * (part[i][t][e] - zc * xs[t][e]);
+      }
+    }
+  };
+  if (n > 0) {
+    Chunk c[2];
+    load(0, c[0]);
+    store(0);
+    __syncthreads();
+    auto turn = [&](auto now_, int j) __attribute__((always_inline)) {
+      constexpr int now = decltype(now_)::value;
+      load(j + 1, c[now ^ 1]);
+      __builtin_amdgcn_sched_barrier(0);
+      if (2 * (first + j * step) + half < a.chunks) compute(c[now], img[now]);
+      __builtin_amdgcn_sched_barrier(0);
+      store(now ^ 1);
+      __syncthreads();
+    };
+    for (int j = 0; j < n; j += 2) {
+      turn(std::integral_constant<int, 0>{}, j);
+      if (j + 1 < n) turn(std::integral_constant<int, 1>{}, j + 1);
+    }
+  }
+  // the second half's sums to the first; lane (q, r): tokens 4 q + e of row r
+  f32x4* red = reinterpret_cast<f32x4*>(img);
+  __syncthreads();
+  if (half) {
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+      for (int t = 0; t < T; ++t) red[(((wid & 3) * RT + i) * T + t) * 64 + lane] = acc[i][t];
+  }
+  __syncthreads();
+  if (half) return;
+#pragma unroll
+  for (int i = 0; i < RT; ++i)
+#pragma unroll
+    for (int t = 0; t < T; ++t) {
+      acc[i][t] += red[((wid * RT + i) * T + t) * 64 + lane];
+      const int row = 16 * (nt0 + i) + r;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int tok = m0 + 16 * t + 4 * q + e;
+        if (row < a.N && tok < a.M) {
+          if (gridDim.z == 1) a.y[(int64_t)tok * a.ldy + row] = f32_to_bf16(acc[i][t][e]);
+          else a.ws[((int64_t)blockIdx.z * a.M + tok) * a.N + row] = acc[i][t][e];
+        }
+      }
+    }
+}
+
 // y = the splits' sums, in their order
 __global__ void __launch_bounds__(256) w4_sum_kernel(bf16_t* __restrict__ y, int64_t ldy, const float* __restrict__ ws, int M, int N, int splits) {
   const int n = blockIdx.x * 256 + threadIdx.x, m = blockIdx.y;
@@ -207,6 +359,25 @@ template <int RT, int T, int E> int launch_group(const W4Args& a, int group, int
   return -1;
 }
 
+template <int T> int launch_wide(const W4Args& a, int group, int splits, hipStream_t st) {
+  const dim3 grid(((a.N + 15) / 16 + 7) / 8, (a.M + 16 * T - 1) / (16 * T), splits);
+  const bool z = a.z != nullptr;
+#define DX_W4W(GS)                                                  \
+  do {                                                              \
+    if (z) w4_wide_kernel<T, GS, true><<<grid, 512, 0, st>>>(a);    \
+    else w4_wide_kernel<T, GS, false><<<grid, 512, 0, st>>>(a);     \
+  } while (0)
+  switch (group) {
+    case 32: DX_W4W(1); break;
+    case 64: DX_W4W(2); break;
+    case 128: DX_W4W(4); break;
+    default: return -1;
+  }
+#undef DX_W4W
+  if (splits > 1) w4_sum_kernel<<<dim3((a.N + 255) / 256, a.M), 256, 0, st>>>(a.y, a.ldy, a.ws, a.M, a.N, splits);
+  return (int)hipGetLastError();
+}
+
 }  // namespace
 
 extern "C" int dx_w4_gemm(void* y, int64_t ldy, const void* x, int64_t ldx, const void* w, const void* s, const void* z, float* ws, int M, int N, int K,
@@ -225,9 +396,7 @@ extern "C" int dx_w4_gemm(void* y, int64_t ldy, const void* x, int64_t ldx, cons
   if (M <= 4) DX_W4(1, 1);
   if (M <= 8) DX_W4(1, 2);
   if (M <= 16) DX_W4(1, 4);
-  if (M <= 32) DX_W4(2, 4);
-  if (rt == 4) rt = 2;
-  if (rt == 2) return launch_group<2, 4, 4>(a, group, waves, splits, stream);
-  return launch_group<1, 4, 4>(a, group, waves, splits, stream);
+  if (splits < 1 || (splits > 1 && ws == nullptr)) return -3;
+  return M <= 32 ? launch_wide<2>(a, group, splits, stream) : launch_wide<4>(a, group, splits, stream);
 #undef DX_W4
 }
