@@ -561,7 +561,7 @@ def test_captured_step_replays():
         step()
         torch.cuda.synchronize()
         graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph):
+        with torch.inference_mode(), torch.cuda.graph(graph):
             step()
         graphs.append((graph, st, step, table, k8, v8, scales))
     g = torch.Generator().manual_seed(4)
