@@ -39,7 +39,7 @@ int dx_decode_attention(void*, float*, float*, const void*, int64_t, const void*
 int dx_prefill_attention(void*, const void*, int64_t, const void*, const void*, const int*, int, const int*,
                          const int*, const int*, int, int, int, int, int, float, int, int, hipStream_t);
 int dx_prefill_tile_tokens(int, int, int);
-int dx_block_append(const void*, const void*, const void*, int64_t, void*, int64_t, const void*, int, const float*, const float*,
+int dx_block_append(const void*, const void*, const void*, int64_t, void*, int64_t, const void*, int, const float*, int, const float*,
                     const int64_t*, void*, void*, float*, float*, int, int, int, int, int, int, int, int, hipStream_t);
 int dx_block_dequant(const void*, const void*, const float*, const float*, void*, void*, const int*, int, const int*, const int*, int,
                      int, int, int, int, int, int, int, hipStream_t);
@@ -140,9 +140,9 @@ PYBIND11_MODULE(_C_kernels, m) {
           "prefill_attention");
   });
   m.def("prefill_tile_tokens", &dx_prefill_tile_tokens);
-  m.def("block_append", [](u q, u k, u v, int64_t stride, u qo, int64_t qos, u pos, int pos_i64, u cs, u rs, u slots, u kc, u vc, u ks,
+  m.def("block_append", [](u q, u k, u v, int64_t stride, u qo, int64_t qos, u pos, int pos_i64, u cs, int n_pos, u rs, u slots, u kc, u vc, u ks,
                            u vs, int tokens, int hq, int hkv, int hd, int bs, int nb, int rotate_q, int code, u st) {
-    check(dx_block_append(P(q), P(k), P(v), stride, P(qo), qos, P(pos), pos_i64, (const float*)cs, (const float*)rs,
+    check(dx_block_append(P(q), P(k), P(v), stride, P(qo), qos, P(pos), pos_i64, (const float*)cs, n_pos, (const float*)rs,
                           (const int64_t*)slots, P(kc), P(vc), (float*)ks, (float*)vs, tokens, hq, hkv, hd, bs, nb, rotate_q, code, S(st)),
           "block_append");
   });

@@ -62,11 +62,12 @@ struct AppendArgs {
   float *k_scales, *v_scales;
   int64_t stride, q_out_stride;
   int64_t num_slots;
-  int tokens, n_q, n_kv, bs_shift, pos_i64, rotate_q, units_x, window;
+  int tokens, n_q, n_kv, bs_shift, pos_i64, rotate_q, units_x, window, last_position;
 };
 
 __device__ __forceinline__ int64_t position(const AppendArgs& g, int64_t t) {
-  return g.pos_i64 ? static_cast<const int64_t*>(g.positions)[t] : (int64_t)static_cast<const int32_t*>(g.positions)[t];
+  const int64_t p = g.pos_i64 ? static_cast<const int64_t*>(g.positions)[t] : (int64_t)static_cast<const int32_t*>(g.positions)[t];
+  return min(max(p, (int64_t)0), (int64_t)g.last_position);  // (a row of the table, whatever is asked for)
 }
 
 // one run: by a workgroup, or (WAVE) n rows by a wave
@@ -313,10 +314,12 @@ __global__ void __launch_bounds__(kThreads)
 // code: 0 int8, 1 e4m3fn.  q, k, v: bf16 rows `stride` elements apart, 16-byte aligned; q_out nullptr: K and V alone;
 // slots nullptr: Q alone.
 extern "C" int dx_block_append(const void* q, const void* k, const void* v, int64_t stride, void* q_out, int64_t q_out_stride,
-                               const void* positions, int pos_i64, const float* cos_sin, const float* row_scale, const int64_t* slots,
+                               const void* positions, int pos_i64, const float* cos_sin, int n_positions, const float* row_scale, const int64_t* slots,
                                void* k_codes, void* v_codes, float* k_scales, float* v_scales, int tokens, int n_q, int n_kv,
                                int head_dim, int block_size, int num_blocks, int rotate_q, int code, hipStream_t stream) {
-  if (head_dim != D || block_size < 16 || block_size > kMostBlock || (block_size & (block_size - 1)) || stride % 8 || q_out_stride % 8) return -1;
+  if (head_dim != D || block_size < 16 || block_size > kMostBlock || (block_size & (block_size - 1)) || stride % 8 || q_out_stride % 8 ||
+      (cos_sin != nullptr && n_positions < 1))
+    return -1;
   if (tokens <= 0) return 0;
   AppendArgs g{};
   g.q = (const bf16_t*)q, g.k = (const bf16_t*)k, g.v = (const bf16_t*)v, g.q_out = (bf16_t*)q_out;
@@ -325,7 +328,7 @@ extern "C" int dx_block_append(const void* q, const void* k, const void* v, int6
   g.stride = stride, g.q_out_stride = q_out_stride;
   g.tokens = tokens, g.n_q = n_q, g.n_kv = n_kv, g.bs_shift = __builtin_ctz((unsigned)block_size);
   g.num_slots = (int64_t)num_blocks << g.bs_shift;
-  g.pos_i64 = pos_i64, g.rotate_q = rotate_q;
+  g.pos_i64 = pos_i64, g.rotate_q = rotate_q, g.last_position = n_positions - 1;
   g.window = tokens > 512 ? 32 : 4;
   const int64_t units = slots ? (int64_t)((tokens + g.window - 1) / g.window) * 2 * n_kv : 0;
   const int64_t grid = units + (q_out ? (tokens + 3) / 4 : 0);

@@ -241,19 +241,21 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
       }
     }
     // a score's factor, and what its exponent is short of: one of a tile, or one each 16 keys (group 2 sub + s2 of this wave's)
+    // (a factor is never 0: a masked score is -infinity times it)
     float sc[2][2], lg[2][2];
     uint32_t one[2][2];
+    auto factor = [&](float ks) __attribute__((always_inline)) { return fmaxf(q_unit * ks, 0x1p-126f); };
 #pragma unroll
     for (int sub = 0; sub < SUBS; ++sub)
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
         if constexpr (ONE) {
-          sc[sub][s2] = q_unit * ks_now[0], lg[sub][s2] = part_log[0], one[sub][s2] = ones[0];
+          sc[sub][s2] = factor(ks_now[0]), lg[sub][s2] = part_log[0], one[sub][s2] = ones[0];
         } else if constexpr (KW == 1) {
-          sc[sub][s2] = q_unit * ks_now[NG > 1 ? 2 * sub + s2 : 0], lg[sub][s2] = part_log[NG > 1 ? 2 * sub + s2 : 0], one[sub][s2] = ones[NG > 1 ? 2 * sub + s2 : 0];
+          sc[sub][s2] = factor(ks_now[NG > 1 ? 2 * sub + s2 : 0]), lg[sub][s2] = part_log[NG > 1 ? 2 * sub + s2 : 0], one[sub][s2] = ones[NG > 1 ? 2 * sub + s2 : 0];
         } else {
           constexpr int kHi = NG > 2 ? 2 : 0;
-          sc[sub][s2] = q_unit * (kw ? ks_now[kHi + (NG > 1 ? s2 : 0)] : ks_now[NG > 1 ? s2 : 0]);
+          sc[sub][s2] = factor(kw ? ks_now[kHi + (NG > 1 ? s2 : 0)] : ks_now[NG > 1 ? s2 : 0]);
           lg[sub][s2] = kw ? part_log[kHi + (NG > 1 ? s2 : 0)] : part_log[NG > 1 ? s2 : 0];
           one[sub][s2] = kw ? ones[kHi + (NG > 1 ? s2 : 0)] : ones[NG > 1 ? s2 : 0];
         }

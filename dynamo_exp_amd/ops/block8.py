@@ -74,7 +74,7 @@ def _check_on(device, **tensors):
 
 def append(q, k, v, positions, cos_sin, slot_mapping, k_cache, v_cache, kv_scales, rotate_q=True, q_out=None, row_scale=None):
     """Rotate, quantise and append.  q [T, Hq, 128] (or None), k, v [T, Hkv, 128] bf16 views whose tokens lie equally far apart;
-    cos_sin None: as they come.  q_out [T, Hq, 128] takes the rotated q (it may be q).
+    cos_sin None: as they come; a position past its rows takes the last one.  q_out [T, Hq, 128] takes the rotated q (it may be q).
 
     slot_mapping [T] int64: block * BS + offset, negative (or past the cache) for rows that have no place.  Tokens that go into one
     block lie behind one another, at offsets that rise by one; what the block holds in front of them belongs to the sequence, what
@@ -117,7 +117,7 @@ def append_rows(qp, kp, vp, T, stride, nq, hkv, qop, q_out_stride, positions, co
         raise ValueError("append: rows are 16-byte aligned")
     dev = k_cache.device
     if cos_sin is not None:
-        if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or cos_sin.shape[1] != d or not cos_sin.is_contiguous() or cos_sin.data_ptr() % 16:
+        if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or cos_sin.shape[0] < 1 or cos_sin.shape[1] != d or not cos_sin.is_contiguous() or cos_sin.data_ptr() % 16:
             raise ValueError("append: cos_sin is [positions, 128] float32, contiguous")
         if positions.dtype not in (torch.int64, torch.int32) or positions.dim() != 1 or positions.shape[0] != T or not positions.is_contiguous():
             raise ValueError("append: positions are [T] int64 or int32, contiguous")
@@ -130,14 +130,15 @@ def append_rows(qp, kp, vp, T, stride, nq, hkv, qop, q_out_stride, positions, co
         raise ValueError("append: row_scale is [T] float32, contiguous, on the cache's device")
     _native.kernels().block_append(
         qp, kp, vp, stride, qop, q_out_stride, positions.data_ptr() if cos_sin is not None else 0,
-        int(cos_sin is not None and positions.dtype == torch.int64), 0 if cos_sin is None else cos_sin.data_ptr(),
+        int(cos_sin is not None and positions.dtype == torch.int64), 0 if cos_sin is None else cos_sin.data_ptr(), 0 if cos_sin is None else cos_sin.shape[0],
         0 if row_scale is None else row_scale.data_ptr(), 0 if slot_mapping is None else slot_mapping.data_ptr(), k_cache.data_ptr(),
         v_cache.data_ptr(), kv_scales[0].data_ptr(), kv_scales[1].data_ptr(), T, nq, hkv, d, bs, nb, int(rotate_q), CODES[k_cache.dtype],
         _stream(k_cache))
 
 
 def read_back(k_cache, v_cache, kv_scales, block_tables, ctx_lens, scratch, workspaces):
-    """ops.kv_dequant_scratch of a block-scaled cache."""
+    """ops.kv_dequant_scratch of a block-scaled cache.  K and V lie in a workspace of the stream, which its next call writes again; a
+    captured call has one of its own."""
     _check_cache(k_cache, v_cache, kv_scales)
     nb, hkv, bs, d = k_cache.shape
     n, cols = block_tables.shape
@@ -148,13 +149,23 @@ def read_back(k_cache, v_cache, kv_scales, block_tables, ctx_lens, scratch, work
     dev = k_cache.device
     if block_tables.device != dev or ctx_lens.device != dev:
         raise ValueError(f"kv_dequant_scratch: tables on {block_tables.device}, lengths on {ctx_lens.device}, the cache on {dev}")
-    stream = _stream(k_cache)
+    if not k_cache.is_cuda:
+        table = torch.arange(n * cols, dtype=torch.int32).view(n, cols) if scratch is None else scratch[0]
+        ks, vs = (torch.zeros((max(n * cols if scratch is None else scratch[1], 1), hkv, bs, d), dtype=torch.bfloat16) for _ in range(2))
+        for i, ctx in enumerate(ctx_lens.tolist()):
+            need = min(-(-ctx // bs), cols)
+            src, dst = block_tables[i, :need].long(), table[i, :need].long()
+            ks[dst] = ref.block_values(k_cache[src], kv_scales[0][src]).bfloat16()
+            vs[dst] = ref.block_values(v_cache[src], kv_scales[1][src]).bfloat16()
+        return ks, vs, table
+    stream, captured = _stream(k_cache), torch.cuda.is_current_stream_capturing()
     need = n * cols if scratch is None else scratch[1]
-    ws = workspaces.get((dev, stream))
+    ws = None if captured else workspaces.get((dev, stream))
     if ws is None or ws[0].shape[0] < need or ws[0].shape[1:] != k_cache.shape[1:]:
         cap = max(need, 64)
         ws = (*(torch.empty((cap, hkv, bs, d), dtype=torch.bfloat16, device=dev) for _ in range(2)), torch.arange(cap, dtype=torch.int32, device=dev))
-        workspaces[(dev, stream)] = ws
+        if not captured:
+            workspaces[(dev, stream)] = ws
     ks, vs = (ws[0], ws[1]) if ws[0].shape[0] == need else (ws[0][:max(need, 1)], ws[1][:max(need, 1)])
     if scratch is None:
         table = ws[2].as_strided((n, cols), (cols, 1))
@@ -172,6 +183,8 @@ def _check_reader(q, out, k_cache, v_cache, kv_scales, block_tables, ctx_lens, n
     _check_cache(k_cache, v_cache, kv_scales)
     T, hq, d = q.shape
     hkv = k_cache.shape[1]
+    if k_cache.shape[0] < 1:
+        raise ValueError("attention over a block-scaled cache: the cache has no block")
     if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
         raise TypeError("attention over a block-scaled cache: q and out are bfloat16")
     if d != HEAD_DIM or hq % hkv or out.shape != q.shape or not out.is_contiguous():
@@ -335,6 +348,8 @@ def prefill(q, k_cache, v_cache, block_tables, cu_seqlens_q, ctx_lens, scale, ou
     if (plan.rows, plan.sequences, plan.n_q, plan.n_kv, plan.causal) != (T, n, hq, hkv, causal):
         raise ValueError(f"prefill_attention: a plan of {plan.rows} rows, {plan.sequences} sequences, {plan.n_q} / {plan.n_kv} heads, causal "
                          f"{plan.causal} for {T}, {n}, {hq} / {hkv}, {causal}")
+    if not scale >= 0:
+        raise ValueError(f"prefill_attention: scale {scale}, over a block-scaled cache it is not negative")
     _check_on(q.device, cu_seqlens_q=cu_seqlens_q, work=plan.work)
     o = ml = few_o = few_ml = 0
     tiles, few = plan.places * hkv * plan.tile, plan.few_places * hkv * FEW_ROWS

@@ -153,7 +153,7 @@ def block_values(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
 def block_append(q, k, v, positions, cos_sin, slot_mapping, k_cache, v_cache, kv_scales, rotate_q=True, q_out=None, row_scale=None):
     """The append to a block-scaled cache (ops.block8.append), run by run."""
     rows = lambda x: x.float() if row_scale is None else x.float() * row_scale[:, None, None]  # noqa: E731
-    turn = (lambda x: apply_rope(x, positions, cos_sin)) if cos_sin is not None else (lambda x: x)
+    turn = (lambda x: apply_rope(x, positions.clamp(0, cos_sin.shape[0] - 1), cos_sin)) if cos_sin is not None else (lambda x: x)
     kf, vf = turn(rows(k)), rows(v)
     if q is not None:
         q_out = q if q_out is None else q_out

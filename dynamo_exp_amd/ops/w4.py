@@ -129,15 +129,19 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, out: torch.Tensor | None = None
     if m and (x.stride(1) != 1 or (m > 1 and x.stride(0) % 8) or x.data_ptr() % 16):
         raise ValueError("w4_linear: rows of x have unit stride and are 16-byte aligned")
     dev = torch._C._cuda_getDevice()
-    if x.device.index != dev or weight.packed.device != x.device:
-        raise ValueError(f"w4_linear: x on {x.device}, the weight on {weight.packed.device}, current device cuda:{dev}")
+    p, s, z, n, k, group = weight
+    if x.device.index != dev or p.device != x.device or s.device != x.device or (z is not None and z.device != x.device):
+        raise ValueError(f"w4_linear: x on {x.device}, the weight on {p.device}, current device cuda:{dev}")
+    chunks = -(-n // 16) * -(-k // 128)
+    if p.numel() != 256 * chunks or s.numel() * group != 2048 * chunks or (z is not None and z.numel() != s.numel()):
+        raise ValueError(f"w4_linear: a weight {(n, k)} in groups of {group} laid out as {tuple(p.shape)} and {tuple(s.shape)}")
     if out is None:
-        out = torch.empty((m, weight.n), dtype=x.dtype, device=x.device)
-    elif out.shape != (m, weight.n) or out.dtype != x.dtype or out.device != x.device or (m and out.stride(1) != 1):
+        out = torch.empty((m, n), dtype=x.dtype, device=x.device)
+    elif out.shape != (m, n) or out.dtype != x.dtype or out.device != x.device or (m and out.stride(1) != 1):
         raise ValueError("w4_linear: bad out tensor")
-    waves, rt, splits = _shape(m, weight.n, weight.k)
-    ws = torch.empty(splits * m * weight.n, dtype=torch.float32, device=x.device) if splits > 1 and m else None
-    _native.kernels().w4_gemm(out.data_ptr(), out.stride(0), x.data_ptr(), x.stride(0) if m > 1 else 0, weight.packed.data_ptr(),
-                              weight.scales.data_ptr(), 0 if weight.zeros is None else weight.zeros.data_ptr(), 0 if ws is None else ws.data_ptr(), m, weight.n, weight.k, weight.group, waves, rt, splits,
+    waves, rt, splits = _shape(m, n, k)
+    ws = torch.empty(splits * m * n, dtype=torch.float32, device=x.device) if splits > 1 and m else None
+    _native.kernels().w4_gemm(out.data_ptr(), out.stride(0), x.data_ptr(), x.stride(0) if m > 1 else 0, p.data_ptr(), s.data_ptr(),
+                              0 if z is None else z.data_ptr(), 0 if ws is None else ws.data_ptr(), m, n, k, group, waves, rt, splits,
                               torch._C._cuda_getCurrentRawStream(dev))
     return out

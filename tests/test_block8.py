@@ -753,3 +753,108 @@ def test_append_rows_without_a_place_between(codes):
         got.append([t.cpu() for t in (k8, v8, *scales)])
     for a, b in zip(*got):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bs", [16, 64])
+def test_prefill_tiny_scores_beside_a_block_of_zeros(bs):
+    """Keys of zeros (scale 2^-126) behind queries of 2^-40: a score's factor is no number that fp32 holds, and masked scores are
+    infinities times it."""
+    nq, nkv, new, ctx = 8, 2, [90], [200]
+    table, k8, v8, ks, vs = cache_of("int8", nkv, bs, ctx, 5)
+    for j in range(-(-ctx[0] // bs)):
+        if j != 1:
+            bits(k8)[int(table[0, j])] = 0
+            ks[int(table[0, j])] = 2.0 ** -126
+    q = (torch.randn((90, nq, D), generator=torch.Generator().manual_seed(3)) * 2.0 ** -40).bfloat16()
+    cu = torch.tensor([0, 90], dtype=torch.int32)
+    out = torch.empty((90, nq, D), dtype=torch.bfloat16, device="cuda")
+    dev = on_gpu(q, k8, v8, table, cu, torch.tensor(ctx, dtype=torch.int32))
+    ops.prefill_attention(*dev, SCALE, out, work=ops.prefill_plan(new, ctx, nq, nkv), kv_scales=tuple(on_gpu(ks, vs)))
+    near(out.cpu(), *attention64(q, k8, v8, ks, vs, table, new, ctx), 2, fp16_floor(ctx, v8, vs))
+
+
+@pytest.mark.gpu
+@both
+@pytest.mark.parametrize("T", [3, 600])
+def test_positions_past_the_table(codes, T):
+    """A position that cos_sin has no row for takes its last (or first) one."""
+    cs = ref.rope_cos_sin(D, 50, 500000.0)
+    qkv = torch.randn((T, 4 * D), generator=torch.Generator().manual_seed(T)).bfloat16()
+    slots = torch.arange(T)
+    wild = torch.where(torch.arange(T) % 3 == 0, 2 ** 40, -(2 ** 33))
+    got = []
+    for pos in (wild, torch.where(torch.arange(T) % 3 == 0, 49, 0), torch.where(torch.arange(T) % 3 == 0, 2 ** 31 - 1, -5).int()):
+        k8, v8, scales = block8.alloc(40, 1, 16, CODES[codes])
+        row = qkv.cuda()
+        ops.rope_cache(row, pos.cuda(), cs.cuda(), slots.cuda(), k8, v8, 2, 1, D, 16, kv_scales=scales)
+        got.append([t.cpu().view(torch.uint8) for t in (row, k8, v8, *scales)])
+    for other in got[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got[0], other))
+
+
+@both
+def test_read_back_cpu(codes):
+    k8, ks = random_cache(9, 3, 32, CODES[codes], 4)
+    v8, vs = random_cache(9, 3, 32, CODES[codes], 5, pow2=False)
+    table, ctx = torch.tensor([[4, 2, 8], [0, 7, 1]], dtype=torch.int32), torch.tensor([65, 31], dtype=torch.int32)
+    packed = torch.tensor([[0, 1, 2], [3, 0, 0]], dtype=torch.int32)
+    for scratch in (None, (packed, 4)):
+        gk, gv, t = ops.kv_dequant_scratch(k8, v8, table, ctx, kv_scales=(ks, vs), scratch=scratch)
+        for i, n in ((0, 3), (1, 1)):
+            for j in range(n):
+                b, to = int(table[i, j]), int(t[i, j])
+                assert torch.equal(gk[to], ref.block_values(k8[b], ks[b]).bfloat16())
+                assert torch.equal(gv[to], ref.block_values(v8[b], vs[b]).bfloat16())
+
+
+@pytest.mark.gpu
+def test_captured_read_back_has_its_own_workspace():
+    """A graph's copies lie in memory of the graph: eager calls, small and so large that their workspace is made anew, leave them, and
+    two graphs leave each other's."""
+    k8, ks = random_cache(200, 2, 16, torch.int8, 4)
+    v8, vs = random_cache(200, 2, 16, torch.int8, 5)
+    dev = on_gpu(k8, v8)
+    scales = tuple(on_gpu(ks, vs))
+    tables = [torch.arange(n, dtype=torch.int32, device="cuda").view(1, n) + at for at, n in ((3, 5), (20, 7))]
+    lens = [torch.tensor([16 * t.shape[1]], dtype=torch.int32, device="cuda") for t in tables]
+    call = lambda t, n: ops.kv_dequant_scratch(*dev, t, n, kv_scales=scales)  # noqa: E731
+    s = torch.cuda.Stream()
+    with torch.inference_mode(), torch.cuda.stream(s):
+        call(tables[0], lens[0])
+        s.synchronize()
+        graphs = []
+        for t, n in zip(tables, lens):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=s):
+                got = call(t, n)
+            graphs.append((graph, got))
+        for turn in range(3):
+            for graph, _ in graphs:
+                graph.replay()
+            s.synchronize()
+            held = [[x.clone() for x in got[:2]] for _, got in graphs]
+            wide = torch.arange(70 + 40 * turn, dtype=torch.int32, device="cuda").view(1, -1) + 10
+            eager = call(wide, torch.tensor([16 * wide.shape[1]], dtype=torch.int32, device="cuda"))
+            s.synchronize()
+            assert torch.equal(eager[0][0].cpu(), ref.block_values(k8[10], ks[10]).bfloat16())
+            for (_, got), old, t in zip(graphs, held, tables):
+                b = t[0].cpu().long()
+                for x, o, codes, sc in zip(got, old, (k8, v8), (ks, vs)):
+                    assert torch.equal(x[:len(b)], o[:len(b)]) and torch.equal(x[:len(b)].cpu(), ref.block_values(codes[b], sc[b]).bfloat16())
+
+
+def test_readers_refuse_a_cache_without_blocks():
+    k8, v8, scales = block8.alloc(0, 2, 16, torch.int8, "cpu")
+    q = torch.zeros((1, 4, D), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="no block"):
+        block8._check_reader(q, q.clone(), k8, v8, scales, torch.zeros((1, 1), dtype=torch.int32), torch.ones(1, dtype=torch.int32), 1)
+
+
+def test_prefill_refuses_a_negative_scale():
+    k8, v8, scales = block8.alloc(4, 2, 16, torch.int8, "cpu")
+    q = torch.zeros((3, 4, D), dtype=torch.bfloat16)
+    cu, ctx, bt = torch.tensor([0, 3], dtype=torch.int32), torch.tensor([3], dtype=torch.int32), torch.zeros((1, 1), dtype=torch.int32)
+    for scale in (-SCALE, NAN):
+        with pytest.raises(ValueError, match="not negative"):
+            block8.prefill(q, k8, v8, bt, cu, ctx, scale, q.clone(), ops.prefill_plan([3], [3], 4, 2, "cpu"), scales, True)

@@ -168,3 +168,14 @@ def test_refusals_gpu():
         ops.w4_linear(b(2, 128), weight, b(2, 17))
     with pytest.raises(ValueError):
         ops.w4_linear(b(2, 128), ops.w4_pack(codes, scales, z, 32))
+
+
+@pytest.mark.gpu
+def test_refuses_a_weight_laid_out_otherwise():
+    codes, scales, z, _ = make(48, 256, 32, True)
+    w = ops.w4_pack(codes.cuda(), scales.cuda(), z.cuda(), 32)
+    x = torch.zeros((2, 256), dtype=torch.bfloat16, device="cuda")
+    for bad in (w._replace(packed=w.packed[:2]), w._replace(scales=w.scales[:, :1]), w._replace(zeros=w.zeros[:1]), w._replace(n=64), w._replace(group=64),
+                w._replace(scales=w.scales.cpu()), w._replace(zeros=w.zeros.cpu())):
+        with pytest.raises(ValueError):
+            ops.w4_linear(x, bad)
