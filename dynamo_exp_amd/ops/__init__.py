@@ -174,23 +174,23 @@ def rope_cache(qkv, positions, cos_sin, slot_mapping, k_cache, v_cache, n_q, n_k
         if isinstance(qkv, SplitK):
             qkv = splitk_reduce(qkv)
         q_end, k_end = n_q * head_dim, (n_q + n_kv) * head_dim
-        if qkv.dim() != 2 or qkv.shape[1] != k_end + n_kv * head_dim or k_cache.shape[2] != block_size:
-            raise ValueError(f"rope_cache: qkv {tuple(qkv.shape)} for {n_q} + 2 x {n_kv} heads of {head_dim}, blocks of {block_size}")
-        T, rows = qkv.shape[0], qkv.stride(0)
+        shape = qkv.shape
+        if len(shape) != 2 or shape[1] != k_end + n_kv * head_dim or k_cache.shape[2] != block_size:
+            raise ValueError(f"rope_cache: qkv {tuple(shape)} for {n_q} + 2 x {n_kv} heads of {head_dim}, blocks of {block_size}")
         if not qkv.is_cuda:
             q, k, v = (t.unflatten(1, (-1, head_dim)) for t in (qkv[:, :q_end], qkv[:, q_end:k_end], qkv[:, k_end:]))
             block8.append(q, k, v, positions, cos_sin, slot_mapping, k_cache, v_cache, kv_scales, rotate_q,
-                          None if out is None else out.view(T, n_q, head_dim), row_scale)
+                          None if out is None else out.view(-1, n_q, head_dim), row_scale)
             return qkv if out is None else out
-        to = qkv if out is None else out
+        to, T, rows = qkv if out is None else out, shape[0], qkv.stride()
         if qkv.dtype != torch.bfloat16 or to.dtype != torch.bfloat16:
             raise TypeError("rope_cache: rows are bfloat16")
-        if T and (qkv.stride(1) != 1 or (out is not None and (out.shape != (T, q_end) or out.stride(1) != 1))):
+        if T and (rows[1] != 1 or (out is not None and (out.shape != (T, q_end) or out.stride(1) != 1))):
             raise ValueError("rope_cache: rows of unit stride, out [T, n_q * head_dim]")
-        dev, p = k_cache.device, qkv.data_ptr()
-        if qkv.device != dev or to.device != dev or head_dim != block8.HEAD_DIM:
-            raise ValueError(f"rope_cache: rows on {qkv.device}, out on {to.device}, the cache on {dev}; heads of {head_dim}")
-        block8.append_rows(p, p + 2 * q_end, p + 2 * k_end, T, rows if T > 1 else 0, n_q, n_kv, to.data_ptr(), to.stride(0) if T > 1 else 0,
+        dev, p = k_cache.get_device(), qkv.data_ptr()
+        if qkv.get_device() != dev or to.get_device() != dev or head_dim != block8.HEAD_DIM:
+            raise ValueError(f"rope_cache: rows on {qkv.device}, out on {to.device}, the cache on {k_cache.device}; heads of {head_dim}")
+        block8.append_rows(p, p + 2 * q_end, p + 2 * k_end, T, rows[0] if T > 1 else 0, n_q, n_kv, to.data_ptr(), to.stride(0) if T > 1 else 0,
                            positions, cos_sin, slot_mapping, k_cache, v_cache, kv_scales, rotate_q, row_scale)
         return qkv if out is None else out
     if row_scale is not None:

@@ -41,19 +41,24 @@ def alloc(num_blocks: int, n_kv: int, block_size: int, dtype=torch.int8, device=
 
 def _stream(t: torch.Tensor) -> int:
     dev = torch._C._cuda_getDevice()
-    if t.device.index != dev:
+    if t.get_device() != dev:
         raise ValueError(f"block-scaled cache: tensors on {t.device}, current device is cuda:{dev}")
     return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _check_cache(k, v, kv_scales):
+    """(blocks, heads, tokens of a block, device's number).  (A call of few tokens takes its checks as long as its kernel: what is asked of
+    a tensor is asked once.)"""
     ks, vs = kv_scales
-    if k.dtype not in CODES or v.dtype != k.dtype:
+    dtype = k.dtype
+    if dtype not in CODES or v.dtype is not dtype:
         raise TypeError(f"block-scaled cache: int8 or float8_e4m3fn codes, got {k.dtype} and {v.dtype}")
-    if ks.dtype != torch.float32 or vs.dtype != torch.float32:
+    if ks.dtype is not torch.float32 or vs.dtype is not torch.float32:
         raise TypeError("block-scaled cache: scales are float32")
-    nb, hkv, bs, d = k.shape
-    if v.shape != k.shape or ks.shape != (nb, hkv) or vs.shape != (nb, hkv):
+    shape = k.shape
+    nb, hkv, bs, d = shape
+    heads = (nb, hkv)
+    if v.shape != shape or ks.shape != heads or vs.shape != heads:
         raise ValueError(f"block-scaled cache: codes {tuple(k.shape)} {tuple(v.shape)}, scales {tuple(ks.shape)} {tuple(vs.shape)}")
     if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
         raise ValueError("block-scaled cache: codes and scales are contiguous")
@@ -61,9 +66,10 @@ def _check_cache(k, v, kv_scales):
         raise ValueError(f"block-scaled cache: heads of {HEAD_DIM}, blocks of 16, 32, 64 or 128 tokens; got {d} and {bs}")
     if (k.data_ptr() | v.data_ptr()) % 16:
         raise ValueError("block-scaled cache: codes are 16-byte aligned")
-    dev = k.device
-    if v.device != dev or ks.device != dev or vs.device != dev:
+    dev = k.get_device()
+    if v.get_device() != dev or ks.get_device() != dev or vs.get_device() != dev:
         raise ValueError("block-scaled cache: codes and scales on one device")
+    return nb, hkv, bs, dev
 
 
 def _check_on(device, **tensors):
@@ -109,28 +115,30 @@ def append(q, k, v, positions, cos_sin, slot_mapping, k_cache, v_cache, kv_scale
 
 def append_rows(qp, kp, vp, T, stride, nq, hkv, qop, q_out_stride, positions, cos_sin, slot_mapping, k_cache, v_cache, kv_scales, rotate_q, row_scale):
     """append() on rows that the caller has looked at: bf16 at qp, kp, vp, tokens `stride` elements apart, on the cache's device."""
-    _check_cache(k_cache, v_cache, kv_scales)
-    nb, heads, bs, d = k_cache.shape
+    nb, heads, bs, number = _check_cache(k_cache, v_cache, kv_scales)
+    d = HEAD_DIM
     if heads != hkv:
         raise ValueError(f"append: {hkv} heads, the cache has {heads}")
     if (qp | kp | vp | qop) % 16 or stride % 8 or q_out_stride % 8:
         raise ValueError("append: rows are 16-byte aligned")
-    dev = k_cache.device
+    n_cos = 0
     if cos_sin is not None:
-        if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or cos_sin.shape[0] < 1 or cos_sin.shape[1] != d or not cos_sin.is_contiguous() or cos_sin.data_ptr() % 16:
+        table = cos_sin.shape
+        n_cos = table[0]
+        if cos_sin.dtype is not torch.float32 or len(table) != 2 or n_cos < 1 or table[1] != d or not cos_sin.is_contiguous() or cos_sin.data_ptr() % 16:
             raise ValueError("append: cos_sin is [positions, 128] float32, contiguous")
-        if positions.dtype not in (torch.int64, torch.int32) or positions.dim() != 1 or positions.shape[0] != T or not positions.is_contiguous():
+        if positions.dtype not in (torch.int64, torch.int32) or positions.dim() != 1 or positions.numel() != T or not positions.is_contiguous():
             raise ValueError("append: positions are [T] int64 or int32, contiguous")
-        if positions.device != dev or cos_sin.device != dev:
-            raise ValueError(f"append: positions on {positions.device}, cos_sin on {cos_sin.device}, the cache on {dev}")
-    if slot_mapping is not None and (slot_mapping.dtype != torch.int64 or slot_mapping.dim() != 1 or slot_mapping.shape[0] != T
-                                     or not slot_mapping.is_contiguous() or slot_mapping.device != dev):
+        if positions.get_device() != number or cos_sin.get_device() != number:
+            raise ValueError(f"append: positions on {positions.device}, cos_sin on {cos_sin.device}, the cache on {k_cache.device}")
+    if slot_mapping is not None and (slot_mapping.dtype is not torch.int64 or slot_mapping.dim() != 1 or slot_mapping.numel() != T
+                                     or not slot_mapping.is_contiguous() or slot_mapping.get_device() != number):
         raise ValueError("append: slot_mapping is [T] int64, contiguous, on the cache's device")
-    if row_scale is not None and (row_scale.dtype != torch.float32 or row_scale.shape != (T,) or not row_scale.is_contiguous() or row_scale.device != dev):
+    if row_scale is not None and (row_scale.dtype != torch.float32 or row_scale.shape != (T,) or not row_scale.is_contiguous() or row_scale.get_device() != number):
         raise ValueError("append: row_scale is [T] float32, contiguous, on the cache's device")
     _native.kernels().block_append(
         qp, kp, vp, stride, qop, q_out_stride, positions.data_ptr() if cos_sin is not None else 0,
-        int(cos_sin is not None and positions.dtype == torch.int64), 0 if cos_sin is None else cos_sin.data_ptr(), 0 if cos_sin is None else cos_sin.shape[0],
+        int(cos_sin is not None and positions.dtype == torch.int64), 0 if cos_sin is None else cos_sin.data_ptr(), n_cos,
         0 if row_scale is None else row_scale.data_ptr(), 0 if slot_mapping is None else slot_mapping.data_ptr(), k_cache.data_ptr(),
         v_cache.data_ptr(), kv_scales[0].data_ptr(), kv_scales[1].data_ptr(), T, nq, hkv, d, bs, nb, int(rotate_q), CODES[k_cache.dtype],
         _stream(k_cache))
@@ -180,39 +188,38 @@ def read_back(k_cache, v_cache, kv_scales, block_tables, ctx_lens, scratch, work
 
 
 def _check_reader(q, out, k_cache, v_cache, kv_scales, block_tables, ctx_lens, n):
-    _check_cache(k_cache, v_cache, kv_scales)
-    T, hq, d = q.shape
-    hkv = k_cache.shape[1]
-    if k_cache.shape[0] < 1:
+    nb, hkv, bs, dev = _check_cache(k_cache, v_cache, kv_scales)
+    shape = q.shape
+    T, hq, d = shape
+    if nb < 1:
         raise ValueError("attention over a block-scaled cache: the cache has no block")
-    if q.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
+    if q.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16:
         raise TypeError("attention over a block-scaled cache: q and out are bfloat16")
-    if d != HEAD_DIM or hq % hkv or out.shape != q.shape or not out.is_contiguous():
+    if d != HEAD_DIM or hq % hkv or out.shape != shape or not out.is_contiguous():
         raise ValueError(f"attention over a block-scaled cache: q {tuple(q.shape)}, out {tuple(out.shape)}, {hkv} key/value heads")
+    rows = 0
     if T:
         rows, heads, cols = q.stride()
         if cols != 1 or (hq > 1 and heads != d) or (T > 1 and rows % 8) or (q.data_ptr() | out.data_ptr()) % 16:
             raise ValueError("attention over a block-scaled cache: q's heads behind one another, its rows and out 16-byte aligned")
-    if block_tables.dtype != torch.int32 or ctx_lens.dtype != torch.int32:
+    if block_tables.dtype is not torch.int32 or ctx_lens.dtype is not torch.int32:
         raise TypeError("attention over a block-scaled cache: tables and lengths are int32")
-    table = block_tables.shape
-    if (len(table) != 2 or table[0] != n or table[1] < 1 or (table[1] > 1 and block_tables.stride(1) != 1) or ctx_lens.dim() != 1 or
-            ctx_lens.shape[0] != n or not ctx_lens.is_contiguous()):
+    table, strides = block_tables.shape, block_tables.stride()
+    if (len(table) != 2 or table[0] != n or table[1] < 1 or (table[1] > 1 and strides[1] != 1) or ctx_lens.dim() != 1 or
+            ctx_lens.numel() != n or not ctx_lens.is_contiguous()):
         raise ValueError(f"attention over a block-scaled cache: block_tables {tuple(table)}, ctx_lens {tuple(ctx_lens.shape)}, {n} sequences")
-    dev = k_cache.device
-    if q.device != dev or out.device != dev or block_tables.device != dev or ctx_lens.device != dev:
+    if q.get_device() != dev or out.get_device() != dev or block_tables.get_device() != dev or ctx_lens.get_device() != dev:
         raise ValueError(f"attention over a block-scaled cache: q on {q.device}, out on {out.device}, block_tables on {block_tables.device}, "
-                         f"ctx_lens on {ctx_lens.device}, the cache on {dev}")
+                         f"ctx_lens on {ctx_lens.device}, the cache on {k_cache.device}")
+    return T, hq, d, nb, hkv, bs, rows if T > 1 else 0, table[1], strides[0]
 
 
 def decode(q, k_cache, v_cache, block_tables, ctx_lens, scale, out, n_parts, workspace, kv_scales):
-    B, hq, d = q.shape
-    _check_reader(q, out, k_cache, v_cache, kv_scales, block_tables, ctx_lens, B)
-    nb, hkv, bs, _ = k_cache.shape
+    B, hq, d, nb, hkv, bs, rows, cols, table_rows = _check_reader(q, out, k_cache, v_cache, kv_scales, block_tables, ctx_lens, q.shape[0])
     if hq // hkv > MAX_GROUP:
         raise ValueError(f"decode_attention: at most {MAX_GROUP} query heads per key/value head, got {hq // hkv}")
     if n_parts is None:
-        n_parts = decode_parts(B, hkv, block_tables.shape[1] * bs)
+        n_parts = decode_parts(B, hkv, cols * bs)
     if n_parts < 1:
         raise ValueError(f"decode_attention: {n_parts} parts")
     t0 = t1 = 0
@@ -229,9 +236,9 @@ def decode(q, k_cache, v_cache, block_tables, ctx_lens, scale, out, n_parts, wor
                 raise ValueError(f"decode_attention: workspace {tuple(o.shape)} {tuple(ml.shape)} for {(B, hq, n_parts, d)}")
             _check_on(q.device, workspace=o, sums=ml)
             t0, t1 = o.data_ptr(), ml.data_ptr()
-    _native.kernels().block_decode(out.data_ptr(), t0, t1, q.data_ptr(), q.stride(0) if B > 1 else 0, k_cache.data_ptr(), v_cache.data_ptr(),
-                                   kv_scales[0].data_ptr(), kv_scales[1].data_ptr(), block_tables.data_ptr(), block_tables.stride(0),
-                                   block_tables.shape[1], ctx_lens.data_ptr(), B, hq, hkv, d, bs, nb, int(n_parts), float(scale),
+    _native.kernels().block_decode(out.data_ptr(), t0, t1, q.data_ptr(), rows, k_cache.data_ptr(), v_cache.data_ptr(),
+                                   kv_scales[0].data_ptr(), kv_scales[1].data_ptr(), block_tables.data_ptr(), table_rows, cols,
+                                   ctx_lens.data_ptr(), B, hq, hkv, d, bs, nb, int(n_parts), float(scale),
                                    CODES[k_cache.dtype], _stream(q))
     return out
 
@@ -339,10 +346,8 @@ def prefill(q, k_cache, v_cache, block_tables, cu_seqlens_q, ctx_lens, scale, ou
         plan = prefill_plan([b - a for a, b in zip(cu, cu[1:])], ctx_lens.tolist(), q.shape[1], k_cache.shape[1], q.device, causal)
     if not isinstance(plan, PrefillPlan):
         raise TypeError("prefill_attention: over a block-scaled cache `work` is a plan of prefill_plan")
-    T, hq, d = q.shape
-    nb, hkv, bs, _ = k_cache.shape
     n = cu_seqlens_q.shape[0] - 1
-    _check_reader(q, out, k_cache, v_cache, kv_scales, block_tables, ctx_lens, n)
+    T, hq, d, nb, hkv, bs, rows, cols, table_rows = _check_reader(q, out, k_cache, v_cache, kv_scales, block_tables, ctx_lens, n)
     if cu_seqlens_q.dtype != torch.int32 or not cu_seqlens_q.is_contiguous():
         raise TypeError("prefill_attention: cu_seqlens_q is int32, contiguous")
     if (plan.rows, plan.sequences, plan.n_q, plan.n_kv, plan.causal) != (T, n, hq, hkv, causal):
@@ -360,9 +365,9 @@ def prefill(q, k_cache, v_cache, block_tables, cu_seqlens_q, ctx_lens, scale, ou
         ml = few_o + 4 * few * d
         few_ml = ml + 8 * tiles
     work = plan.work.data_ptr()
-    _native.kernels().block_prefill(out.data_ptr(), o, ml, few_o, few_ml, q.data_ptr(), q.stride(0) if T > 1 else 0, k_cache.data_ptr(),
+    _native.kernels().block_prefill(out.data_ptr(), o, ml, few_o, few_ml, q.data_ptr(), rows, k_cache.data_ptr(),
                                     v_cache.data_ptr(), kv_scales[0].data_ptr(), kv_scales[1].data_ptr(), block_tables.data_ptr(),
-                                    block_tables.stride(0), block_tables.shape[1], cu_seqlens_q.data_ptr(), ctx_lens.data_ptr(), work, plan.n_work,
+                                    table_rows, cols, cu_seqlens_q.data_ptr(), ctx_lens.data_ptr(), work, plan.n_work,
                                     plan.n_few, work + 24 * (plan.n_work + plan.n_few), plan.n_joins, plan.n_few_joins, plan.tile, plan.few_groups,
                                     hq, hkv, d, bs, nb, float(scale), int(causal), CODES[k_cache.dtype], _stream(q))
     return out

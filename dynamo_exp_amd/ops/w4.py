@@ -4,6 +4,7 @@
 GPU tensors run csrc/kernels/w4_gemm.hip, CPU tensors PyTorch in fp32."""
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple
 
 import torch
@@ -89,6 +90,7 @@ def w4_unpack(weight: W4Weight) -> torch.Tensor:
     return (c - zeros) * rows(weight.scales)
 
 
+@functools.lru_cache(maxsize=4096)
 def _shape(m: int, n: int, k: int) -> tuple[int, int, int]:
     """(waves of a workgroup, 16-row tiles of weights a wave, workgroups that K is split over).  Tiles share x's way from L2, but need
     workgroups enough for 256 CUs; us with 1, 2 and 4 tiles, groups of 128, one row: 4096 x 4096 (256 tiles of rows) 4.4, 5.0, -;
@@ -116,9 +118,10 @@ def _shape(m: int, n: int, k: int) -> tuple[int, int, int]:
 
 def w4_linear(x: torch.Tensor, weight: W4Weight, out: torch.Tensor | None = None) -> torch.Tensor:
     """y [m, n] = x [m, k] . w^T for up to 256 rows of bf16, sums in fp32."""
-    if x.dim() != 2 or x.shape[1] != weight.k:
-        raise ValueError(f"w4_linear: x {tuple(x.shape)}, weight {(weight.n, weight.k)}")
-    m = x.shape[0]
+    shape, (p, s, z, n, k, group) = x.shape, weight
+    if len(shape) != 2 or shape[1] != k:
+        raise ValueError(f"w4_linear: x {tuple(shape)}, weight {(n, k)}")
+    m = shape[0]
     if not x.is_cuda:
         y = (x.float() @ w4_unpack(weight).t()).to(x.dtype)
         return y if out is None else out.copy_(y)
@@ -126,22 +129,23 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, out: torch.Tensor | None = None
         raise TypeError(f"w4_linear: x is bfloat16, got {x.dtype}")
     if m > MAX_ROWS:
         raise ValueError(f"w4_linear: at most {MAX_ROWS} rows, got {m}")
-    if m and (x.stride(1) != 1 or (m > 1 and x.stride(0) % 8) or x.data_ptr() % 16):
+    rows, cols = x.stride()
+    xp, number = x.data_ptr(), x.get_device()
+    if m and (cols != 1 or (m > 1 and rows % 8) or xp % 16):
         raise ValueError("w4_linear: rows of x have unit stride and are 16-byte aligned")
     dev = torch._C._cuda_getDevice()
-    p, s, z, n, k, group = weight
-    if x.device.index != dev or p.device != x.device or s.device != x.device or (z is not None and z.device != x.device):
+    if number != dev or p.get_device() != dev or s.get_device() != dev or (z is not None and z.get_device() != dev):
         raise ValueError(f"w4_linear: x on {x.device}, the weight on {p.device}, current device cuda:{dev}")
     chunks = -(-n // 16) * -(-k // 128)
     if p.numel() != 256 * chunks or s.numel() * group != 2048 * chunks or (z is not None and z.numel() != s.numel()):
         raise ValueError(f"w4_linear: a weight {(n, k)} in groups of {group} laid out as {tuple(p.shape)} and {tuple(s.shape)}")
     if out is None:
         out = torch.empty((m, n), dtype=x.dtype, device=x.device)
-    elif out.shape != (m, n) or out.dtype != x.dtype or out.device != x.device or (m and out.stride(1) != 1):
+    elif out.shape != (m, n) or out.dtype is not x.dtype or out.get_device() != dev or (m and out.stride(1) != 1):
         raise ValueError("w4_linear: bad out tensor")
     waves, rt, splits = _shape(m, n, k)
     ws = torch.empty(splits * m * n, dtype=torch.float32, device=x.device) if splits > 1 and m else None
-    _native.kernels().w4_gemm(out.data_ptr(), out.stride(0), x.data_ptr(), x.stride(0) if m > 1 else 0, p.data_ptr(), s.data_ptr(),
+    _native.kernels().w4_gemm(out.data_ptr(), out.stride(0), xp, rows if m > 1 else 0, p.data_ptr(), s.data_ptr(),
                               0 if z is None else z.data_ptr(), 0 if ws is None else ws.data_ptr(), m, n, k, group, waves, rt, splits,
                               torch._C._cuda_getCurrentRawStream(dev))
     return out
