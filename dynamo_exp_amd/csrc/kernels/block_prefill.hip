@@ -3,20 +3,18 @@
 //   out[i, h] = sum_j p_j vs_j v_j,  p = softmax_j(scale ks_j (q_i . k_j)),  j <= position of i (causal) or j < ctx
 // with k_j, v_j the codes of token j and ks_j, vs_j the scales of its block.
 //
-// Bound by the matrix products of long chunks and by the cache's bytes of short ones.  A workgroup takes 32 rows a wave of one
-// key/value head, a row being one query head of one token (token-major: row = token G + head), so that chunks of few tokens fill
-// waves at any group size, and a wave's rows span few positions.  Tiles of 64 keys: their codes are asked for a tile ahead, 16
-// bytes a lane, and become fp16 in a swizzled double-buffered LDS image behind the tile's products (a workgroup widens a code once
-// for all its rows, by 0.5 or 1.25 instructions).  S^T = K Q^T and O^T = V^T P^T on 32 x 32 x 16 products: a lane's scores are one
-// row's, the softmax is lane-local but for one exchange between the halves, the weights are the second product's operand as they are, V
-// is read transposed, and the row sum is taken of the fp16 weights that the second product sees, two by an instruction.  The running maximum
-// moves when a tile's exceeds it by 2^8, and weights are held as 2^7 times themselves, 2^15 at most: fp16 rounds those over 2^-21 (of the
-// running maximum's) to 2^-11 of themselves, smaller ones to 2^-32.  Q is brought under 2 by a power of two a row (what lies 2^14 under the row's largest value loses digits).
+// Bound by the matrix products and the exponentials of long chunks and by the cache's bytes of short ones.  A workgroup takes 32 rows a
+// wave of one key/value head, a row being one query head of one token (token-major: row = token G + head), so that chunks of few tokens
+// fill waves at any group size, and a wave's rows span few positions.  Tiles of 64 keys: their codes are asked for a tile ahead, 16
+// bytes a lane, and become bf16, which holds them exactly, in swizzled LDS images (a workgroup widens a code once for all its rows).
+// S^T = K Q^T and O^T = V^T P^T on 32 x 32 x 16 products: a lane's scores are one row's, the softmax is lane-local but for one exchange
+// between the halves, the weights are the second product's operand as they are, V is read transposed, and the row sum is taken of the
+// bf16 weights that the second product sees (rounded to 2^-8 of themselves), two by an instruction.  The running maximum moves when a
+// tile's exceeds it by 2^8.
 //
-// Scales stay out of the products and cost no instruction a score: ks is a factor of the scores, O is held in units of a vs that the
-// tiles agree on, and what a tile's vs is of the unit (1 to 2^-8) is added to its exponents; the row sum's ones are its inverse.  The unit
-// follows the largest vs up, and down by 2^8 steps; a block whose vs is less than 2^-8 of the unit (blocks of 16 and 32 keys, next to
-// larger ones of their tile) is widened to fp16 as so much less, exact to 2^-24 of a code.
+// Scales stay out of the products and cost no instruction a score: ks is a factor of the scores; O is held in units of the largest vs
+// that the workgroup has come upon, and what a tile's vs is of the unit is added to its exponents; the row sum's ones are its inverse
+// (2^-100 at least: what lies further apart is taken for that, and weights under 2^-26 of it are lost to the row sum).
 //
 // Few rows behind many keys are split over the keys (the plan says where), each part leaves its sums in fp32, and a second kernel
 // joins them.
@@ -28,7 +26,7 @@ namespace {
 
 constexpr int D = 128, BQ = 32, BKV = 64;
 constexpr int kTileBytes = BKV * D * 2;
-constexpr float kRescale = 8.0f, kLift = 7.0f;
+constexpr float kRescale = 8.0f;
 constexpr int kItem = 6;  // seq, first row, first key, end of the keys, place of its sums (or -1), 0
 constexpr int kFewRows = 32;  // rows that block_rows_kernel takes
 constexpr int kJoin = 4;  // seq, first row, first place, places
@@ -49,10 +47,13 @@ struct PrefillArgs {
   float scale_log2e;
 };
 
-// a pair of fp16 times another, added to a sum in fp32
+// a pair of bf16 times another, added to a sum in fp32
 __device__ __forceinline__ float sum2(uint32_t a, uint32_t b, float c) {
-  return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, a), __builtin_bit_cast(f16x2, b), c, false);
+  typedef __bf16 pair __attribute__((ext_vector_type(2)));
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pair, a), __builtin_bit_cast(pair, b), c, false);
 }
+
+template <int I> using at_t = std::integral_constant<int, I>;
 
 // RW: row waves of 32 rows; KW: waves that share a tile's keys (1, or 2: 32 each); ONE: a tile's keys lie in one block
 template <int CODE, int RW, int KW, bool ONE>
@@ -60,7 +61,7 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
   constexpr int NW = RW * KW, PIECES = 8 / NW;  // pieces of 8 rows of a tile that a wave brings
   constexpr int SUBS = 2 / KW;                  // 32-key pieces of a tile that a wave multiplies
   constexpr int NG = ONE ? 1 : 4;               // scales of a tile
-  constexpr bool kRaised = NW == 8;
+  constexpr bool kPhases = NW == 8 && ONE;      // two halves of the waves, in turn with products and with the softmax
   __shared__ __attribute__((aligned(16))) char smem[2 * 2 * kTileBytes];
   const int* item = a.work + (int64_t)blockIdx.y * kItem;
   const int kvh = blockIdx.x, G = a.G;
@@ -70,15 +71,24 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
   const int rw = wid % RW, kw = wid / RW;
   const int r = lane & 31, h = lane >> 5;
   const int* bt = a.block_tables + (int64_t)seq * a.bt_stride;
-  // the blocks of the tiles and their scales, 64 at a time, a lane each (a table's columns are all that may be read of it)
+  // the blocks of the tiles, 64 at a time, a lane each (a table's columns are all that may be read of it)
   int first = key0 >> a.bs_shift, ids = bt[min(first + lane, a.bt_cols - 1)];
   const int q_start = __builtin_amdgcn_readfirstlane(a.cu[seq]), qlen = __builtin_amdgcn_readfirstlane(a.cu[seq + 1]) - q_start;
   const int ctx = __builtin_amdgcn_readfirstlane((int)min((int64_t)a.ctx_lens[seq], (int64_t)a.bt_cols << a.bs_shift));
   const int last = max(ctx - 1, 0) >> a.bs_shift;
-  float ks_l, vs_l;
+  // ... and what becomes of their scales: a score's factor (never 0: a masked score is -infinity times it), the logarithm of vs in
+  // units of the largest so far, and its inverse as a pair of bf16
+  float sc_l, lg_l, unit = 0x1p-126f;
+  uint32_t ones_l;
   auto scales = [&]() __attribute__((always_inline)) {
     ids = (unsigned)ids < (unsigned)a.num_blocks ? ids : 0;
-    ks_l = a.ks[(int64_t)ids * a.n_kv + kvh], vs_l = a.vs[(int64_t)ids * a.n_kv + kvh];
+    const float ks = a.ks[(int64_t)ids * a.n_kv + kvh], vs = a.vs[(int64_t)ids * a.n_kv + kvh];
+    sc_l = fmaxf(ks * a.scale_log2e, 0x1p-126f);
+    const float top = wave_reduce_max(first + lane <= last ? vs : 0.f);  // (a scale behind the context may be anything)
+    unit = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(fmaxf(unit, top))));
+    const float part = fmaxf(vs * __builtin_amdgcn_rcpf(unit), 0x1p-100f), inv = __builtin_amdgcn_rcpf(part);  // (of powers of two: exact)
+    lg_l = __builtin_amdgcn_logf(part);
+    ones_l = pack_bf16x2(inv, inv);
   };
   scales();
   const int pos0 = ctx - qlen, rows = qlen * G;
@@ -92,145 +102,86 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
   const int kv_end = min(min(key1, ctx), wg_max + 1);
   const int n_tiles = max(kv_end - key0 + BKV - 1, 0) / BKV;
 
-  int koff[8], voff[4][2];
-#pragma unroll
-  for (int s = 0; s < 8; ++s) koff[s] = tile_off(r, 2 * s + h);
-  {
-    const int g16 = (lane >> 4) & 1, qq = (lane & 15) >> 2, pp = lane & 3;
-#pragma unroll
-    for (int dt = 0; dt < 4; ++dt) {
-      const int ch = dt * 4 + 2 * g16 + (pp >> 1);
-      voff[dt][0] = tile_off(4 * h + qq, ch) + 8 * (pp & 1);
-      voff[dt][1] = tile_off(4 * h + qq + 8, ch) + 8 * (pp & 1);
-    }
-  }
   // ---- a tile's codes: piece p of this wave is rows 8 (PIECES wid + p) .. + 7, a lane 16 columns of one of them
   raw4 kr[PIECES], vr[PIECES];
-  float ks_next[NG], vs_next[NG];  // the scales of the tile on its way
-  float unit = 0x1p-126f, most = 0.f;  // what O is in, from that tile on; the largest vs so far
-  float vs_part[NG];                   // its values' scales in units of that
-  auto load = [&](int t) __attribute__((always_inline)) {
-    const int j0 = key0 + t * BKV;
-    if (min((j0 + BKV - 1) >> a.bs_shift, last) - first >= 64) {
-      first = j0 >> a.bs_shift;
+  float sc_next[NG], lg_next[NG], sc_now[NG], lg_now[NG];  // of the tile on its way, and of the one in use
+  uint32_t ones_next[NG], ones_now[NG];
+  float unit_next = unit, unit_now = unit, unit_o = unit;  // what its exponents are short of; what this wave's O is in
+  auto at_block = [&](int j) __attribute__((always_inline)) { return min(j >> a.bs_shift, last) - first; };
+  auto window = [&](int t0, int t1) __attribute__((always_inline)) {  // the blocks of tiles t0 to t1 are among the 64 here
+    if (min((key0 + (t1 + 1) * BKV - 1) >> a.bs_shift, last) - first >= 64) {
+      first = (key0 + t0 * BKV) >> a.bs_shift;
       ids = bt[min(first + lane, a.bt_cols - 1)];
       scales();
     }
-    auto at_block = [&](int j) { return min(j >> a.bs_shift, last) - first; };
+  };
+  auto load = [&](const uint8_t* from, int t, raw4(&to)[PIECES]) __attribute__((always_inline)) {
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
-      const int j = j0 + 8 * (PIECES * wid + p);
+      const int j = key0 + t * BKV + 8 * (PIECES * wid + p);
       const int64_t block = (int64_t)__builtin_amdgcn_readlane(ids, at_block(j)) * a.n_kv + kvh;
-      const int64_t base = ((block << a.bs_shift) + (j & ((1 << a.bs_shift) - 1)) + (lane >> 3)) * D + 16 * (lane & 7);
-      kr[p] = *reinterpret_cast<const raw4*>(a.k + base);
-      vr[p] = *reinterpret_cast<const raw4*>(a.v + base);
+      const uint8_t* at = from + ((block << a.bs_shift) + (j & ((1 << a.bs_shift) - 1))) * D;  // (the same in all lanes)
+      to[p] = *reinterpret_cast<const raw4*>(at + (uint32_t)(lane >> 3) * D + 16 * (lane & 7));
     }
+  };
+  auto load_scales = [&](int t) __attribute__((always_inline)) {
+    unit_next = unit;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      const int i = at_block(j0 + 16 * g);
-      ks_next[g] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(ks_l), i));
-      vs_next[g] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(vs_l), i));
+      const int i = at_block(key0 + t * BKV + 16 * g);
+      sc_next[g] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc_l), i));
+      lg_next[g] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lg_l), i));
+      ones_next[g] = __builtin_amdgcn_readlane(ones_l, i);
     }
   };
-  // (what is the same in all lanes, in scalar registers)
-  auto uni = [](float x) __attribute__((always_inline)) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(x))); };
-  auto agree = [&]() __attribute__((always_inline)) {
-    float top = vs_next[0];
+  auto turn_over = [&]() __attribute__((always_inline)) {  // the tile that was on its way is the tile in use
+    unit_now = unit_next;
 #pragma unroll
-    for (int g = 1; g < NG; ++g) top = fmaxf(top, vs_next[g]);
-    // (never 2^60 under the largest: O stays a number, and what is less would hardly be seen beside it; a block of zeros may have scale 0)
-    most = uni(fmaxf(most, top));
-    if (top > unit || (top < unit * 0x1p-8f && top > most * 0x1p-60f)) unit = uni(top);
-#pragma unroll
-    for (int g = 0; g < NG; ++g) vs_part[g] = uni(vs_next[g] * __builtin_amdgcn_rcpf(unit));  // (of a power of two: exact)
+    for (int g = 0; g < NG; ++g) sc_now[g] = sc_next[g], lg_now[g] = lg_next[g], ones_now[g] = ones_next[g];
   };
-  auto store = [&](char* kb, int t) __attribute__((always_inline)) {
-    const int j0 = key0 + t * BKV;
-    if (j0 + BKV > ctx) {  // (whatever lies behind the context may be a NaN)
-#pragma unroll
-      for (int p = 0; p < PIECES; ++p)
-        if (j0 + 8 * (PIECES * wid + p) + (lane >> 3) >= ctx) kr[p] = vr[p] = raw4{0u, 0u, 0u, 0u};
-    }
+  // (whatever lies behind the context may be a NaN)
+  auto behind = [&](int t, raw4(&x)[PIECES]) __attribute__((always_inline)) {
 #pragma unroll
     for (int p = 0; p < PIECES; ++p) {
-      const int row = 8 * (PIECES * wid + p) + (lane >> 3), to = tile_off(row, 2 * (lane & 7)), to1 = tile_off(row, 2 * (lane & 7) + 1);
-      raw4 o[2];
-      widen16_f16<CODE, false>(kr[p], 1.f, o);
-      *reinterpret_cast<raw4*>(kb + to) = o[0];
-      *reinterpret_cast<raw4*>(kb + to1) = o[1];
-      const int g = ONE ? 0 : (PIECES * wid + p) >> 1;
-      const float part = g == 0 ? vs_part[0] : g == 1 ? vs_part[NG > 1 ? 1 : 0] : g == 2 ? vs_part[NG > 2 ? 2 : 0] : vs_part[NG > 3 ? 3 : 0];
-      if (part < 0x1p-8f) widen16_f16<CODE, true>(vr[p], part * 0x1p8f, o);
-      else widen16_f16<CODE, false>(vr[p], 1.f, o);
-      *reinterpret_cast<raw4*>(kb + kTileBytes + to) = o[0];
-      *reinterpret_cast<raw4*>(kb + kTileBytes + to1) = o[1];
+      const bool none = key0 + t * BKV + 8 * (PIECES * wid + p) + (lane >> 3) >= ctx;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[p][i] = none ? 0u : x[p][i];
     }
   };
-  if (n_tiles > 0) load(0);
+  int to_off[PIECES][2];
+#pragma unroll
+  for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) to_off[p][i] = tile_off(8 * (PIECES * wid + p) + (lane >> 3), 2 * (lane & 7) + i);
+  auto store = [&](int image, const raw4(&x)[PIECES]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int p = 0; p < PIECES; ++p)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const raw2 lo = widen4_bf16<CODE, false>(x[p][2 * i], 1.f), hi = widen4_bf16<CODE, false>(x[p][2 * i + 1], 1.f);
+        *reinterpret_cast<raw4*>(smem + image + to_off[p][i]) = raw4{lo[0], lo[1], hi[0], hi[1]};
+      }
+  };
+  if (n_tiles > 0) {
+    load(a.k, 0, kr);
+    if constexpr (!kPhases) load(a.v, 0, vr);
+    load_scales(0);
+    turn_over();
+  }
 
-  // ---- Q in fp16, under 2; what a score is worth then
   u16x8 qf[8];
-  float q_unit;
   {
     const bf16_t* qp = a.q + (int64_t)(q_start + tok) * a.q_stride + (int64_t)(kvh * G + hq) * D + 8 * h;
-    float amax = 0.f;
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      qf[s] = valid ? *reinterpret_cast<const u16x8*>(qp + 16 * s) : u16x8{{0, 0, 0, 0}};
-#pragma unroll
-      for (int w = 0; w < 4; ++w) amax = fmaxf(fmaxf(amax, fabsf(bf16lo(qf[s].w[w]))), fabsf(bf16hi(qf[s].w[w])));
-    }
-    const float unit = unit_factor(halves_max(amax));
-#pragma unroll
-    for (int s = 0; s < 8; ++s)
-#pragma unroll
-      for (int w = 0; w < 4; ++w) qf[s].w[w] = pack_f16x2(bf16lo(qf[s].w[w]) * unit, bf16hi(qf[s].w[w]) * unit);
-    q_unit = a.scale_log2e / unit;
+    for (int s = 0; s < 8; ++s) qf[s] = valid ? *reinterpret_cast<const u16x8*>(qp + 16 * s) : u16x8{{0, 0, 0, 0}};
   }
   f32x16 o_acc[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) o_acc[i] = f32x16{};
   float m_i = -1e30f, l_i = 0.f;  // (l: of this lane's keys)
-  float ks_now[NG], part_log[NG], unit_now = 1.f, unit_o = 0.f;  // of the tile in use; what this wave's O is in
-  uint32_t ones[NG];                                             // fp16 pairs
-  auto vread = [&](const char* vb, int i) __attribute__((always_inline)) {  // columns 32 (i % 4) .. + 31 of keys 16 (i / 4) .. + 15
-    const i16x4 lo = read_tr16((const lds_i16x4*)(vb + i / 4 * 4096 + voff[i % 4][0]));
-    const i16x4 hi = read_tr16((const lds_i16x4*)(vb + i / 4 * 4096 + voff[i % 4][1]));
-    return __builtin_bit_cast(f16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-  };
-  constexpr int kAhead = 4;  // fragments asked for ahead of their products
-  auto compute = [&](const char* tile, int t) __attribute__((always_inline)) {
-    const int j0 = key0 + t * BKV + 32 * SUBS * kw;  // this wave's first key
-    if (j0 > wave_max) return;
-    const char* kb = tile + 8192 * SUBS * kw;
-    const bool live1 = SUBS == 2 && j0 + 32 <= wave_max;
-    f32x16 s0 = f32x16{}, s1 = f32x16{};
-    f16x8 kf[kAhead], vf[kAhead];
-    auto kread = [&](int i) __attribute__((always_inline)) { return __builtin_bit_cast(f16x8, *reinterpret_cast<const raw4*>(kb + 8192 * (i >> 3) + koff[i & 7])); };
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) kf[i] = kread(i);
-    __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
-#pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      const f16x8 x = kf[s % kAhead];
-      if (SUBS == 2 || s + kAhead < 8) kf[s % kAhead] = kread(s + kAhead);
-      s0 = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, __builtin_bit_cast(f16x8, qf[s]), s0, 0, 0, 0);
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      if (SUBS == 2 || s + kAhead < 8) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-    }
-    if (live1) {
-#pragma unroll
-      for (int s = 0; s < 8; ++s) {
-        const f16x8 x = kf[s % kAhead];
-        if (s + kAhead < 8) kf[s % kAhead] = kread(8 + s + kAhead);
-        s1 = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, __builtin_bit_cast(f16x8, qf[s]), s1, 0, 0, 0);
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        if (s + kAhead < 8) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      }
-    }
-    const char* vb = tile + kTileBytes + 8192 * SUBS * kw;
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) vf[i] = vread(vb, i);
+  f32x16 s0, s1;                  // a tile's scores
+  u16x8 pf[2][2];                 // its weights
+  auto weights = [&](int j0) __attribute__((always_inline)) {
     if (j0 + 32 * SUBS - 1 > wave_min || j0 + 32 * SUBS > ctx) {  // the diagonal, or the context's end
       const int lim = min(my_pos, ctx - 1) - j0 - 4 * h;
 #pragma unroll
@@ -241,24 +192,14 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
       }
     }
     // a score's factor, and what its exponent is short of: one of a tile, or one each 16 keys (group 2 sub + s2 of this wave's)
-    // (a factor is never 0: a masked score is -infinity times it)
     float sc[2][2], lg[2][2];
-    uint32_t one[2][2];
-    auto factor = [&](float ks) __attribute__((always_inline)) { return fmaxf(q_unit * ks, 0x1p-126f); };
 #pragma unroll
     for (int sub = 0; sub < SUBS; ++sub)
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
-        if constexpr (ONE) {
-          sc[sub][s2] = factor(ks_now[0]), lg[sub][s2] = part_log[0], one[sub][s2] = ones[0];
-        } else if constexpr (KW == 1) {
-          sc[sub][s2] = factor(ks_now[NG > 1 ? 2 * sub + s2 : 0]), lg[sub][s2] = part_log[NG > 1 ? 2 * sub + s2 : 0], one[sub][s2] = ones[NG > 1 ? 2 * sub + s2 : 0];
-        } else {
-          constexpr int kHi = NG > 2 ? 2 : 0;
-          sc[sub][s2] = factor(kw ? ks_now[kHi + (NG > 1 ? s2 : 0)] : ks_now[NG > 1 ? s2 : 0]);
-          lg[sub][s2] = kw ? part_log[kHi + (NG > 1 ? s2 : 0)] : part_log[NG > 1 ? s2 : 0];
-          one[sub][s2] = kw ? ones[kHi + (NG > 1 ? s2 : 0)] : ones[NG > 1 ? s2 : 0];
-        }
+        const int g = NG == 1 ? 0 : 2 * sub + s2, g1 = NG == 1 ? 0 : 2 + s2;  // (g1: of the second wave of two that share a tile)
+        sc[sub][s2] = KW == 2 && kw ? sc_now[g1] : sc_now[g];
+        lg[sub][s2] = KW == 2 && kw ? lg_now[g1] : lg_now[g];
       }
     float t_s;
     if constexpr (ONE) {
@@ -288,74 +229,161 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
     const float m_new = t_s > m_i + kRescale ? t_s : m_i;
     const float alpha = fast_exp2(m_i - m_new);
     m_i = m_new;
-    u16x8 pf[2][2];
 #pragma unroll
     for (int s2 = 0; s2 < 2; ++s2) {
-      const float b0 = m_new - (kLift + lg[0][s2]), b1 = SUBS == 2 ? m_new - (kLift + lg[SUBS - 1][s2]) : 0.f;
+      const float b0 = m_new - lg[0][s2], b1 = SUBS == 2 ? m_new - lg[SUBS - 1][s2] : 0.f;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const int i = 8 * s2 + 2 * w;
-        pf[0][s2].w[w] = pack_f16x2(fast_exp2(s0[i] * sc[0][s2] - b0), fast_exp2(s0[i + 1] * sc[0][s2] - b0));
-        if constexpr (SUBS == 2) pf[1][s2].w[w] = pack_f16x2(fast_exp2(s1[i] * sc[1][s2] - b1), fast_exp2(s1[i + 1] * sc[1][s2] - b1));
+        pf[0][s2].w[w] = pack_bf16x2(fast_exp2(s0[i] * sc[0][s2] - b0), fast_exp2(s0[i + 1] * sc[0][s2] - b0));
+        if constexpr (SUBS == 2) pf[1][s2].w[w] = pack_bf16x2(fast_exp2(s1[i] * sc[1][s2] - b1), fast_exp2(s1[i + 1] * sc[1][s2] - b1));
       }
     }
     l_i *= alpha;
-#pragma unroll
-    for (int sub = 0; sub < SUBS; ++sub)
-#pragma unroll
-      for (int s2 = 0; s2 < 2; ++s2)
-#pragma unroll
-        for (int w = 0; w < 4; ++w) l_i = sum2(pf[sub][s2].w[w], one[sub][s2], l_i);
-    const bool other = unit_o != unit_now;
-    if (other || __builtin_amdgcn_ballot_w64(alpha != 1.f)) {
+    if (unit_o != unit_now || __builtin_amdgcn_ballot_w64(alpha != 1.f)) {
       const float both = alpha * (unit_o * __builtin_amdgcn_rcpf(unit_now));
       unit_o = unit_now;
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt) o_acc[dt] *= both;
     }
-    if constexpr (kRaised) __builtin_amdgcn_s_setprio(0);
-#pragma unroll
-    for (int sub = 0; sub < SUBS; ++sub)
-      if (sub == 0 || live1) {
-#pragma unroll
-        for (int i = 8 * sub; i < 8 * sub + 8; ++i) {
-          const int s2 = (i >> 2) & 1;
-          const f16x8 p = __builtin_bit_cast(f16x8, pf[sub][s2]), x = vf[i % kAhead];
-          if (i + kAhead < 8 * SUBS) vf[i % kAhead] = vread(vb, i + kAhead);
-          o_acc[i & 3] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, p, o_acc[i & 3], 0, 0, 0);
-          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-          if (i + kAhead < 8 * SUBS) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-        }
-      }
-    if constexpr (kRaised) __builtin_amdgcn_s_setprio(1);
   };
-  auto turn_over = [&]() __attribute__((always_inline)) {  // the tile that was on its way is the tile in use
-    unit_now = unit;
+  // pair i of a wave's 8 SUBS pairs of weights, added to the row sum
+  auto add_pair = [&](int i) __attribute__((always_inline)) {
+    const int sub = i >> 3, s2 = (i >> 2) & 1, g = NG == 1 ? 0 : 2 * sub + s2, g1 = NG == 1 ? 0 : 2 + s2;
+    l_i = sum2(pf[sub][s2].w[i & 3], KW == 2 && kw ? ones_now[g1] : ones_now[g], l_i);
+  };
+  auto mfma = [](const u16x8& x, const u16x8& y, const f32x16& c) __attribute__((always_inline)) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, x), __builtin_bit_cast(bf16x8_t, y), c, 0, 0, 0);
+  };
+  // ---- fragments, by one address each of K and V: what a fragment's place differs by is an exclusive or, or a constant.  (The addresses
+  // are taken anew in each tile: there are not registers for a place each.)
+  int kbase = tile_off(r, h), vbase = tile_off(4 * h + ((lane & 15) >> 2), 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + 8 * (lane & 1);
+  auto again = [&]() __attribute__((always_inline)) { asm volatile("" : "+v"(kbase), "+v"(vbase)); };
+  auto kfrag = [&](int image, int i) __attribute__((always_inline)) {  // columns 16 (i % 8) .. + 15 of keys 32 (i / 8) .. + 31
+    return __builtin_bit_cast(u16x8, *reinterpret_cast<const raw4*>(smem + (kbase ^ (32 * (i & 7))) + image + 8192 * (i >> 3)));
+  };
+  auto vfrag = [&](int image, int i) __attribute__((always_inline)) {  // columns 32 (i % 4) .. + 31 of keys 16 (i / 4) .. + 15
+    const char* at = smem + image + 4096 * (i >> 2);
+    const i16x4 lo = read_tr16((const lds_i16x4*)(at + (vbase ^ (64 * (i & 3)))));
+    const i16x4 hi = read_tr16((const lds_i16x4*)(at + (vbase ^ (64 * (i & 3) + 32)) + 2048));
+    return __builtin_bit_cast(u16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
+  // Products FROM .. TO of the scores' (0 .. 15) and values' (16 .. 31), in one line with their fragments kAhead ahead; between(i) comes
+  // behind product i.
+  constexpr int kAhead = 6;
+  auto line = [&](auto from_, auto to_, int k_image, int v_image, auto between) __attribute__((always_inline)) {
+    constexpr int FROM = decltype(from_)::value, TO = decltype(to_)::value;
+    u16x8 x[kAhead];
+    auto read = [&](int i) __attribute__((always_inline)) { return i < 16 ? kfrag(k_image, i) : vfrag(v_image, i - 16); };
+    if constexpr (FROM == 0) s0 = s1 = f32x16{};
 #pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const float part = fmaxf(vs_part[g], 0x1p-8f);
-      ks_now[g] = ks_next[g];
-      part_log[g] = uni(__builtin_amdgcn_logf(part));
-      ones[g] = __builtin_amdgcn_readfirstlane(pack_f16x2(__builtin_amdgcn_rcpf(part), __builtin_amdgcn_rcpf(part)));
+    for (int i = 0; i < kAhead; ++i) x[i] = read(FROM + i);
+    __builtin_amdgcn_sched_group_barrier(0x100, FROM < 16 ? kAhead : 2 * kAhead, 0);
+#pragma unroll
+    for (int i = FROM; i < TO; ++i) {
+      const u16x8 now = x[(i - FROM) % kAhead];
+      if (i + kAhead < TO) x[(i - FROM) % kAhead] = read(i + kAhead);
+      if (i < 8) s0 = mfma(now, qf[i & 7], s0);
+      else if (i < 16) s1 = mfma(now, qf[i & 7], s1);
+      else o_acc[i & 3] = mfma(now, pf[(i >> 3) & 1][(i >> 2) & 1], o_acc[i & 3]);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if (i + kAhead < TO && i + kAhead < 16) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      else if (i + kAhead < TO) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      between(i);
     }
   };
+  auto nothing = [](int) {};
 
-  if (n_tiles > 0) {
-    agree();
-    store(smem, 0);
-    turn_over();
-  }
-  __syncthreads();
-  for (int t = 0; t < n_tiles; ++t) {
-    char *now = smem + (t & 1) * 2 * kTileBytes, *next = smem + ((t + 1) & 1) * 2 * kTileBytes;
-    if (t + 1 < n_tiles) load(t + 1);
-    compute(now, t);
-    if (t + 1 < n_tiles) {
-      agree();
-      store(next, t + 1);
+  const int jw = key0 + 32 * SUBS * kw;  // this wave's first key of a tile
+  if constexpr (kPhases) {
+    // The products of one half of the waves run while the other half has its softmax.  With a wave's products, which leave the
+    // vector pipe seven cycles of eight, go the row sum of the tile before and this wave's part of the next codes.  K's image is a
+    // tile ahead of V's: products of t read K of t and V of t - 1, and bring V of t and K of t + 1.
+    const int late = wid / 4;  // (the waves of a SIMD are one of either half)
+    auto meet = [&]() __attribute__((always_inline)) {
+      __builtin_amdgcn_sched_barrier(0);
+      __syncthreads();
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    auto k_at = [](int t) { return (t & 1) * kTileBytes; };
+    auto v_at = [](int t) { return (2 + (t & 1)) * kTileBytes; };
+    const int end = n_tiles - 1;  // (behind the last tile that one again, read by none)
+    auto fetch = [&](int t) __attribute__((always_inline)) {  // V of t, K of the next, their scales
+      const int tv = min(t, end), tk = min(t + 1, end);
+      load(a.v, tv, vr);
+      load(a.k, tk, kr);
+      load_scales(tv);
+    };
+    auto bring = [&](int t) __attribute__((always_inline)) {
+      behind(min(t, end), vr);
+      store(v_at(t), vr);
+      behind(min(t + 1, end), kr);
+      store(k_at(t + 1), kr);
+      fetch(t + 1);
+    };
+    if (n_tiles > 0) {
+      behind(0, kr);
+      store(k_at(0), kr);
+      window(0, min(1, end));
+      fetch(0);
+      meet();
+      if (late) meet();
+      line(at_t<0>{}, at_t<16>{}, k_at(0), 0, nothing);
       turn_over();
+      window(min(1, end), min(2, end));
+      bring(0);
+      for (int t = 0; t < end; ++t) {
+        meet();
+        weights(jw + t * BKV);
+        again();
+        window(min(t + 2, end), min(t + 3, end));
+        meet();
+        line(at_t<0>{}, at_t<32>{}, k_at(t + 1), v_at(t), [&](int i) __attribute__((always_inline)) {
+          if (i >= 14 && i < 30) add_pair(i - 14);
+        });
+        turn_over();
+        bring(t + 1);
+      }
+      meet();
+      weights(jw + end * BKV);
+      again();
+      meet();
+      line(at_t<16>{}, at_t<32>{}, 0, v_at(end), [&](int i) __attribute__((always_inline)) { add_pair(i - 16); });
+      if (!late) meet();
+    }
+  } else {
+    auto image = [](int t) { return (t & 1) * 2 * kTileBytes; };
+    if (n_tiles > 0) {
+      behind(0, kr);
+      store(image(0), kr);
+      behind(0, vr);
+      store(image(0) + kTileBytes, vr);
     }
     __syncthreads();
+    for (int t = 0; t < n_tiles; ++t) {
+      if (t + 1 < n_tiles) {
+        window(t + 1, t + 1);
+        load(a.k, t + 1, kr);
+        load(a.v, t + 1, vr);
+        load_scales(t + 1);
+      }
+      const int j0 = jw + t * BKV;
+      if (j0 <= wave_max) {
+        const int kb = image(t) + 8192 * SUBS * kw, vb = kb + kTileBytes;
+        again();
+        line(at_t<0>{}, at_t<8 * SUBS>{}, kb, 0, nothing);
+        weights(j0);
+        line(at_t<16>{}, at_t<16 + 8 * SUBS>{}, 0, vb, [&](int i) __attribute__((always_inline)) { add_pair(i - 16); });
+      }
+      if (t + 1 < n_tiles) {
+        behind(t + 1, kr);
+        store(image(t + 1), kr);
+        behind(t + 1, vr);
+        store(image(t + 1) + kTileBytes, vr);
+        turn_over();
+      }
+      __syncthreads();
+    }
   }
 
   // ---- lane (r, h) holds columns 32 dt + 8 g + 4 h .. + 3 of its row
