@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
   };
   // Products FROM .. TO of the scores' (0 .. 15) and values' (16 .. 31), in one line with their fragments kAhead ahead; between(i) comes
   // behind product i.
-  constexpr int kAhead = 6;
+  constexpr int kAhead = 4;
   auto line = [&](auto from_, auto to_, int k_image, int v_image, auto between) __attribute__((always_inline)) {
     constexpr int FROM = decltype(from_)::value, TO = decltype(to_)::value;
     u16x8 x[kAhead];
@@ -296,9 +296,11 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
 
   const int jw = key0 + 32 * SUBS * kw;  // this wave's first key of a tile
   if constexpr (kPhases) {
-    // The products of one half of the waves run while the other half has its softmax.  With a wave's products, which leave the
-    // vector pipe seven cycles of eight, go the row sum of the tile before and this wave's part of the next codes.  K's image is a
-    // tile ahead of V's: products of t read K of t and V of t - 1, and bring V of t and K of t + 1.
+    // The products of one half of the waves run while the other half has its softmax: left to themselves the two waves of a SIMD, held
+    // together by the barriers, come to either at once, and wait.  Products of t read K of t and V of t - 1; the row sum of t - 1 and a
+    // wave's part of the next K go with them, its part of the next V with the softmax, so that the two take about as long.  Half h is a
+    // meeting behind half 0: it brings V a tile further.  us, 5000 + 4000 tokens of 32 / 8 heads, int8: no phases 411, with these
+    // 328; without priority for the products 344, K and V brought with the products 342, with the softmax 350.
     const int late = wid / 4;  // (the waves of a SIMD are one of either half)
     auto meet = [&]() __attribute__((always_inline)) {
       __builtin_amdgcn_sched_barrier(0);
@@ -308,44 +310,48 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
     auto k_at = [](int t) { return (t & 1) * kTileBytes; };
     auto v_at = [](int t) { return (2 + (t & 1)) * kTileBytes; };
     const int end = n_tiles - 1;  // (behind the last tile that one again, read by none)
-    auto fetch = [&](int t) __attribute__((always_inline)) {  // V of t, K of the next, their scales
-      const int tv = min(t, end), tk = min(t + 1, end);
-      load(a.v, tv, vr);
-      load(a.k, tk, kr);
-      load_scales(tv);
-    };
-    auto bring = [&](int t) __attribute__((always_inline)) {
+    auto bring_v = [&](int t) __attribute__((always_inline)) {
       behind(min(t, end), vr);
       store(v_at(t), vr);
-      behind(min(t + 1, end), kr);
-      store(k_at(t + 1), kr);
-      fetch(t + 1);
+      load(a.v, min(t + 1, end), vr);
+    };
+    auto bring_k = [&](int t) __attribute__((always_inline)) {
+      behind(min(t, end), kr);
+      store(k_at(t), kr);
+      load(a.k, min(t + 1, end), kr);
     };
     if (n_tiles > 0) {
-      behind(0, kr);
-      store(k_at(0), kr);
-      window(0, min(1, end));
-      fetch(0);
+      window(0, min(2, end));
+      bring_k(0);
+      load(a.v, 0, vr);
+      load_scales(0);
       meet();
-      if (late) meet();
+      if (late) {
+        bring_v(0);
+        meet();
+      }
       line(at_t<0>{}, at_t<16>{}, k_at(0), 0, nothing);
       turn_over();
-      window(min(1, end), min(2, end));
-      bring(0);
+      bring_k(1);
       for (int t = 0; t < end; ++t) {
         meet();
+        __builtin_amdgcn_s_setprio(0);
+        window(t + 1, min(t + 3, end));
+        load_scales(t + 1);
+        bring_v(t + late);
         weights(jw + t * BKV);
         again();
-        window(min(t + 2, end), min(t + 3, end));
         meet();
+        __builtin_amdgcn_s_setprio(1);
         line(at_t<0>{}, at_t<32>{}, k_at(t + 1), v_at(t), [&](int i) __attribute__((always_inline)) {
           if (i >= 14 && i < 30) add_pair(i - 14);
         });
         turn_over();
-        bring(t + 1);
+        bring_k(t + 2);
       }
       meet();
       weights(jw + end * BKV);
+      bring_v(end + late);
       again();
       meet();
       line(at_t<16>{}, at_t<32>{}, 0, v_at(end), [&](int i) __attribute__((always_inline)) { add_pair(i - 16); });
