@@ -653,56 +653,69 @@ __global__ void __launch_bounds__(256, 2) block_rows_kernel(const PrefillArgs a)
   }
 }
 
-// One row a workgroup: its parts' sums under a common maximum, over their common sum.  Eight groups of 32 lanes x 4 columns take every
-// eighth part, two of them on their way at once.
+// A row's parts' sums under a common maximum, over their common sum: by 32 lanes x 4 columns where parts are few, eight rows a
+// workgroup, by all eight groups of 32 lanes where they are many, each taking every eighth part, two of them on their way at once.
+template <int GROUPS>
 __global__ void __launch_bounds__(256) block_prefill_join_kernel(bf16_t* __restrict__ out, const float* __restrict__ ws_o, const float* __restrict__ ws_ml,
                                                                  const int* __restrict__ joins, const int* __restrict__ cu, int n_kv, int G, int tile) {
   __shared__ __attribute__((aligned(16))) f32x4 other[8][D / 4];
   __shared__ float dens[8];
-  const int lane = threadIdx.x & 63, grp = threadIdx.x >> 5, col = threadIdx.x & 31, in = blockIdx.x, kvh = blockIdx.y;
+  const int grp = threadIdx.x >> 5, col = threadIdx.x & 31, in = blockIdx.x * (8 / GROUPS) + grp / GROUPS, kvh = blockIdx.y;
   const int* item = joins + (int64_t)blockIdx.z * kJoin;
   const int seq = item[0], f = item[1] + in, place = item[2], n = item[3];
   const int q_start = cu[seq], rows = (cu[seq + 1] - q_start) * G;
-  if (f >= rows) return;
+  if (in >= tile || f >= rows) return;  // (of one row: all of the workgroup)
   const int64_t step = (int64_t)n_kv * tile, row = ((int64_t)place * n_kv + kvh) * tile + in;
   float M = -1e30f;
-  for (int p = lane; p < n; p += 64) M = fmaxf(M, ws_ml[(row + p * step) * 2]);
+  for (int p = col; p < n; p += 32) M = fmaxf(M, ws_ml[(row + p * step) * 2]);
+#pragma unroll
+  for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor(M, d, 64));
   float den = 0.f;
   f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-  M = wave_reduce_max(M);
-  for (int p = grp; p < n; p += 16) {
-    const int p2 = min(p + 8, n - 1);
+  for (int p = grp % GROUPS; p < n; p += 2 * GROUPS) {
+    const int p2 = min(p + GROUPS, n - 1);
     const f32x2 ml = *reinterpret_cast<const f32x2*>(ws_ml + (row + p * step) * 2), ml2 = *reinterpret_cast<const f32x2*>(ws_ml + (row + p2 * step) * 2);
     const f32x4 x = *reinterpret_cast<const f32x4*>(ws_o + (row + p * step) * D + 4 * col), x2 = *reinterpret_cast<const f32x4*>(ws_o + (row + p2 * step) * D + 4 * col);
-    const float w = fast_exp2(ml.x - M), w2 = p + 8 < n ? fast_exp2(ml2.x - M) : 0.f;
+    const float w = fast_exp2(ml.x - M), w2 = p + GROUPS < n ? fast_exp2(ml2.x - M) : 0.f;
     den += w * ml.y + w2 * ml2.y;
     sum += w * x + w2 * x2;
   }
-  other[grp][col] = sum;
-  if (col == 0) dens[grp] = den;
-  __syncthreads();
-  if (grp) return;
+  if constexpr (GROUPS > 1) {
+    other[grp][col] = sum;
+    if (col == 0) dens[grp] = den;
+    __syncthreads();
+    if (grp) return;
 #pragma unroll
-  for (int k = 1; k < 8; ++k) sum += other[k][col], den += dens[k];
+    for (int k = 1; k < 8; ++k) sum += other[k][col], den += dens[k];
+  }
   const float inv = den != 0.f ? 1.f / den : 0.f;
   const int tok = f / G, hq = f - tok * G;
   *reinterpret_cast<uint2*>(out + ((int64_t)(q_start + tok) * n_kv * G + kvh * G + hq) * D + 4 * col) =
       uint2{pack_bf16x2(sum[0] * inv, sum[1] * inv), pack_bf16x2(sum[2] * inv, sum[3] * inv)};
 }
 
+// rows: those of the longest joined item; parts: of the most cut one
+void join_parts(const PrefillArgs& a, const int* joins, int n_joins, int rows, int parts, int tile, hipStream_t stream) {
+  if (!n_joins) return;
+  if (parts <= 4)
+    block_prefill_join_kernel<1><<<dim3((rows + 7) / 8, a.n_kv, n_joins), 256, 0, stream>>>(a.out, a.ws_o, a.ws_ml, joins, a.cu, a.n_kv, a.G, tile);
+  else
+    block_prefill_join_kernel<8><<<dim3(rows, a.n_kv, n_joins), 256, 0, stream>>>(a.out, a.ws_o, a.ws_ml, joins, a.cu, a.n_kv, a.G, tile);
+}
+
 }  // namespace
 
 // q [T, Hq, 128] rows q_stride apart (16-byte aligned); out [T, Hq, 128]; work [n_work + n_few][6] (tiles, then sequences of few rows),
 // joins [n_joins + n_few_joins][4] and the places of their sums (ws_o [places, Hkv, tile, 128], ws_ml [..., 2] fp32; few: [places, Hkv,
-// 32, ...]) as the plan says; tile: rows of a work item (64, 128, 256); few_groups: 16s of rows (1, 2).  code: 0 int8, 1 e4m3fn.
+// 32, ...]) as the plan says; join_rows, most_parts: rows and parts that a joined item has at most; tile: rows of a work item (64, 128, 256); few_groups: 16s of rows (1, 2).  code: 0 int8, 1 e4m3fn.
 extern "C" int dx_block_prefill(void* out, float* ws_o, float* ws_ml, float* few_o, float* few_ml, const void* q, int64_t q_stride, const void* k,
                                 const void* v, const float* ks, const float* vs, const int* block_tables, int bt_stride, int bt_cols, const int* cu,
-                                const int* ctx_lens, const int* work, int n_work, int n_few, const int* joins, int n_joins, int n_few_joins, int tile,
-                                int few_groups, int n_q, int n_kv, int head_dim, int block_size, int num_blocks, float scale, int causal, int code,
+                                const int* ctx_lens, const int* work, int n_work, int n_few, const int* joins, int n_joins, int n_few_joins, int join_rows,
+                                int few_join_rows, int most_parts, int few_most_parts, int tile, int few_groups, int n_q, int n_kv, int head_dim, int block_size, int num_blocks, float scale, int causal, int code,
                                 hipStream_t stream) {
   if (head_dim != D || block_size < 16 || (block_size & (block_size - 1)) || n_kv < 1 || n_kv > 65535 || n_q % n_kv || q_stride % 8 || bt_cols < 1 ||
       (tile != 64 && tile != 128 && tile != 256) || (few_groups != 1 && few_groups != 2) || n_work > 65535 || n_few > 65535 || n_joins > 65535 ||
-      n_few_joins > 65535)
+      n_few_joins > 65535 || (n_joins && (join_rows < 1 || join_rows > tile)) || (n_few_joins && (few_join_rows < 1 || few_join_rows > kFewRows)))
     return -1;
   PrefillArgs a{};
   a.out = (bf16_t*)out, a.ws_o = ws_o, a.ws_ml = ws_ml, a.q = (const bf16_t*)q;
@@ -729,7 +742,7 @@ extern "C" int dx_block_prefill(void* out, float* ws_o, float* ws_ml, float* few
     else DX_BP(kInt8);
 #undef DX_BP
 #undef DX_BPT
-    if (n_joins) block_prefill_join_kernel<<<dim3(tile, n_kv, n_joins), 256, 0, stream>>>(a.out, ws_o, ws_ml, joins, cu, n_kv, a.G, tile);
+    join_parts(a, joins, n_joins, join_rows, most_parts, tile, stream);
   }
   if (n_few) {
     a.work = work + kItem * n_work, a.ws_o = few_o, a.ws_ml = few_ml;
@@ -742,9 +755,7 @@ extern "C" int dx_block_prefill(void* out, float* ws_o, float* ws_ml, float* few
     if (code == kE4m3) DX_BR(kE4m3);
     else DX_BR(kInt8);
 #undef DX_BR
-    if (n_few_joins)
-      block_prefill_join_kernel<<<dim3(16 * few_groups, n_kv, n_few_joins), 256, 0, stream>>>(a.out, few_o, few_ml, joins + kJoin * n_joins, cu, n_kv, a.G,
-                                                                                              kFewRows);
+    join_parts(a, joins + kJoin * n_joins, n_few_joins, few_join_rows, few_most_parts, kFewRows, stream);
   }
   return (int)hipGetLastError();
 }

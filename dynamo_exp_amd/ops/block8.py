@@ -276,6 +276,10 @@ class PrefillPlan(NamedTuple):
     n_few_joins: int
     places: int  # tiles of sums in the workspace
     few_places: int
+    join_rows: int  # rows and parts that a joined item has at most
+    few_join_rows: int
+    parts: int
+    few_parts: int
     tile: int  # rows of a work item
     few_groups: int  # 16s of rows that the sequences of few rows have at most
     rows: int
@@ -285,7 +289,10 @@ class PrefillPlan(NamedTuple):
     causal: bool
 
 
-PREFILL_WGS, SPLIT_WGS, PREFILL_TILES = 512, 256, 4
+# Key tiles of 64 a CU from which 256-row workgroups, one a CU, are worth it, workgroups that leave no CU idle, key tiles of a part.  us with 128
+# and 256 rows, 32 / 8 heads: 300 tokens behind 3700 (9.7 tiles a CU) 60, 66; six chunks of 1000 tokens' contexts (14) 42, 41; 2000 (16) 61.0,
+# 57.8; 3000 (35) 91, 87; 4000 (63) 156, 130; 200 behind 19800 (39) 148, 102; 500 (1) 22.5, 24.5; six of 700 behind 200 (18, 2.06 turns) 60, 64.
+WIDE_TILES, SPLIT_WGS, PREFILL_TILES = 12, 256, 4
 FEW_ROWS, FEW_WGS, FEW_KEYS = 32, 256, 256
 
 
@@ -300,12 +307,25 @@ def prefill_plan(q_lens: list[int], ctx_lens: list[int], n_q: int, n_kv: int, de
     g = n_q // n_kv
     few = [s for s, ql in enumerate(q_lens) if 0 < ql * g <= FEW_ROWS]
     many = [s for s, ql in enumerate(q_lens) if ql * g > FEW_ROWS]
-    count = lambda tile: n_kv * sum(-(-q_lens[s] * g // tile) for s in many)  # noqa: E731
-    tile = 256 if count(256) >= PREFILL_WGS else 128 if any(q_lens[s] * g > 64 for s in many) else 64
 
-    def cut(items, unit, per):
+    def tiles(tile):
+        """[key tiles, sequence, first row] of row tiles."""
+        items = []
+        for s in many:
+            ql, cl = q_lens[s], ctx_lens[s]
+            for r0 in range(0, ql * g, tile):
+                seen = cl - ql + (min(r0 + tile, ql * g) - 1) // g + 1 if causal else cl
+                items.append((-(-seen // 64), s, r0))
+        return items
+
+    tile, items = 256, tiles(256)
+    if sum(i[0] for i in items) * n_kv < WIDE_TILES * CUS:
+        tile = 128 if any(q_lens[s] * g > 64 for s in many) else 64
+        items = tiles(tile)
+
+    def cut(items, unit, per, most):
         """items (units of keys, sequence, first row) -> work and joins: those of over 1.5 `per` units in parts of about `per`."""
-        work, joins, places = [], [], 0
+        work, joins, places, rows, cuts = [], [], 0, 0, 0
         for n, s, r0 in items:
             parts = -(-n // per) if 2 * n > 3 * per else 1
             each = -(-n // parts)
@@ -314,6 +334,7 @@ def prefill_plan(q_lens: list[int], ctx_lens: list[int], n_q: int, n_kv: int, de
                 work.append((n, [s, r0, 0, unit * n, -1, 0]))
                 continue
             joins += [s, r0, places, parts]
+            rows, cuts = max(rows, min(most, q_lens[s] * g - r0)), max(cuts, parts)
             for p in range(parts):
                 end = min((p + 1) * each, n)
                 work.append((end - p * each, [s, r0, unit * p * each, unit * end, places + p, 0]))
@@ -321,23 +342,17 @@ def prefill_plan(q_lens: list[int], ctx_lens: list[int], n_q: int, n_kv: int, de
         if len(work) > 65535:
             raise ValueError(f"prefill_plan: {len(work)} work items, at most 65535")
         work.sort(key=lambda w: -w[0])
-        return [x for _, w in work for x in w], joins, places
+        return [x for _, w in work for x in w], joins, places, rows, cuts
 
-    items = []  # key tiles, sequence, first row
-    for s in many:
-        ql, cl = q_lens[s], ctx_lens[s]
-        for r0 in range(0, ql * g, tile):
-            seen = cl - ql + (min(r0 + tile, ql * g) - 1) // g + 1 if causal else cl
-            items.append((-(-seen // 64), s, r0))
     total = sum(i[0] for i in items)
-    work, joins, places = cut(items, 64, max(PREFILL_TILES, -(-total * n_kv // SPLIT_WGS)) if len(items) * n_kv < SPLIT_WGS else 1 << 30)
+    work, joins, places, rows, parts = cut(items, 64, max(PREFILL_TILES, -(-total * n_kv // SPLIT_WGS)) if len(items) * n_kv < SPLIT_WGS else 1 << 30, tile)
     items = [(-(-ctx_lens[s] // 128), s, 0) for s in few]
     total = sum(i[0] for i in items)
-    few_work, few_joins, few_places = cut(items, 128, max(FEW_KEYS // 128, -(-total * n_kv // FEW_WGS)))
+    few_work, few_joins, few_places, few_rows, few_parts = cut(items, 128, max(FEW_KEYS // 128, -(-total * n_kv // FEW_WGS)), FEW_ROWS)
     flat = work + few_work + joins + few_joins
     most = max([q_lens[s] * g for s in few], default=0)
     return PrefillPlan(torch.tensor(flat or [0], dtype=torch.int32).to(device), len(work) // 6, len(few_work) // 6, len(joins) // 4, len(few_joins) // 4,
-                       places, few_places, tile, 1 if most <= 16 else 2, sum(q_lens), len(q_lens), n_q, n_kv, causal)
+                       places, few_places, rows, few_rows, parts, few_parts, tile, 1 if most <= 16 else 2, sum(q_lens), len(q_lens), n_q, n_kv, causal)
 
 
 def prefill(q, k_cache, v_cache, block_tables, cu_seqlens_q, ctx_lens, scale, out, plan, kv_scales, causal):
@@ -368,6 +383,7 @@ def prefill(q, k_cache, v_cache, block_tables, cu_seqlens_q, ctx_lens, scale, ou
     _native.kernels().block_prefill(out.data_ptr(), o, ml, few_o, few_ml, q.data_ptr(), rows, k_cache.data_ptr(),
                                     v_cache.data_ptr(), kv_scales[0].data_ptr(), kv_scales[1].data_ptr(), block_tables.data_ptr(),
                                     table_rows, cols, cu_seqlens_q.data_ptr(), ctx_lens.data_ptr(), work, plan.n_work,
-                                    plan.n_few, work + 24 * (plan.n_work + plan.n_few), plan.n_joins, plan.n_few_joins, plan.tile, plan.few_groups,
+                                    plan.n_few, work + 24 * (plan.n_work + plan.n_few), plan.n_joins, plan.n_few_joins, plan.join_rows, plan.few_join_rows, plan.parts,
+                                    plan.few_parts, plan.tile, plan.few_groups,
                                     hq, hkv, d, bs, nb, float(scale), int(causal), CODES[k_cache.dtype], _stream(q))
     return out
