@@ -80,9 +80,12 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
   // units of the largest so far, and its inverse as a pair of bf16
   float sc_l, lg_l, unit = 0x1p-126f;
   uint32_t ones_l;
-  auto scales = [&]() __attribute__((always_inline)) {
+  float ks, vs;
+  auto ask = [&]() __attribute__((always_inline)) {
     ids = (unsigned)ids < (unsigned)a.num_blocks ? ids : 0;
-    const float ks = a.ks[(int64_t)ids * a.n_kv + kvh], vs = a.vs[(int64_t)ids * a.n_kv + kvh];
+    ks = a.ks[(int64_t)ids * a.n_kv + kvh], vs = a.vs[(int64_t)ids * a.n_kv + kvh];
+  };
+  auto scales = [&]() __attribute__((always_inline)) {
     sc_l = fmaxf(ks * a.scale_log2e, 0x1p-126f);
     const float top = wave_reduce_max(first + lane <= last ? vs : 0.f);  // (a scale behind the context may be anything)
     unit = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(fmaxf(unit, top))));
@@ -90,7 +93,7 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
     lg_l = __builtin_amdgcn_logf(part);
     ones_l = pack_bf16x2(inv, inv);
   };
-  scales();
+  ask();
   const int pos0 = ctx - qlen, rows = qlen * G;
   const int w0 = row0 + BQ * rw, f = w0 + r;
   const bool valid = f < rows;
@@ -106,12 +109,13 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
   raw4 kr[PIECES], vr[PIECES];
   float sc_next[NG], lg_next[NG], sc_now[NG], lg_now[NG];  // of the tile on its way, and of the one in use
   uint32_t ones_next[NG], ones_now[NG];
-  float unit_next = unit, unit_now = unit, unit_o = unit;  // what its exponents are short of; what this wave's O is in
+  float unit_next, unit_now = 1.f;  // what its exponents are short of
   auto at_block = [&](int j) __attribute__((always_inline)) { return min(j >> a.bs_shift, last) - first; };
   auto window = [&](int t0, int t1) __attribute__((always_inline)) {  // the blocks of tiles t0 to t1 are among the 64 here
     if (min((key0 + (t1 + 1) * BKV - 1) >> a.bs_shift, last) - first >= 64) {
       first = (key0 + t0 * BKV) >> a.bs_shift;
       ids = bt[min(first + lane, a.bt_cols - 1)];
+      ask();
       scales();
     }
   };
@@ -165,15 +169,18 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
   if (n_tiles > 0) {
     load(a.k, 0, kr);
     if constexpr (!kPhases) load(a.v, 0, vr);
-    load_scales(0);
-    turn_over();
   }
-
   u16x8 qf[8];
   {
     const bf16_t* qp = a.q + (int64_t)(q_start + tok) * a.q_stride + (int64_t)(kvh * G + hq) * D + 8 * h;
 #pragma unroll
     for (int s = 0; s < 8; ++s) qf[s] = valid ? *reinterpret_cast<const u16x8*>(qp + 16 * s) : u16x8{{0, 0, 0, 0}};
+  }
+  scales();  // (behind the loads that do not need them)
+  float unit_o = unit;  // what this wave's O is in
+  if (n_tiles > 0) {
+    load_scales(0);
+    turn_over();
   }
   f32x16 o_acc[4];
 #pragma unroll
