@@ -147,43 +147,48 @@ def append_rows(qp, kp, vp, T, stride, nq, hkv, qop, q_out_stride, positions, co
 def read_back(k_cache, v_cache, kv_scales, block_tables, ctx_lens, scratch, workspaces):
     """ops.kv_dequant_scratch of a block-scaled cache.  K and V lie in a workspace of the stream, which its next call writes again; a
     captured call has one of its own."""
-    _check_cache(k_cache, v_cache, kv_scales)
-    nb, hkv, bs, d = k_cache.shape
+    nb, hkv, bs, dev = _check_cache(k_cache, v_cache, kv_scales)
     n, cols = block_tables.shape
-    if block_tables.dtype != torch.int32 or ctx_lens.dtype != torch.int32:
+    rows, step = block_tables.stride()
+    if block_tables.dtype is not torch.int32 or ctx_lens.dtype is not torch.int32:
         raise TypeError("kv_dequant_scratch: tables and lengths are int32")
-    if (cols > 1 and block_tables.stride(1) != 1) or ctx_lens.dim() != 1 or ctx_lens.shape[0] != n or not ctx_lens.is_contiguous():
+    if (cols > 1 and step != 1) or ctx_lens.dim() != 1 or ctx_lens.numel() != n or not ctx_lens.is_contiguous():
         raise ValueError(f"kv_dequant_scratch: block_tables {tuple(block_tables.shape)}, ctx_lens {tuple(ctx_lens.shape)}")
-    dev = k_cache.device
-    if block_tables.device != dev or ctx_lens.device != dev:
-        raise ValueError(f"kv_dequant_scratch: tables on {block_tables.device}, lengths on {ctx_lens.device}, the cache on {dev}")
-    if not k_cache.is_cuda:
-        table = torch.arange(n * cols, dtype=torch.int32).view(n, cols) if scratch is None else scratch[0]
-        ks, vs = (torch.zeros((max(n * cols if scratch is None else scratch[1], 1), hkv, bs, d), dtype=torch.bfloat16) for _ in range(2))
+    if block_tables.get_device() != dev or ctx_lens.get_device() != dev:
+        raise ValueError(f"kv_dequant_scratch: tables on {block_tables.device}, lengths on {ctx_lens.device}, the cache on {k_cache.device}")
+    need = n * cols if scratch is None else scratch[1]
+    if dev < 0:
+        table = torch.arange(need, dtype=torch.int32).view(n, cols) if scratch is None else scratch[0]
+        ks, vs = (torch.zeros((max(need, 1), hkv, bs, HEAD_DIM), dtype=torch.bfloat16) for _ in range(2))
         for i, ctx in enumerate(ctx_lens.tolist()):
-            need = min(-(-ctx // bs), cols)
-            src, dst = block_tables[i, :need].long(), table[i, :need].long()
+            blocks = min(-(-ctx // bs), cols)
+            src, dst = block_tables[i, :blocks].long(), table[i, :blocks].long()
             ks[dst] = ref.block_values(k_cache[src], kv_scales[0][src]).bfloat16()
             vs[dst] = ref.block_values(v_cache[src], kv_scales[1][src]).bfloat16()
         return ks, vs, table
-    stream, captured = _stream(k_cache), torch.cuda.is_current_stream_capturing()
-    need = n * cols if scratch is None else scratch[1]
-    ws = None if captured else workspaces.get((dev, stream))
-    if ws is None or ws[0].shape[0] < need or ws[0].shape[1:] != k_cache.shape[1:]:
+    stream, captured = _stream(k_cache), torch._C._cuda_isCurrentStreamCapturing()
+    key = (dev, stream, hkv, bs)
+    ws = None if captured else workspaces.get(key)
+    if ws is None or ws[2].numel() < need:
         cap = max(need, 64)
-        ws = (*(torch.empty((cap, hkv, bs, d), dtype=torch.bfloat16, device=dev) for _ in range(2)), torch.arange(cap, dtype=torch.int32, device=dev))
+        ws = (*(torch.empty((cap, hkv, bs, HEAD_DIM), dtype=torch.bfloat16, device=k_cache.device) for _ in range(2)),
+              torch.arange(cap, dtype=torch.int32, device=k_cache.device))
         if not captured:
-            workspaces[(dev, stream)] = ws
-    ks, vs = (ws[0], ws[1]) if ws[0].shape[0] == need else (ws[0][:max(need, 1)], ws[1][:max(need, 1)])
+            workspaces[key] = ws
+    ks, vs, order = ws
+    blocks = order.numel()
+    if blocks != need:
+        blocks = max(need, 1)
+        ks, vs = ks[:blocks], vs[:blocks]
     if scratch is None:
-        table = ws[2].as_strided((n, cols), (cols, 1))
+        table = order.as_strided((n, cols), (cols, 1))
     else:
         table = scratch[0]
-        if table.dtype != torch.int32 or table.shape != (n, cols) or not table.is_contiguous() or table.device != dev:
-            raise ValueError(f"kv_dequant_scratch: the scratch's table is [{n}, {cols}] int32, contiguous, on {dev}")
+        if table.dtype != torch.int32 or table.shape != (n, cols) or not table.is_contiguous() or table.get_device() != dev:
+            raise ValueError(f"kv_dequant_scratch: the scratch's table is [{n}, {cols}] int32, contiguous, on {k_cache.device}")
     _native.kernels().block_dequant(k_cache.data_ptr(), v_cache.data_ptr(), kv_scales[0].data_ptr(), kv_scales[1].data_ptr(), ks.data_ptr(),
-                                    vs.data_ptr(), block_tables.data_ptr(), block_tables.stride(0), ctx_lens.data_ptr(), table.data_ptr(), n, cols,
-                                    nb, ks.shape[0], hkv, bs, d, CODES[k_cache.dtype], stream)
+                                    vs.data_ptr(), block_tables.data_ptr(), rows, ctx_lens.data_ptr(), table.data_ptr(), n, cols,
+                                    nb, blocks, hkv, bs, HEAD_DIM, CODES[k_cache.dtype], stream)
     return ks, vs, table
 
 
