@@ -294,10 +294,13 @@ class PrefillPlan(NamedTuple):
     causal: bool
 
 
-# Key tiles of 64 a CU from which 256-row workgroups, one a CU, are worth it, workgroups that leave no CU idle, key tiles of a part.  us with 128
-# and 256 rows, 32 / 8 heads: 300 tokens behind 3700 (9.7 tiles a CU) 60, 66; six chunks of 1000 tokens' contexts (14) 42, 41; 2000 (16) 61.0,
-# 57.8; 3000 (35) 91, 87; 4000 (63) 156, 130; 200 behind 19800 (39) 148, 102; 500 (1) 22.5, 24.5; six of 700 behind 200 (18, 2.06 turns) 60, 64.
-WIDE_TILES, SPLIT_WGS, PREFILL_TILES = 12, 256, 4
+# Key tiles of 64 a CU from which 256-row workgroups, one a CU, are worth it.  us with 128 and 256 rows, 32 / 8 heads: 300 tokens behind 3700
+# (9.7 tiles a CU) 51, 65; six chunks of 1000 tokens' contexts (14) 42, 41; 2000 (16) 61.0, 57.8; 3000 (35) 91, 87; 4000 (63) 156, 130; 200
+# behind 19800 (39) 148, 97; 500 (1) 18.8, 21.3; six of 700 behind 200 (18, 2.06 turns) 60, 64.
+WIDE_TILES = 12
+# Key tiles of a part at least, and those of a part from which two parts a CU hide each other's waits: 16 tokens, us with one and two a CU,
+# of 20480 (5 tiles a part of two) 24.0, 24.8, of 40960 (10) 35.0, 32.2, of 81920 61, 52; 32 tokens 29.9, 32.2; 44.4, 45.2; 81, 73.
+PREFILL_TILES, PAIR_TILES = 4, 10
 FEW_ROWS, FEW_WGS, FEW_KEYS = 32, 256, 256
 
 
@@ -323,10 +326,13 @@ def prefill_plan(q_lens: list[int], ctx_lens: list[int], n_q: int, n_kv: int, de
                 items.append((-(-seen // 64), s, r0))
         return items
 
-    tile, items = 256, tiles(256)
-    if sum(i[0] for i in items) * n_kv < WIDE_TILES * CUS:
-        tile = 128 if any(q_lens[s] * g > 64 for s in many) else 64
-        items = tiles(tile)
+    tile = 128 if any(q_lens[s] * g > 64 for s in many) else 64
+    items = tiles(tile)
+    if tile == 128:  # (rows of 256 that are mostly none cost what they are all worth)
+        wide = tiles(256)
+        total = sum(i[0] for i in wide)
+        if total * n_kv >= WIDE_TILES * CUS and 8 * total <= 5 * sum(i[0] for i in items):
+            tile, items = 256, wide
 
     def cut(items, unit, per, most):
         """items (units of keys, sequence, first row) -> work and joins: those of over 1.5 `per` units in parts of about `per`."""
@@ -350,7 +356,8 @@ def prefill_plan(q_lens: list[int], ctx_lens: list[int], n_q: int, n_kv: int, de
         return [x for _, w in work for x in w], joins, places, rows, cuts
 
     total = sum(i[0] for i in items)
-    work, joins, places, rows, parts = cut(items, 64, max(PREFILL_TILES, -(-total * n_kv // SPLIT_WGS)) if len(items) * n_kv < SPLIT_WGS else 1 << 30, tile)
+    wgs = CUS * (2 if tile < 256 and total * n_kv >= 2 * CUS * PAIR_TILES else 1)
+    work, joins, places, rows, parts = cut(items, 64, max(PREFILL_TILES, -(-total * n_kv // wgs)) if len(items) * n_kv < wgs else 1 << 30, tile)
     items = [(-(-ctx_lens[s] // 128), s, 0) for s in few]
     total = sum(i[0] for i in items)
     few_work, few_joins, few_places, few_rows, few_parts = cut(items, 128, max(FEW_KEYS // 128, -(-total * n_kv // FEW_WGS)), FEW_ROWS)

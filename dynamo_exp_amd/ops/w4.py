@@ -94,10 +94,10 @@ def w4_unpack(weight: W4Weight) -> torch.Tensor:
 def _shape(m: int, n: int, k: int) -> tuple[int, int, int]:
     """(waves of a workgroup, 16-row tiles of weights a wave, workgroups that K is split over).  Tiles share x's way from L2, but need
     workgroups enough for 256 CUs; us with 1, 2 and 4 tiles, groups of 128, one row: 4096 x 4096 (256 tiles of rows) 4.4, 5.0, -;
-    6144 x 4096 6.3, 5.2, 7.2; 28672 x 4096 13.9, 13.3, 12.4; 16 rows of 8192 x 8192 (512) -, 11.9, 13.2, of 11008 x 4096 (688) -, 11.5, 9.7.  More than 8 rows of a long K take two tiles and halve K: 16 rows of
-    4096 x 14336 18.2 -> 12.9 (8 rows 10.9, 10.8).  Few rows of weights split K until there are 256 workgroups or a wave has its one
-    chunk: 17 x 16000 26 -> 4.6, 1000 x 8192 11 -> 5.3.  More than 16 rows (w4_wide_kernel) split K up to 16 times: 64 rows of 4096 x 14336
-    90 -> 24.5, of 28672 x 4096 (224 workgroups) 36, 45 in two."""
+    6144 x 4096 6.3, 5.2, 7.2; 28672 x 4096 13.9, 13.3, 12.4; 16 rows: 8192 x 8192 (512) -, 11.9, 13.2; 11008 x 4096 (688) -, 11.5, 9.7.
+    More than 8 rows of a long K take two tiles and halve K: 16 rows of 4096 x 14336 18.2 -> 12.9 (8 rows 10.9, 10.8).  Few rows of weights
+    split K until there are 256 workgroups or a wave has its one chunk: 17 x 16000 26 -> 4.6, 1000 x 8192 11 -> 5.3.  More than 16 rows
+    (w4_wide_kernel) split K up to 16 times: 64 rows of 4096 x 14336 90 -> 24.5, of 28672 x 4096 (224 workgroups) 36, 45 in two."""
     tiles, chunks = -(-n // 16), -(-k // 128)
     if m > 16:  # eight tiles a workgroup, K split until there are 256 workgroups or it has two steps of 256 columns
         return 8, 2, max(1, min(chunks // 4, 16, 256 // (-(-tiles // 8) * -(-m // 64))))
