@@ -297,7 +297,7 @@ class PrefillPlan(NamedTuple):
 # Key tiles of 64 a CU from which 256-row workgroups, one a CU, are worth it.  us with 128 and 256 rows, 32 / 8 heads: 300 tokens behind 3700
 # (9.7 tiles a CU) 51, 65; six chunks of 1000 tokens' contexts (14) 42, 41; 2000 (16) 61.0, 57.8; 3000 (35) 91, 87; 4000 (63) 156, 130; 200
 # behind 19800 (39) 148, 97; 500 (1) 18.8, 21.3; six of 700 behind 200 (18, 2.06 turns) 60, 64.
-WIDE_TILES = 12
+WIDE_TILES, WIDE_WASTE = 12, 1.25
 # Key tiles of a part at least, and those of a part from which two parts a CU hide each other's waits: 16 tokens, us with one and two a CU,
 # of 20480 (5 tiles a part of two) 24.0, 24.8, of 40960 (10) 35.0, 32.2, of 81920 61, 52; 32 tokens 29.9, 32.2; 44.4, 45.2; 81, 73.
 PREFILL_TILES, PAIR_TILES = 4, 10
@@ -331,7 +331,7 @@ def prefill_plan(q_lens: list[int], ctx_lens: list[int], n_q: int, n_kv: int, de
     if tile == 128:  # (rows of 256 that are mostly none cost what they are all worth)
         wide = tiles(256)
         total = sum(i[0] for i in wide)
-        if total * n_kv >= WIDE_TILES * CUS and 8 * total <= 5 * sum(i[0] for i in items):
+        if total * n_kv >= WIDE_TILES * CUS and 2 * total <= WIDE_WASTE * sum(i[0] for i in items):
             tile, items = 256, wide
 
     def cut(items, unit, per, most):

@@ -858,3 +858,62 @@ def test_prefill_refuses_a_negative_scale():
     for scale in (-SCALE, NAN):
         with pytest.raises(ValueError, match="not negative"):
             block8.prefill(q, k8, v8, bt, cu, ctx, scale, q.clone(), ops.prefill_plan([3], [3], 4, 2, "cpu"), scales, True)
+
+
+@pytest.mark.gpu
+@both
+@pytest.mark.parametrize("bs", [16, 64, 128])
+@pytest.mark.parametrize("nq,nkv,new,ctx", [
+    (32, 8, [41], [41]), (32, 8, [64], [64]), (32, 8, [65, 64], [65, 129]), (8, 2, [130, 257, 80], [200, 5000, 80]), (16, 2, [90], [6000]),
+    (14, 2, [300, 1, 45], [310, 700, 4200]), (3, 3, [700], [900])])
+def test_prefill_wide_tiles(codes, bs, nq, nkv, new, ctx, monkeypatch):
+    """256 rows a workgroup whatever the sizes: one tile of keys, two, many, parts of them that begin anywhere, more than 64 blocks a
+    part, waves without rows, rows that end in a wave."""
+    monkeypatch.setattr(block8, "WIDE_TILES", 0)
+    monkeypatch.setattr(block8, "WIDE_WASTE", 9)
+    plan = run_prefill(codes, nq, nkv, bs, new, ctx, seed=nq + bs)
+    assert plan.tile == 256
+    monkeypatch.setattr(block8, "PREFILL_TILES", 10 ** 6)  # (keys in one part)
+    run_prefill(codes, nq, nkv, bs, new, ctx, seed=nq)
+    run_prefill(codes, nq, nkv, bs, new, ctx, seed=nq, causal=False)
+
+
+@pytest.mark.gpu
+@both
+@pytest.mark.parametrize("bs", [16, 64])
+@pytest.mark.parametrize("wide", [True, False])
+@pytest.mark.parametrize("apart", [24, 60])
+def test_prefill_scales_that_rise_and_fall(codes, bs, wide, apart, monkeypatch):
+    """Value scales 2^apart from one end of 9000 tokens to the other, either way round: the unit that sums are held in rises where the
+    64 blocks whose scales are at hand do."""
+    monkeypatch.setattr(block8, "PREFILL_TILES", 10 ** 6)  # (keys in one part)
+    if wide:
+        monkeypatch.setattr(block8, "WIDE_TILES", 0)
+        monkeypatch.setattr(block8, "WIDE_WASTE", 9)
+    nq, nkv, new, ctx = 8, 2, [70, 90], [9000, 5000]
+    table, k8, v8, ks, vs = cache_of(codes, nkv, bs, ctx, 5, junk=False)
+    for s, up in ((0, 1), (1, -1)):
+        n = -(-ctx[s] // bs)
+        vs[table[s, :n].long()] *= 2.0 ** (up * (torch.arange(n) * apart // n - apart // 2).float())[:, None]
+    q = torch.randn((160, nq, D), generator=torch.Generator().manual_seed(3)).bfloat16()
+    cu = torch.tensor([0, 70, 160], dtype=torch.int32)
+    out = torch.empty((160, nq, D), dtype=torch.bfloat16, device="cuda")
+    dev = on_gpu(q, k8, v8, table, cu, torch.tensor(ctx, dtype=torch.int32))
+    plan = ops.prefill_plan(new, ctx, nq, nkv)
+    assert (plan.tile == 256) == wide
+    ops.prefill_attention(*dev, SCALE, out, work=plan, kv_scales=tuple(on_gpu(ks, vs)))
+    want, size = attention64(q, k8, v8, ks, vs, table, new, ctx)
+    # weights of blocks 2^-apart of the unit: what falls under 2^-126 may be lost, 2^(apart - 126) of a row's largest weight a key
+    near(out.cpu(), want, size, 2, 9000 * 2.0 ** (apart - 126) * float((v8.float().abs().amax() * vs).max()))
+
+
+@pytest.mark.gpu
+@both
+def test_join_of_few_and_many_parts(codes):
+    """Parts up to four are joined eight rows a workgroup, more by a workgroup a row; rows that are not a multiple of eight."""
+    plan = run_prefill(codes, 8, 2, 64, [33, 45], [700, 900], seed=6)
+    assert plan.n_joins and 1 < plan.parts <= 4
+    plan = run_prefill(codes, 8, 2, 64, [21], [700], seed=6)
+    assert 1 < plan.parts <= 4 and plan.join_rows == 84
+    plan = run_prefill(codes, 4, 1, 64, [33], [6000], seed=6)
+    assert plan.parts > 4
