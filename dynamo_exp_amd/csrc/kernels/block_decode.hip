@@ -14,6 +14,9 @@
 // for the second product (relative 2^-8 each, as in the bf16 form; a power of two leaves that rounding as it is).  The row sum is
 // taken of the unrounded weights in fp32.
 //
+// 96 sequences of up to 3150 tokens, 32 / 8 heads, int8: 89 us, 5.5 TB/s; three of up to 60001, 64 / 8 heads, e4m3: 38.5 us with the join, 5.4
+// TB/s; one of 700 8.7 us, 44 of up to 76 in blocks of 16 5.5, both latency.
+//
 // Layouts of a chunk (lane = 16 g + r): S^T row block bb, row rho -> token 8 (rho >> 2) + 4 bb + (rho & 3), so that a lane's eight
 // scores of head r are tokens 8 g .. 8 g + 7 and, as bf16, the B operand of O^T = V^T P^T.  K comes straight from global memory (a
 // lane's 32 bytes are columns 32 g ..), V goes through a wave's own 8 KB image in LDS and is read transposed.

@@ -14,6 +14,9 @@
 // The K axis is split over the waves of a workgroup, whose sums are added in LDS in the waves' order, and over workgroups where rows
 // are few (their sums in fp32, added by a second kernel).  x rows come from L2 once for RT tiles.
 //
+// One row of 4096 x 4096 4.4 us, of 28672 x 4096 (groups of 64, zeros) 13.5 (4.7 TB/s of weights), 16 rows of 4096 x 14336 (groups of 32,
+// zeros) 14.3, of which the joined halves of K take 2.4: the latency of seven chunks a wave.
+//
 // More than 16 rows (w4_wide_kernel): x would come from L2 more often than the weights from HBM (64 rows of 28672 x 4096 took 89 us that
 // way), so a workgroup's eight waves, four tile pairs by two halves of 256 columns, read it from LDS, staged a step ahead.
 #include "block8.h"
