@@ -27,8 +27,7 @@
 
 namespace {
 
-constexpr int D = 128, BQ = 32, BKV = 64;
-constexpr int kTileBytes = BKV * D * 2;
+constexpr int D = 128, BQ = 32;
 constexpr float kRescale = 8.0f;
 constexpr int kItem = 6;  // seq, first row, first key, end of the keys, place of its sums (or -1), 0
 constexpr int kFewRows = 32;  // rows that block_rows_kernel takes
@@ -58,13 +57,15 @@ __device__ __forceinline__ float sum2(uint32_t a, uint32_t b, float c) {
 
 template <int I> using at_t = std::integral_constant<int, I>;
 
-// RW: row waves of 32 rows; KW: waves that share a tile's keys (1, or 2: 32 each); ONE: a tile's keys lie in one block
+// RW: row waves of 32 rows; KW: waves that share a tile's keys (1: 64 keys, or 4: 128, 32 each); ONE: a wave's keys of a tile lie in one block
 template <int CODE, int RW, int KW, bool ONE>
 __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const PrefillArgs a) {
-  constexpr int NW = RW * KW, PIECES = 8 / NW;  // pieces of 8 rows of a tile that a wave brings
-  constexpr int SUBS = 2 / KW;                  // 32-key pieces of a tile that a wave multiplies
-  constexpr int NG = ONE ? 1 : 4;               // scales of a tile
-  constexpr bool kPhases = NW == 8 && ONE;      // two halves of the waves, in turn with products and with the softmax
+  static_assert(KW == 1 || KW == 4, "keys of a tile");
+  constexpr int BKV = KW == 1 ? 64 : 128, kTileBytes = BKV * D * 2;
+  constexpr int NW = RW * KW, PIECES = BKV / 8 / NW;  // pieces of 8 rows of a tile that a wave brings
+  constexpr int SUBS = KW == 1 ? 2 : 1;         // 32-key pieces of a tile that a wave multiplies
+  constexpr int NG = ONE ? 1 : 2 * SUBS;        // scales of a wave's keys of a tile
+  constexpr bool kPhases = RW == 8 && ONE;      // two halves of the waves, in turn with products and with the softmax
   __shared__ __attribute__((aligned(16))) char smem[2 * 2 * kTileBytes];
   const int* item = a.work + (int64_t)blockIdx.y * kItem;
   const int kvh = blockIdx.x, G = a.G;
@@ -135,7 +136,7 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
     unit_next = unit;
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      const int i = at_block(key0 + t * BKV + 16 * g);
+      const int i = at_block(key0 + t * BKV + 32 * SUBS * kw + 16 * g);
       sc_next[g] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc_l), i));
       lg_next[g] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lg_l), i));
       ones_next[g] = __builtin_amdgcn_readlane(ones_l, i);
@@ -207,9 +208,8 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
     for (int sub = 0; sub < SUBS; ++sub)
 #pragma unroll
       for (int s2 = 0; s2 < 2; ++s2) {
-        const int g = NG == 1 ? 0 : 2 * sub + s2, g1 = NG == 1 ? 0 : 2 + s2;  // (g1: of the second wave of two that share a tile)
-        sc[sub][s2] = KW == 2 && kw ? sc_now[g1] : sc_now[g];
-        lg[sub][s2] = KW == 2 && kw ? lg_now[g1] : lg_now[g];
+        const int g = NG == 1 ? 0 : 2 * sub + s2;
+        sc[sub][s2] = sc_now[g], lg[sub][s2] = lg_now[g];
       }
     float t_s;
     if constexpr (ONE) {
@@ -259,8 +259,8 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
   };
   // pair i of a wave's 8 SUBS pairs of weights, added to the row sum
   auto add_pair = [&](int i) __attribute__((always_inline)) {
-    const int sub = i >> 3, s2 = (i >> 2) & 1, g = NG == 1 ? 0 : 2 * sub + s2, g1 = NG == 1 ? 0 : 2 + s2;
-    l_i = sum2(pf[sub][s2].w[i & 3], KW == 2 && kw ? ones_now[g1] : ones_now[g], l_i);
+    const int sub = i >> 3, s2 = (i >> 2) & 1;
+    l_i = sum2(pf[sub][s2].w[i & 3], ones_now[NG == 1 ? 0 : 2 * sub + s2], l_i);
   };
   auto mfma = [](const u16x8& x, const u16x8& y, const f32x16& c) __attribute__((always_inline)) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, x), __builtin_bit_cast(bf16x8_t, y), c, 0, 0, 0);
@@ -406,24 +406,36 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
   l_i = halves_sum(l_i);
 #pragma unroll
   for (int dt = 0; dt < 4; ++dt) o_acc[dt] *= unit_o;
-  if constexpr (KW == 2) {  // the second half of the waves hands its sums to the first
-    float* so = reinterpret_cast<float*>(smem) + rw * (BQ * D);  // [64 lanes] x 64 values, a lane's apart by 64 so that a wave's lie together
-    float* sml = reinterpret_cast<float*>(smem + RW * BQ * D * 4) + rw * 128;
+  if constexpr (KW > 1) {  // the waves of the other keys hand their sums to those of the first
+    float* so = reinterpret_cast<float*>(smem);  // [KW - 1][RW][64 lanes] x 64 values, a lane's apart by 64 so that a wave's lie together
+    float* sml = so + (KW - 1) * RW * (BQ * D);
+    static_assert((KW - 1) * RW * (BQ * D + 128) * 4 <= 4 * kTileBytes, "the images hold the sums");
     if (kw) {
+      const int at = (kw - 1) * RW + rw;
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) so[(dt * 16 + i) * 64 + lane] = o_acc[dt][i];
-      sml[lane] = m_i, sml[64 + lane] = l_i;
+        for (int i = 0; i < 16; ++i) so[at * (BQ * D) + (dt * 16 + i) * 64 + lane] = o_acc[dt][i];
+      sml[at * 128 + lane] = m_i, sml[at * 128 + 64 + lane] = l_i;
     }
     __syncthreads();
     if (kw) return;
-    const float m2 = sml[lane], l2 = sml[64 + lane], M = fmaxf(m_i, m2), e1 = fast_exp2(m_i - M), e2 = fast_exp2(m2 - M);
+    float m[KW - 1], M = m_i;
 #pragma unroll
-    for (int dt = 0; dt < 4; ++dt)
+    for (int k = 0; k < KW - 1; ++k) M = fmaxf(M, m[k] = sml[(k * RW + rw) * 128 + lane]);
+    const float e0 = fast_exp2(m_i - M);
+    l_i *= e0;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) o_acc[dt][i] = e1 * o_acc[dt][i] + e2 * so[(dt * 16 + i) * 64 + lane];
-    l_i = e1 * l_i + e2 * l2;
+    for (int dt = 0; dt < 4; ++dt) o_acc[dt] *= e0;
+#pragma unroll
+    for (int k = 0; k < KW - 1; ++k) {
+      const float e = fast_exp2(m[k] - M);
+      l_i += e * sml[(k * RW + rw) * 128 + 64 + lane];
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o_acc[dt][i] += e * so[(k * RW + rw) * (BQ * D) + (dt * 16 + i) * 64 + lane];
+    }
     m_i = M;
   }
   if (place >= 0) {  // the sums as they are
@@ -737,16 +749,12 @@ extern "C" int dx_block_prefill(void* out, float* ws_o, float* ws_ml, float* few
   if (n_work) {
     const dim3 grid(n_kv, n_work);
     a.tile = tile;
-#define DX_BPT(C, ONE)                                                                         \
-  do {                                                                                         \
-    if (tile == 256) block_prefill_kernel<C, 8, 1, ONE><<<grid, 512, 0, stream>>>(a);          \
-    else if (tile == 128) block_prefill_kernel<C, 4, 1, ONE><<<grid, 256, 0, stream>>>(a);     \
-    else block_prefill_kernel<C, 2, 2, ONE><<<grid, 256, 0, stream>>>(a);                      \
-  } while (0)
-#define DX_BP(C)                              \
-  do {                                        \
-    if (block_size >= BKV) DX_BPT(C, true);   \
-    else DX_BPT(C, false);                    \
+#define DX_BPT(C, RW, KW, ONE) block_prefill_kernel<C, RW, KW, ONE><<<grid, 64 * RW * KW, 0, stream>>>(a)
+#define DX_BP(C)                                                                                      \
+  do {                                                                                                \
+    if (tile == 256) block_size >= 64 ? DX_BPT(C, 8, 1, true) : DX_BPT(C, 8, 1, false);               \
+    else if (tile == 128) block_size >= 64 ? DX_BPT(C, 4, 1, true) : DX_BPT(C, 4, 1, false);          \
+    else block_size >= 32 ? DX_BPT(C, 2, 4, true) : DX_BPT(C, 2, 4, false);                           \
   } while (0)
     if (code == kE4m3) DX_BP(kE4m3);
     else DX_BP(kInt8);

@@ -298,9 +298,9 @@ class PrefillPlan(NamedTuple):
 # (9.7 tiles a CU) 51, 65; six chunks of 1000 tokens' contexts (14) 42, 41; 2000 (16) 61.0, 57.8; 3000 (35) 91, 87; 4000 (63) 156, 130; 200
 # behind 19800 (39) 148, 97; 500 (1) 18.8, 21.3; six of 700 behind 200 (18, 2.06 turns) 60, 64.
 WIDE_TILES, WIDE_WASTE = 12, 1.25
-# Key tiles of a part at least, and those of a part from which two parts a CU hide each other's waits: 16 tokens, us with one and two a CU,
-# of 20480 (5 tiles a part of two) 24.0, 24.8, of 40960 (10) 35.0, 32.2, of 81920 61, 52; 32 tokens 29.9, 32.2; 44.4, 45.2; 81, 73.
-PREFILL_TILES, PAIR_TILES = 4, 10
+# Keys of a part at least, and key tiles of a part from which two parts of 128 rows a CU hide each other's waits: 32 tokens, us with one and
+# two a CU, of 20480 (5 tiles a part of two) 29.9, 32.2, of 40960 (10) 44.4, 45.2, of 81920 81, 73.
+PREFILL_KEYS, PAIR_TILES = 256, 16
 FEW_ROWS, FEW_WGS, FEW_KEYS = 32, 256, 256
 
 
@@ -318,12 +318,12 @@ def prefill_plan(q_lens: list[int], ctx_lens: list[int], n_q: int, n_kv: int, de
 
     def tiles(tile):
         """[key tiles, sequence, first row] of row tiles."""
-        items = []
+        items, keys = [], 128 if tile == 64 else 64
         for s in many:
             ql, cl = q_lens[s], ctx_lens[s]
             for r0 in range(0, ql * g, tile):
                 seen = cl - ql + (min(r0 + tile, ql * g) - 1) // g + 1 if causal else cl
-                items.append((-(-seen // 64), s, r0))
+                items.append((-(-seen // keys), s, r0))
         return items
 
     tile = 128 if any(q_lens[s] * g > 64 for s in many) else 64
@@ -356,8 +356,10 @@ def prefill_plan(q_lens: list[int], ctx_lens: list[int], n_q: int, n_kv: int, de
         return [x for _, w in work for x in w], joins, places, rows, cuts
 
     total = sum(i[0] for i in items)
-    wgs = CUS * (2 if tile < 256 and total * n_kv >= 2 * CUS * PAIR_TILES else 1)
-    work, joins, places, rows, parts = cut(items, 64, max(PREFILL_TILES, -(-total * n_kv // wgs)) if len(items) * n_kv < wgs else 1 << 30, tile)
+    wgs = CUS * (2 if tile == 128 and total * n_kv >= 2 * CUS * PAIR_TILES else 1)
+    unit = 128 if tile == 64 else 64
+    per = max(PREFILL_KEYS // unit, -(-total * n_kv // wgs)) if len(items) * n_kv < wgs else 1 << 30
+    work, joins, places, rows, parts = cut(items, unit, per, tile)
     items = [(-(-ctx_lens[s] // 128), s, 0) for s in few]
     total = sum(i[0] for i in items)
     few_work, few_joins, few_places, few_rows, few_parts = cut(items, 128, max(FEW_KEYS // 128, -(-total * n_kv // FEW_WGS)), FEW_ROWS)

@@ -867,7 +867,7 @@ def test_prefill_wide_tiles(codes, bs, nq, nkv, new, ctx, monkeypatch):
     monkeypatch.setattr(block8, "WIDE_WASTE", 9)
     plan = run_prefill(codes, nq, nkv, bs, new, ctx, seed=nq + bs)
     assert plan.tile == 256
-    monkeypatch.setattr(block8, "PREFILL_TILES", 10 ** 6)  # (keys in one part)
+    monkeypatch.setattr(block8, "PREFILL_KEYS", 10 ** 8)  # (keys in one part)
     run_prefill(codes, nq, nkv, bs, new, ctx, seed=nq)
     run_prefill(codes, nq, nkv, bs, new, ctx, seed=nq, causal=False)
 
@@ -880,7 +880,7 @@ def test_prefill_wide_tiles(codes, bs, nq, nkv, new, ctx, monkeypatch):
 def test_prefill_scales_that_rise_and_fall(codes, bs, wide, apart, monkeypatch):
     """Value scales 2^apart from one end of 9000 tokens to the other, either way round: the unit that sums are held in rises where the
     64 blocks whose scales are at hand do."""
-    monkeypatch.setattr(block8, "PREFILL_TILES", 10 ** 6)  # (keys in one part)
+    monkeypatch.setattr(block8, "PREFILL_KEYS", 10 ** 8)  # (keys in one part)
     if wide:
         monkeypatch.setattr(block8, "WIDE_TILES", 0)
         monkeypatch.setattr(block8, "WIDE_WASTE", 9)
