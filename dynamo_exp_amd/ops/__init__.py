@@ -755,7 +755,8 @@ def prefill_attention(q, k_cache, v_cache, block_tables, cu_seqlens_q, ctx_lens,
     `work` is the int32 device tensor from :func:`prefill_work_list`.  An fp8
     cache goes through :func:`kv_dequant_scratch` first (`scratch`: its packed
     table).  kv_scales tensors: a block-scaled cache (block8), read as it is;
-    `work` is a :func:`prefill_plan` then.
+    `work` is a :func:`prefill_plan` then (None: made
+    here, from lengths that are waited for).
     """
     if not q.is_cuda:
         out.copy_(ref.paged_attention(q, k_cache, v_cache, block_tables, cu_seqlens_q, ctx_lens, scale, k_cache.shape[2],
