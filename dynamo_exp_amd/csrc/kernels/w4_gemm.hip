@@ -17,8 +17,9 @@
 // One row of 4096 x 4096 4.4 us, of 28672 x 4096 (groups of 64, zeros) 13.5 (4.7 TB/s of weights), 16 rows of 4096 x 14336 (groups of 32,
 // zeros) 14.3, of which the joined halves of K take 2.4: the latency of seven chunks a wave.
 //
-// More than 16 rows (w4_wide_kernel): x would come from L2 more often than the weights from HBM (64 rows of 28672 x 4096 took 89 us that
-// way), so a workgroup's eight waves, four tile pairs by two halves of 256 columns, read it from LDS, staged a step ahead.
+// More than 16 rows are bands of 16, workgroups of their own, while there is little work; then (w4_wide_kernel) x would come from L2 more often
+// than the weights from HBM (64 rows of 28672 x 4096 50 us, now 31), so a workgroup's eight waves, four tile pairs by two halves of
+// 256 columns, read it from LDS, staged a step ahead.
 #include "block8.h"
 
 #include <type_traits>
@@ -396,10 +397,12 @@ extern "C" int dx_w4_gemm(void* y, int64_t ldy, const void* x, int64_t ldx, cons
     if (rt == 2) return launch_group<2, T_, E_>(a, group, waves, splits, stream);            \
     return launch_group<1, T_, E_>(a, group, waves, splits, stream);                         \
   } while (0)
-  if (M <= 4) DX_W4(1, 1);
-  if (M <= 8) DX_W4(1, 2);
-  if (M <= 16) DX_W4(1, 4);
   if (splits < 1 || (splits > 1 && ws == nullptr)) return -3;
+  if (rt > 0) {
+    if (M <= 4) DX_W4(1, 1);
+    if (M <= 8) DX_W4(1, 2);
+    DX_W4(1, 4);
+  }
   return M <= 32 ? launch_wide<2>(a, group, splits, stream) : launch_wide<4>(a, group, splits, stream);
 #undef DX_W4
 }

@@ -13,6 +13,10 @@ from .. import _native
 
 GROUPS = (32, 64, 128)
 MAX_ROWS = 256
+# More than 16 rows go to w4_wide_kernel, which has x in LDS, from so much work or so many weights on.  us, bands of 16 rows and wide: 64 rows of
+# 2048 x 2048 5.0, 11, of 4096 x 4096 9.3, 15.6, of 8192 x 4096 14.9, 19.6, of 8192 x 8192 26.3, 25.8; 128 rows of 8192 x 4096 26.3, 25.8, of 4096 x
+# 14336 43, 33; 20 rows of 28672 x 4096 24.8, 19.5.
+WIDE_WORK, WIDE_WEIGHTS = 4 << 30, 80 << 20
 
 
 class W4Weight(NamedTuple):
@@ -96,16 +100,18 @@ def _shape(m: int, n: int, k: int) -> tuple[int, int, int]:
     workgroups enough for 256 CUs; us with 1, 2 and 4 tiles, groups of 128, one row: 4096 x 4096 (256 tiles of rows) 4.4, 5.0, -;
     6144 x 4096 6.3, 5.2, 7.2; 28672 x 4096 13.9, 13.3, 12.4; 16 rows: 8192 x 8192 (512) -, 11.9, 13.2; 11008 x 4096 (688) -, 11.5, 9.7.
     More than 8 rows of a long K take two tiles and halve K: 16 rows of 4096 x 14336 18.2 -> 12.9 (8 rows 10.9, 10.8).  Few rows of weights
-    split K until there are 256 workgroups or a wave has its one chunk: 17 x 16000 26 -> 4.6, 1000 x 8192 11 -> 5.3.  More than 16 rows
-    (w4_wide_kernel) split K up to 16 times: 64 rows of 4096 x 14336 90 -> 24.5, of 28672 x 4096 (224 workgroups) 36, 45 in two."""
-    tiles, chunks = -(-n // 16), -(-k // 128)
-    if m > 16:  # eight tiles a workgroup, K split until there are 256 workgroups or it has two steps of 256 columns
-        return 8, 2, max(1, min(chunks // 4, 16, 256 // (-(-tiles // 8) * -(-m // 64))))
-    rt = 4 if tiles >= (640 if m > 8 else 1024) else 2 if tiles >= 384 else 1
+    split K until there are 256 workgroups or a wave has its one chunk: 17 x 16000 26 -> 4.6, 1000 x 8192 11 -> 5.3.  More than 16 rows are
+    bands of 16, which add to the workgroups, or (0 tiles) w4_wide_kernel's, which splits K up to 16 times: 64 rows of 28672 x 4096 (224 workgroups)
+    31 in one part, 42 in two."""
+    tiles, chunks, bands = -(-n // 16), -(-k // 128), max(1, -(-m // 16))
+    if m > 16 and (m * n * k > WIDE_WORK or n * k > WIDE_WEIGHTS):  # eight tiles a workgroup, K split until there are 256 workgroups or it has two steps of 256 columns
+        return 8, 0, max(1, min(chunks // 4, 16, 256 // (-(-tiles // 8) * -(-m // 64))))
+    work = tiles * bands
+    rt = 4 if work >= (640 if m > 8 else 1024) else 2 if work >= 384 else 1
     splits = 1
-    if tiles < 512 and m > 8 and k >= 8192:
+    if work < 384 and m > 8 and k >= 8192:
         rt = splits = 2
-    groups = -(-tiles // rt)
+    groups = -(-tiles // rt) * bands
     if groups < 128:
         splits = max(splits, min(chunks // 8, 256 // groups))
     waves = 8

@@ -179,3 +179,41 @@ def test_refuses_a_weight_laid_out_otherwise():
                 w._replace(scales=w.scales.cpu()), w._replace(zeros=w.zeros.cpu())):
         with pytest.raises(ValueError):
             ops.w4_linear(x, bad)
+
+
+@pytest.fixture
+def wide(monkeypatch):
+    """More than 16 rows through w4_wide_kernel whatever the sizes."""
+    from dynamo_exp_amd.ops import w4
+    monkeypatch.setattr(w4, "WIDE_WORK", -1)
+    w4._shape.cache_clear()
+    yield w4
+    w4._shape.cache_clear()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("m,n,k", [(17, 48, 1152), (33, 250, 256), (64, 31, 4096), (65, 40, 640), (130, 64, 128), (256, 33, 256), (32, 513, 2176), (48, 128, 1408)])
+def test_wide_product(m, n, k, group, zeros, wide):
+    assert wide._shape(m, n, k)[1] == 0
+    codes, scales, z, w = make(n, k, group, zeros, seed=m + n)
+    x = torch.randn((m, k), generator=torch.Generator().manual_seed(k)).bfloat16()
+    weight = ops.w4_pack(codes.cuda(), scales.cuda(), None if z is None else z.cuda(), group)
+    near(ops.w4_linear(x.cuda(), weight).cpu(), x, w, scales, group)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [32, 96, 160, 4128])
+def test_wide_columns_that_end_inside_a_chunk(k, wide):
+    codes, scales, z, w = make(70, k, 32, True, seed=k)
+    x = torch.randn((20, k), generator=torch.Generator().manual_seed(k)).bfloat16()
+    near(ops.w4_linear(x.cuda(), ops.w4_pack(codes.cuda(), scales.cuda(), z.cuda(), 32)).cpu(), x, w, scales, 32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(20, 28672, 4096), (256, 2048, 2048), (100, 17, 16000), (129, 1000, 8192), (17, 4096, 4096)])
+def test_bands_of_rows(m, n, k):
+    codes, scales, z, w = make(n, k, 64, True, seed=n)
+    x = torch.randn((m, k), generator=torch.Generator().manual_seed(k)).bfloat16()
+    near(ops.w4_linear(x.cuda(), ops.w4_pack(codes.cuda(), scales.cuda(), z.cuda(), 64)).cpu(), x, w, scales, 64)
