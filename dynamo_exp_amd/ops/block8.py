@@ -302,12 +302,17 @@ WIDE_TILES, WIDE_WASTE = 12, 1.25
 # two a CU, of 20480 (5 tiles a part of two) 29.9, 32.2, of 40960 (10) 44.4, 45.2, of 81920 81, 73.
 PREFILL_KEYS, PAIR_TILES = 256, 16
 FEW_ROWS, FEW_WGS, FEW_KEYS = 32, 256, 256
+# Keys (times heads) of sequences of few rows that go with the others' tiles, where none is longer than theirs: a launch (and its join) less.  us,
+# apart and together: 5 and 4 tokens, 14 / 2 heads, alone 14.2, 7.6, behind 1700 and 1200 24.1, 12.8; 32 / 8 heads, four of 300 and eight of 4
+# behind 296 23.0, 15.6, 5000 and four of 6 behind 1794 236, 220.
+BESIDE_KEYS = 65536
 
 
 def prefill_plan(q_lens: list[int], ctx_lens: list[int], n_q: int, n_kv: int, device="cuda", causal: bool = True) -> PrefillPlan:
     """Cuts prompt chunks (q_lens new tokens each, the last of ctx_lens tokens) into work items for ``prefill_attention`` over a
     block-scaled cache: tiles of query rows, heaviest first, and where those are too few for the chip, parts of their keys.  Sequences of
-    at most 32 rows a key/value head (new tokens times query heads per key/value head) go to a kernel of their own."""
+    at most 32 rows a key/value head (new tokens times query heads per key/value head) go to a kernel of their own, where they have many keys
+    or are alone."""
     if len(q_lens) != len(ctx_lens) or any(q < 0 or c < q for q, c in zip(q_lens, ctx_lens)):
         raise ValueError(f"prefill_plan: {list(q_lens)} new tokens of {list(ctx_lens)}")
     if n_kv < 1 or n_q % n_kv:
@@ -315,6 +320,8 @@ def prefill_plan(q_lens: list[int], ctx_lens: list[int], n_q: int, n_kv: int, de
     g = n_q // n_kv
     few = [s for s, ql in enumerate(q_lens) if 0 < ql * g <= FEW_ROWS]
     many = [s for s, ql in enumerate(q_lens) if ql * g > FEW_ROWS]
+    if many and sum(ctx_lens[s] for s in few) * n_kv <= BESIDE_KEYS and max((ctx_lens[s] for s in few), default=0) <= max(ctx_lens[s] for s in many):
+        few, many = [], sorted(few + many)
 
     def tiles(tile):
         """[key tiles, sequence, first row] of row tiles."""

@@ -677,8 +677,11 @@ def test_nothing_to_do():
     ops.prefill_attention(q, k8, v8, i32(1, 2), i32(2), i32(1), SCALE, torch.empty_like(q), work=ops.prefill_plan([0], [0], 4, 2), kv_scales=scales)
 
 
-def test_plan_covers_every_row_and_key():
-    """The plan's items: each row tile's keys once, in whole tiles of 64, parts behind one another in the workspace."""
+@pytest.mark.parametrize("beside", [-1, block8.BESIDE_KEYS])
+def test_plan_covers_every_row_and_key(beside, monkeypatch):
+    """The plan's items: each row tile's keys once, in whole tiles of 64, parts behind one another in the workspace; sequences of few rows
+    as a kind of their own, or with the others where they have few keys."""
+    monkeypatch.setattr(block8, "BESIDE_KEYS", beside)
     g = torch.Generator().manual_seed(2)
     for nq, nkv in ((32, 8), (14, 2), (16, 1), (8, 8)):
         for n in range(1, 5):
@@ -693,7 +696,8 @@ def test_plan_covers_every_row_and_key():
             for w, j, places in ((items[:p.n_work], joins[:p.n_joins], p.places), (items[p.n_work:], joins[p.n_joins:], p.few_places)):
                 assert sorted(x[4] for x in w if x[4] >= 0) == list(range(places)) and sum(x[3] for x in j) == places
             for s, (ql, cl) in enumerate(zip(new, ctx)):
-                few = 0 < ql * G <= block8.FEW_ROWS
+                few = any(x[0] == s for x in items[p.n_work:])
+                assert few == (0 < ql * G <= block8.FEW_ROWS) or (beside > 0 and not p.n_few)
                 assert not few or ql * G <= 16 * p.few_groups
                 w, j, step = (items[p.n_work:], joins[p.n_joins:], block8.FEW_ROWS) if few else (items[:p.n_work], joins[:p.n_joins], tile)
                 assert sum(x[0] == s for x in items) == sum(x[0] == s for x in w)
@@ -712,11 +716,14 @@ def test_plan_covers_every_row_and_key():
 @both
 @pytest.mark.parametrize("nq,nkv", [(8, 2), (14, 2), (32, 8), (48, 1), (3, 3)])
 @pytest.mark.parametrize("bs", [16, 64])
-def test_prefill_few_rows(codes, nq, nkv, bs):
+def test_prefill_few_rows(codes, nq, nkv, bs, monkeypatch):
     """Sequences of 1 to 64 rows a key/value head (few, or a tile of 64), in one part and in many, beside one of many rows."""
-    for new, ctx in (([1, 2, 5], [1, 3, 400]), ([16, 1, 100, 3], [2100, 900, 300, 70]), ([4], [9000])):
-        plan = run_prefill(codes, nq, nkv, bs, new, ctx, seed=nq + bs)
-        assert bool(plan.n_few) == any(0 < n * nq // nkv <= block8.FEW_ROWS for n in new)
+    for beside in (-1, block8.BESIDE_KEYS):
+        monkeypatch.setattr(block8, "BESIDE_KEYS", beside)
+        for new, ctx in (([1, 2, 5], [1, 3, 400]), ([16, 1, 100, 3], [2100, 900, 300, 70]), ([4], [9000])):
+            plan = run_prefill(codes, nq, nkv, bs, new, ctx, seed=nq + bs)
+            few = [0 < n * nq // nkv <= block8.FEW_ROWS for n in new]
+            assert bool(plan.n_few) == any(few) or (beside > 0 and not all(few))
     run_prefill(codes, nq, nkv, bs, [3, 1], [777, 1], seed=2, causal=False)
 
 
