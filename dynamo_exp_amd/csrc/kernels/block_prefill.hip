@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
   constexpr int NW = RW * KW, PIECES = BKV / 8 / NW;  // pieces of 8 rows of a tile that a wave brings
   constexpr int SUBS = KW == 1 ? 2 : 1;         // 32-key pieces of a tile that a wave multiplies
   constexpr int NG = ONE ? 1 : 2 * SUBS;        // scales of a wave's keys of a tile
-  constexpr bool kPhases = RW == 8 && ONE;      // two halves of the waves, in turn with products and with the softmax
+  constexpr bool kPhases = RW == 8;             // two halves of the waves, in turn with products and with the softmax
   __shared__ __attribute__((aligned(16))) char smem[2 * 2 * kTileBytes];
   const int* item = a.work + (int64_t)blockIdx.y * kItem;
   const int kvh = blockIdx.x, G = a.G;
@@ -111,9 +111,7 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
 
   // ---- a tile's codes: piece p of this wave is rows 8 (PIECES wid + p) .. + 7, a lane 16 columns of one of them
   raw4 kr[PIECES], vr[PIECES];
-  float sc_next[NG], lg_next[NG], sc_now[NG], lg_now[NG];  // of the tile on its way, and of the one in use
-  uint32_t ones_next[NG], ones_now[NG];
-  float unit_next, unit_now = 1.f;  // what its exponents are short of
+  uint32_t ones_now[NG];  // of the tile whose weights are here
   auto at_block = [&](int j) __attribute__((always_inline)) { return min(j >> a.bs_shift, last) - first; };
   auto window = [&](int t0, int t1) __attribute__((always_inline)) {  // the blocks of tiles t0 to t1 are among the 64 here
     if (min((key0 + (t1 + 1) * BKV - 1) >> a.bs_shift, last) - first >= 64) {
@@ -131,21 +129,6 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
       const uint8_t* at = from + ((block << a.bs_shift) + (j & ((1 << a.bs_shift) - 1))) * D;  // (the same in all lanes)
       to[p] = *reinterpret_cast<const raw4*>(at + (uint32_t)(lane >> 3) * D + 16 * (lane & 7));
     }
-  };
-  auto load_scales = [&](int t) __attribute__((always_inline)) {
-    unit_next = unit;
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-      const int i = at_block(key0 + t * BKV + 32 * SUBS * kw + 16 * g);
-      sc_next[g] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc_l), i));
-      lg_next[g] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lg_l), i));
-      ones_next[g] = __builtin_amdgcn_readlane(ones_l, i);
-    }
-  };
-  auto turn_over = [&]() __attribute__((always_inline)) {  // the tile that was on its way is the tile in use
-    unit_now = unit_next;
-#pragma unroll
-    for (int g = 0; g < NG; ++g) sc_now[g] = sc_next[g], lg_now[g] = lg_next[g], ones_now[g] = ones_next[g];
   };
   // (whatever lies behind the context may be a NaN)
   auto behind = [&](int t, raw4(&x)[PIECES]) __attribute__((always_inline)) {
@@ -182,10 +165,6 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
   }
   scales();  // (behind the loads that do not need them)
   float unit_o = unit;  // what this wave's O is in
-  if (n_tiles > 0) {
-    load_scales(0);
-    turn_over();
-  }
   f32x16 o_acc[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) o_acc[i] = f32x16{};
@@ -205,12 +184,14 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
     // a score's factor, and what its exponent is short of: one of a tile, or one each 16 keys (group 2 sub + s2 of this wave's)
     float sc[2][2], lg[2][2];
 #pragma unroll
-    for (int sub = 0; sub < SUBS; ++sub)
-#pragma unroll
-      for (int s2 = 0; s2 < 2; ++s2) {
-        const int g = NG == 1 ? 0 : 2 * sub + s2;
-        sc[sub][s2] = sc_now[g], lg[sub][s2] = lg_now[g];
-      }
+    for (int g = 0; g < NG; ++g) {
+      const int i = at_block(j0 + 16 * g);
+      const float x = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc_l), i));
+      const float y = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lg_l), i));
+      if (NG == 1) sc[0][0] = sc[0][1] = sc[1][0] = sc[1][1] = x, lg[0][0] = lg[0][1] = lg[1][0] = lg[1][1] = y;
+      else sc[g >> 1][g & 1] = x, lg[g >> 1][g & 1] = y;
+      ones_now[g] = __builtin_amdgcn_readlane(ones_l, i);
+    }
     float t_s;
     if constexpr (ONE) {
       float ta = s0[0], tb = s0[1];
@@ -250,9 +231,9 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
       }
     }
     l_i *= alpha;
-    if (unit_o != unit_now || __builtin_amdgcn_ballot_w64(alpha != 1.f)) {
-      const float both = alpha * (unit_o * __builtin_amdgcn_rcpf(unit_now));
-      unit_o = unit_now;
+    if (unit_o != unit || __builtin_amdgcn_ballot_w64(alpha != 1.f)) {
+      const float both = alpha * (unit_o * __builtin_amdgcn_rcpf(unit));
+      unit_o = unit;
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt) o_acc[dt] *= both;
     }
@@ -334,20 +315,17 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
       window(0, min(2, end));
       bring_k(0);
       load(a.v, 0, vr);
-      load_scales(0);
       meet();
       if (late) {
         bring_v(0);
         meet();
       }
       line(at_t<0>{}, at_t<16>{}, k_at(0), 0, nothing);
-      turn_over();
       bring_k(1);
       for (int t = 0; t < end; ++t) {
         meet();
         __builtin_amdgcn_s_setprio(0);
-        window(t + 1, min(t + 3, end));
-        load_scales(t + 1);
+        window(t, min(t + 3, end));
         bring_v(t + late);
         weights(jw + t * BKV);
         again();
@@ -356,10 +334,10 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
         line(at_t<0>{}, at_t<32>{}, k_at(t + 1), v_at(t), [&](int i) __attribute__((always_inline)) {
           if (i >= 14 && i < 30) add_pair(i - 14);
         });
-        turn_over();
         bring_k(t + 2);
       }
       meet();
+      window(end, end);
       weights(jw + end * BKV);
       bring_v(end + late);
       again();
@@ -377,11 +355,10 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
     }
     __syncthreads();
     for (int t = 0; t < n_tiles; ++t) {
+      window(t, min(t + 1, n_tiles - 1));
       if (t + 1 < n_tiles) {
-        window(t + 1, t + 1);
         load(a.k, t + 1, kr);
         load(a.v, t + 1, vr);
-        load_scales(t + 1);
       }
       const int j0 = jw + t * BKV;
       if (j0 <= wave_max) {
@@ -396,7 +373,6 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
         store(image(t + 1), kr);
         behind(t + 1, vr);
         store(image(t + 1) + kTileBytes, vr);
-        turn_over();
       }
       __syncthreads();
     }
