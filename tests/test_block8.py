@@ -918,3 +918,54 @@ def test_join_of_few_and_many_parts(codes):
     assert 1 < plan.parts <= 4 and plan.join_rows == 84
     plan = run_prefill(codes, 4, 1, 64, [33], [6000], seed=6)
     assert plan.parts > 4
+
+
+@pytest.mark.gpu
+@both
+def test_prefill_captured_and_on_two_streams(codes, monkeypatch):
+    """A step of prompts (tiles, parts and their join, few rows in parts) captured, replayed with other rows and another cache's codes between
+    eager calls; and two such calls at once on two streams, each with its workspace."""
+    monkeypatch.setattr(block8, "BESIDE_KEYS", -1)
+    nq, nkv, bs, new, ctx = 8, 2, 64, [70, 3, 40], [900, 2000, 40]
+    table, k8, v8, ks, vs = cache_of(codes, nkv, bs, ctx, 3)
+    plan = ops.prefill_plan(new, ctx, nq, nkv)
+    assert plan.n_joins and plan.n_few_joins
+    cu = torch.tensor([0, 70, 73, 113], dtype=torch.int32)
+    q, k, v, t, c, n, s0, s1 = on_gpu(torch.zeros((113, nq, D), dtype=torch.bfloat16), k8, v8, table, cu, torch.tensor(ctx, dtype=torch.int32), ks, vs)
+    out = torch.zeros_like(q)
+    call = lambda q, out: ops.prefill_attention(q, k, v, t, c, n, SCALE, out, work=plan, kv_scales=(s0, s1))  # noqa: E731
+    call(q, out)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.inference_mode(), torch.cuda.graph(graph):
+        call(q, out)
+    g = torch.Generator().manual_seed(8)
+    for turn in range(3):
+        rows = torch.randn((113, nq, D), generator=g).bfloat16()
+        bits(k).copy_(bits(k8).roll(turn, 0) if turn else bits(k8))
+        s0.copy_(ks.roll(turn, 0))
+        q.copy_(rows)
+        graph.replay()
+        got = out.clone()
+        eager = torch.empty_like(out)
+        call(q, eager)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got.view(torch.int16), eager.view(torch.int16)) and torch.equal(out.view(torch.int16), eager.view(torch.int16))
+        if turn == 0:
+            near(got.cpu(), *attention64(rows, k8, v8, ks, vs, table, new, ctx), 2)
+    bits(k).copy_(bits(k8))
+    s0.copy_(ks)
+    qs = [torch.randn((113, nq, D), generator=g).bfloat16() for _ in range(2)]
+    streams, outs = [torch.cuda.Stream() for _ in range(2)], []
+    ins = [x.cuda() for x in qs]
+    torch.cuda.synchronize()
+    for x, s in zip(ins, streams):
+        with torch.cuda.stream(s):
+            outs.append([torch.empty_like(out) for _ in range(4)])
+            for o in outs[-1]:
+                call(x, o)
+    torch.cuda.synchronize()
+    for x, os in zip(qs, outs):
+        near(os[0].cpu(), *attention64(x, k8, v8, ks, vs, table, new, ctx), 2)
+        assert all(torch.equal(o.view(torch.int16), os[0].view(torch.int16)) for o in os)
