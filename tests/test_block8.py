@@ -969,3 +969,36 @@ def test_prefill_captured_and_on_two_streams(codes, monkeypatch):
     for x, os in zip(qs, outs):
         near(os[0].cpu(), *attention64(x, k8, v8, ks, vs, table, new, ctx), 2)
         assert all(torch.equal(o.view(torch.int16), os[0].view(torch.int16)) for o in os)
+
+
+@pytest.mark.gpu
+@both
+def test_blocks_past_32_bits(codes):
+    """The last blocks of a cache of 2.7 GB a side: the same results, bit for bit, as at the front of a small one."""
+    nq, nkv, bs, blocks = 16, 8, 64, 41000
+    small = block8.alloc(24, nkv, bs, CODES[codes])
+    big = (*(torch.empty((blocks, nkv, bs, D), dtype=torch.uint8, device="cuda").view(CODES[codes]) for _ in range(2)),
+           tuple(torch.zeros((blocks, nkv), device="cuda") for _ in range(2)))
+    order = torch.randperm(24, generator=torch.Generator().manual_seed(1)).to(torch.int32).view(2, 12)
+    cs = ref.rope_cos_sin(D, 800, 500000.0).cuda()
+    g = torch.Generator().manual_seed(2)
+    spans = [(0, 700), (0, 333)]
+    qkv = torch.randn((1033, (nq + 2 * nkv) * D), generator=g).bfloat16()
+    pos = torch.cat([torch.arange(a, b) for a, b in spans]).cuda()
+    got = []
+    for (k8, v8, scales), first in ((small, 0), (big, blocks - 24)):
+        table = order + first
+        row = qkv.cuda()
+        ops.rope_cache(row, pos, cs, slots_of(table, spans, bs).cuda(), k8, v8, nq, nkv, D, bs, kv_scales=scales)
+        q = row[:, : nq * D].unflatten(1, (nq, D))
+        ctx, cu, bt = torch.tensor([700, 333], dtype=torch.int32).cuda(), torch.tensor([0, 700, 1033], dtype=torch.int32).cuda(), table.cuda()
+        outs = [torch.empty((1033, nq, D), dtype=torch.bfloat16, device="cuda"), torch.empty((2, nq, D), dtype=torch.bfloat16, device="cuda")]
+        ops.prefill_attention(q, k8, v8, bt, cu, ctx, SCALE, outs[0], work=ops.prefill_plan([700, 333], [700, 333], nq, nkv), kv_scales=scales)
+        ops.decode_attention(q[699:701], k8, v8, bt, ctx, SCALE, outs[1], 3, kv_scales=scales)
+        few = torch.empty((3, nq, D), dtype=torch.bfloat16, device="cuda")
+        ops.prefill_attention(q[:3], k8, v8, bt[:1], torch.tensor([0, 3], dtype=torch.int32).cuda(), ctx[:1], SCALE, few, work=ops.prefill_plan([3], [700], nq, nkv), kv_scales=scales)
+        back = ops.kv_dequant_scratch(k8, v8, bt, ctx, kv_scales=scales)
+        got.append([x.clone().cpu() for x in (row, *outs, few, back[0][:10], back[1][:10], scales[0][bt[0, :11].long()], scales[1][bt[0, :11].long()])])
+    for a, b in zip(*got):
+        assert torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
+    near(got[1][1][:700], *attention64(got[1][0][:700, : nq * D].view(700, nq, D), *(x.cpu() for x in (small[0], small[1], *small[2])), order, [700, 0], [700, 333]), 2)
