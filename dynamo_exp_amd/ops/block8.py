@@ -230,7 +230,7 @@ def decode(q, k_cache, v_cache, block_tables, ctx_lens, scale, out, n_parts, wor
     t0 = t1 = 0
     if n_parts > 1 and B:
         if workspace is None:
-            ws = torch.empty(B * hq * n_parts * (d + 2), dtype=torch.float32, device=q.device)
+            ws = q.new_empty(B * hq * n_parts * (d + 2), dtype=torch.float32)
             t0 = ws.data_ptr()
             t1 = t0 + 4 * B * hq * n_parts * d
         else:
@@ -395,7 +395,7 @@ def prefill(q, k_cache, v_cache, block_tables, cu_seqlens_q, ctx_lens, scale, ou
     o = ml = few_o = few_ml = 0
     tiles, few = plan.places * hkv * plan.tile, plan.few_places * hkv * FEW_ROWS
     if tiles or few:
-        ws = torch.empty((tiles + few) * (d + 2), dtype=torch.float32, device=q.device)
+        ws = q.new_empty((tiles + few) * (d + 2), dtype=torch.float32)
         o = ws.data_ptr()
         few_o = o + 4 * tiles * d
         ml = few_o + 4 * few * d

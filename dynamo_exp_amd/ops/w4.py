@@ -146,11 +146,11 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, out: torch.Tensor | None = None
     if p.numel() != 256 * chunks or s.numel() * group != 2048 * chunks or (z is not None and z.numel() != s.numel()):
         raise ValueError(f"w4_linear: a weight {(n, k)} in groups of {group} laid out as {tuple(p.shape)} and {tuple(s.shape)}")
     if out is None:
-        out = torch.empty((m, n), dtype=x.dtype, device=x.device)
+        out = x.new_empty((m, n))
     elif out.shape != (m, n) or out.dtype is not x.dtype or out.get_device() != dev or (m and out.stride(1) != 1):
         raise ValueError("w4_linear: bad out tensor")
     waves, rt, splits = _shape(m, n, k)
-    ws = torch.empty(splits * m * n, dtype=torch.float32, device=x.device) if splits > 1 and m else None
+    ws = x.new_empty(splits * m * n, dtype=torch.float32) if splits > 1 and m else None
     _native.kernels().w4_gemm(out.data_ptr(), out.stride(0), xp, rows if m > 1 else 0, p.data_ptr(), s.data_ptr(),
                               0 if z is None else z.data_ptr(), 0 if ws is None else ws.data_ptr(), m, n, k, group, waves, rt, splits,
                               torch._C._cuda_getCurrentRawStream(dev))
