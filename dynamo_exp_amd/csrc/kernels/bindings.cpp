@@ -41,7 +41,7 @@ int dx_prefill_attention(void*, const void*, int64_t, const void*, const void*, 
 int dx_prefill_tile_tokens(int, int, int);
 int dx_block_append(const void*, const void*, const void*, int64_t, void*, int64_t, const void*, int, const float*, int, const float*,
                     const int64_t*, void*, void*, float*, float*, int, int, int, int, int, int, int, int, hipStream_t);
-int dx_block_dequant(const void*, const void*, const float*, const float*, void*, void*, const int*, int, const int*, const int*, int,
+int dx_block_dequant(const void*, const void*, const float*, const float*, void*, void*, const int*, int, const int*, int*, int, int,
                      int, int, int, int, int, int, int, hipStream_t);
 int dx_block_decode(void*, float*, float*, const void*, int64_t, const void*, const void*, const float*, const float*, const int*, int,
                     int, const int*, int, int, int, int, int, int, int, float, int, hipStream_t);
@@ -146,10 +146,10 @@ PYBIND11_MODULE(_C_kernels, m) {
                           (const int64_t*)slots, P(kc), P(vc), (float*)ks, (float*)vs, tokens, hq, hkv, hd, bs, nb, rotate_q, code, S(st)),
           "block_append");
   });
-  m.def("block_dequant", [](u kc, u vc, u ks, u vs, u ko, u vo, u bt, int bts, u ctx, u dst, int n, int cols, int nb, int ndst, int hkv,
-                            int bs, int hd, int code, u st) {
+  m.def("block_dequant", [](u kc, u vc, u ks, u vs, u ko, u vo, u bt, int bts, u ctx, u dst, int dense, int n, int cols, int nb,
+                            int ndst, int hkv, int bs, int hd, int code, u st) {
     check(dx_block_dequant(P(kc), P(vc), (const float*)ks, (const float*)vs, P(ko), P(vo), (const int*)bt, bts, (const int*)ctx,
-                           (const int*)dst, n, cols, nb, ndst, hkv, bs, hd, code, S(st)),
+                           (int*)dst, dense, n, cols, nb, ndst, hkv, bs, hd, code, S(st)),
           "block_dequant");
   });
   m.def("block_decode", [](u out, u to, u tml, u q, int64_t qs, u kc, u vc, u ks, u vs, u bt, int bts, int btc, u ctx, int batch, int hq,

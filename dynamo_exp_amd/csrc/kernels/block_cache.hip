@@ -271,8 +271,8 @@ __global__ void __launch_bounds__(kThreads) block_append_kernel(const AppendArgs
   }
 }
 
-// Blocks as bf16: grid (blocks per sequence, sequences, 2 = K / V times pieces); dst_table[i][j] takes block j of sequence i,
-// blocks past the sequence's length are left.  Bound by HBM; a thread has its loads of a piece on their way at once (105 blocks of 64 x 8 heads,
+// Blocks as bf16: grid (blocks per sequence, sequences, 2 = K / V times pieces); dst_table[i][j] takes block j of sequence i (dense: that is
+// i max_blocks + j, and written here), blocks past the sequence's length are left.  Bound by HBM; a thread has its loads of a piece on their way at once (105 blocks of 64 x 8 heads,
 // K and V: 11.6 us, 3.5 TB/s read and written).
 constexpr int kVecs = 4, kPiece = kThreads * 16 * kVecs;
 
@@ -281,10 +281,12 @@ __global__ void __launch_bounds__(kThreads)
     block_dequant_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc, const float* __restrict__ k_scales,
                          const float* __restrict__ v_scales, bf16_t* __restrict__ ks, bf16_t* __restrict__ vs,
                          const int* __restrict__ block_tables, int bt_stride, const int* __restrict__ ctx_lens,
-                         const int* __restrict__ dst_table, int max_blocks, int num_blocks, int dst_blocks, int n_kv, int bs_shift) {
+                         int* __restrict__ dst_table, int dense, int max_blocks, int num_blocks, int dst_blocks, int n_kv, int bs_shift) {
   const int j = blockIdx.x, i = blockIdx.y, which = blockIdx.z & 1;
+  const int64_t at_table = (int64_t)i * max_blocks + j;
+  if (dense && blockIdx.z == 0 && threadIdx.x == 0) dst_table[at_table] = (int)at_table;
   if (((int64_t)j << bs_shift) >= ctx_lens[i]) return;
-  const int src = block_tables[(int64_t)i * bt_stride + j], dst = dst_table[(int64_t)i * max_blocks + j];
+  const int src = block_tables[(int64_t)i * bt_stride + j], dst = dense ? (int)at_table : dst_table[at_table];
   if ((unsigned)src >= (unsigned)num_blocks || (unsigned)dst >= (unsigned)dst_blocks) return;
   const int elems = n_kv << bs_shift << 7;
   const uint8_t* from = (which ? vc : kc) + (int64_t)src * elems;
@@ -350,7 +352,7 @@ extern "C" int dx_block_append(const void* q, const void* k, const void* v, int6
 }
 
 extern "C" int dx_block_dequant(const void* kc, const void* vc, const float* k_scales, const float* v_scales, void* ks, void* vs,
-                                const int* block_tables, int bt_stride, const int* ctx_lens, const int* dst_table, int n_seqs,
+                                const int* block_tables, int bt_stride, const int* ctx_lens, int* dst_table, int dense, int n_seqs,
                                 int max_blocks, int num_blocks, int dst_blocks, int n_kv, int block_size, int head_dim, int code,
                                 hipStream_t stream) {
   if (head_dim != D || block_size < 16 || (block_size & (block_size - 1))) return -1;
@@ -361,7 +363,7 @@ extern "C" int dx_block_dequant(const void* kc, const void* vc, const float* k_s
   const int shift = __builtin_ctz((unsigned)block_size);
   auto go = [&](auto kernel) {
     kernel<<<grid, kThreads, 0, stream>>>((const uint8_t*)kc, (const uint8_t*)vc, k_scales, v_scales, (bf16_t*)ks, (bf16_t*)vs,
-                                          block_tables, bt_stride, ctx_lens, dst_table, max_blocks, num_blocks, dst_blocks, n_kv, shift);
+                                          block_tables, bt_stride, ctx_lens, dst_table, dense, max_blocks, num_blocks, dst_blocks, n_kv, shift);
   };
   if (code == kE4m3) go(block_dequant_kernel<kE4m3>);
   else go(block_dequant_kernel<kInt8>);

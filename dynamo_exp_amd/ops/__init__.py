@@ -722,10 +722,11 @@ def kv_dequant_scratch(k_cache, v_cache, block_tables, ctx_lens, kv_scales=(1.0,
     :func:`fp8_scratch_plan` (the model runner's packed, capped layout:
     sum of ceil(ctx / block_size) blocks -- never
     nseq x padded max_blocks); without it (direct calls in tests) the
-    dense table i * max_blocks + j.  kv_scales tensors: a block-scaled cache
-    (block8)."""
+    dense table i * max_blocks + j.  K, V and the dense table lie in a
+    workspace of the stream that its next call writes again.  kv_scales
+    tensors: a block-scaled cache (block8), whose results are the caller's."""
     if block8.blocked(kv_scales):
-        return block8.read_back(k_cache, v_cache, kv_scales, block_tables, ctx_lens, scratch, _KV_SCRATCH)
+        return block8.read_back(k_cache, v_cache, kv_scales, block_tables, ctx_lens, scratch)
     nseq, maxb = block_tables.shape
     _, H, BS, D = k_cache.shape
     n = scratch[1] if scratch is not None else nseq * maxb

@@ -144,9 +144,9 @@ def append_rows(qp, kp, vp, T, stride, nq, hkv, qop, q_out_stride, positions, co
         _stream(k_cache))
 
 
-def read_back(k_cache, v_cache, kv_scales, block_tables, ctx_lens, scratch, workspaces):
-    """ops.kv_dequant_scratch of a block-scaled cache.  K and V lie in a workspace of the stream, which its next call writes again; a
-    captured call has one of its own."""
+def read_back(k_cache, v_cache, kv_scales, block_tables, ctx_lens, scratch):
+    """ops.kv_dequant_scratch of a block-scaled cache.  K, V and a table that is made here are the caller's, as any result; blocks that no
+    sequence's length reaches may hold anything."""
     nb, hkv, bs, dev = _check_cache(k_cache, v_cache, kv_scales)
     n, cols = block_tables.shape
     rows, step = block_tables.stride()
@@ -166,29 +166,17 @@ def read_back(k_cache, v_cache, kv_scales, block_tables, ctx_lens, scratch, work
             ks[dst] = ref.block_values(k_cache[src], kv_scales[0][src]).bfloat16()
             vs[dst] = ref.block_values(v_cache[src], kv_scales[1][src]).bfloat16()
         return ks, vs, table
-    stream, captured = _stream(k_cache), torch._C._cuda_isCurrentStreamCapturing()
-    key = (dev, stream, hkv, bs)
-    ws = None if captured else workspaces.get(key)
-    if ws is None or ws[2].numel() < need:
-        cap = max(need, 64)
-        ws = (*(torch.empty((cap, hkv, bs, HEAD_DIM), dtype=torch.bfloat16, device=k_cache.device) for _ in range(2)),
-              torch.arange(cap, dtype=torch.int32, device=k_cache.device))
-        if not captured:
-            workspaces[key] = ws
-    ks, vs, order = ws
-    blocks = order.numel()
-    if blocks != need:
-        blocks = max(need, 1)
-        ks, vs = ks[:blocks], vs[:blocks]
-    if scratch is None:
-        table = order.as_strided((n, cols), (cols, 1))
+    stream, blocks = _stream(k_cache), max(need, 1)
+    if scratch is None:  # (the kernel writes it)
+        table = k_cache.new_empty((n, cols), dtype=torch.int32)
     else:
         table = scratch[0]
         if table.dtype != torch.int32 or table.shape != (n, cols) or not table.is_contiguous() or table.get_device() != dev:
             raise ValueError(f"kv_dequant_scratch: the scratch's table is [{n}, {cols}] int32, contiguous, on {k_cache.device}")
+    ks, vs = (k_cache.new_empty((blocks, hkv, bs, HEAD_DIM), dtype=torch.bfloat16) for _ in range(2))
     _native.kernels().block_dequant(k_cache.data_ptr(), v_cache.data_ptr(), kv_scales[0].data_ptr(), kv_scales[1].data_ptr(), ks.data_ptr(),
-                                    vs.data_ptr(), block_tables.data_ptr(), rows, ctx_lens.data_ptr(), table.data_ptr(), n, cols,
-                                    nb, blocks, hkv, bs, HEAD_DIM, CODES[k_cache.dtype], stream)
+                                    vs.data_ptr(), block_tables.data_ptr(), rows, ctx_lens.data_ptr(), table.data_ptr(),
+                                    int(scratch is None), n, cols, nb, blocks, hkv, bs, HEAD_DIM, CODES[k_cache.dtype], stream)
     return ks, vs, table
 
 

@@ -1002,3 +1002,26 @@ def test_blocks_past_32_bits(codes):
     for a, b in zip(*got):
         assert torch.equal(a.contiguous().view(torch.uint8), b.contiguous().view(torch.uint8))
     near(got[1][1][:700], *attention64(got[1][0][:700, : nq * D].view(700, nq, D), *(x.cpu() for x in (small[0], small[1], *small[2])), order, [700, 0], [700, 333]), 2)
+
+
+@pytest.mark.gpu
+@both
+def test_read_backs_are_their_callers(codes):
+    """Results of eager calls on one stream, held at once: each is memory of its own, its table too."""
+    dtype, bs, nkv = CODES[codes], 16, 2
+    caches = [(*random_cache(30, nkv, bs, dtype, seed), *random_cache(30, nkv, bs, dtype, seed + 1)) for seed in (4, 6, 8)]
+    tables = [torch.randperm(30, generator=torch.Generator().manual_seed(n)).to(torch.int32)[:n].view(1, n) for n in (9, 5, 9)]
+    got = []
+    for (k8, ks, v8, vs), t in zip(caches, tables):
+        dev = on_gpu(k8, v8, t, torch.tensor([bs * t.shape[1] - 3], dtype=torch.int32))
+        got.append(ops.kv_dequant_scratch(*dev, kv_scales=tuple(on_gpu(ks, vs))))
+        if len(got) == 1:
+            first = got[0][2].cpu()
+            got[0][2].fill_(-1)  # (the caller's to change)
+    assert len({x.data_ptr() for r in got for x in r}) == 9
+    for i, ((k8, ks, v8, vs), t, (gk, gv, to)) in enumerate(zip(caches, tables, got)):
+        at = (first if i == 0 else to.cpu())[0].long()
+        b = t[0].long()
+        assert torch.equal(at, torch.arange(len(b)))
+        assert torch.equal(gk.cpu()[at], ref.block_values(k8.view(torch.uint8)[b].view(dtype), ks[b]).bfloat16())
+        assert torch.equal(gv.cpu()[at], ref.block_values(v8.view(torch.uint8)[b].view(dtype), vs[b]).bfloat16())
