@@ -170,7 +170,7 @@ def rope_cache(qkv, positions, cos_sin, slot_mapping, k_cache, v_cache, n_q, n_k
     (block8.append says how).  Then `out` [T, n_q * head_dim] takes the
     rotated Q and is returned; without it Q is rotated in place and qkv
     returned.  K and V stay in qkv as they were."""
-    if block8.blocked(kv_scales):
+    if block8.blocked(kv_scales, k_cache):
         if isinstance(qkv, SplitK):
             qkv = splitk_reduce(qkv)
         q_end, k_end = n_q * head_dim, (n_q + n_kv) * head_dim
@@ -241,7 +241,7 @@ def row_rrms(x: torch.Tensor, eps: float, out: torch.Tensor | None = None) -> to
 
 def kv_write(k, v, slot_mapping, k_cache, v_cache, block_size, kv_scales=(1.0, 1.0)):
     """k, v: [T, Hkv, D] views with equal token stride.  kv_scales tensors: the append to a block-scaled cache (block8.append)."""
-    if block8.blocked(kv_scales):
+    if block8.blocked(kv_scales, k_cache):
         if k_cache.shape[2] != block_size:
             raise ValueError(f"kv_write: blocks of {k_cache.shape[2]}, not {block_size}")
         block8.append(None, k, v, None, None, slot_mapping, k_cache, v_cache, kv_scales)
@@ -635,7 +635,7 @@ def decode_attention(q, k_cache, v_cache, block_tables, ctx_lens, scale, out, n_
         out.copy_(ref.paged_attention(q, k_cache, v_cache, block_tables, cu, ctx_lens, scale, k_cache.shape[2],
                                       kv_scales))
         return out
-    if block8.blocked(kv_scales):
+    if block8.blocked(kv_scales, k_cache):
         return block8.decode(q, k_cache, v_cache, block_tables, ctx_lens, scale, out, n_parts, workspace, kv_scales)
     B, Hq, D = q.shape
     Hkv, BS = k_cache.shape[1], k_cache.shape[2]
@@ -725,7 +725,7 @@ def kv_dequant_scratch(k_cache, v_cache, block_tables, ctx_lens, kv_scales=(1.0,
     dense table i * max_blocks + j.  K, V and the dense table lie in a
     workspace of the stream that its next call writes again.  kv_scales
     tensors: a block-scaled cache (block8), whose results are the caller's."""
-    if block8.blocked(kv_scales):
+    if block8.blocked(kv_scales, k_cache):
         return block8.read_back(k_cache, v_cache, kv_scales, block_tables, ctx_lens, scratch)
     nseq, maxb = block_tables.shape
     _, H, BS, D = k_cache.shape
@@ -763,7 +763,7 @@ def prefill_attention(q, k_cache, v_cache, block_tables, cu_seqlens_q, ctx_lens,
         out.copy_(ref.paged_attention(q, k_cache, v_cache, block_tables, cu_seqlens_q, ctx_lens, scale, k_cache.shape[2],
                                       kv_scales, causal=causal))
         return out
-    if block8.blocked(kv_scales):
+    if block8.blocked(kv_scales, k_cache):
         return block8.prefill(q, k_cache, v_cache, block_tables, cu_seqlens_q, ctx_lens, scale, out, work, kv_scales, causal)
     if _kv_fp8(k_cache):
         k_cache, v_cache, block_tables = kv_dequant_scratch(k_cache, v_cache, block_tables, ctx_lens, kv_scales,

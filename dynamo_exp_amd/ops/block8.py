@@ -1,7 +1,7 @@
 """The paged KV cache in 8 bits with a scale for each block and key/value head: its writer and its readers.
 
 codes [num_blocks, Hkv, BS, 128] int8 or float8_e4m3fn, scales [num_blocks, Hkv] float32, value = code * scale, for K and V each.
-The engine ops of the package take such a cache where their ``kv_scales`` are tensors: ``rope_cache`` and ``kv_write`` append to it,
+The engine ops of the package take such a cache where their ``kv_scales`` are tensors [num_blocks, Hkv]: ``rope_cache`` and ``kv_write`` append to it,
 ``decode_attention`` and ``prefill_attention`` read it, ``kv_dequant_scratch`` hands its blocks back as bf16.  GPU tensors run
 csrc/kernels/block_cache.hip, block_decode.hip and block_prefill.hip, CPU tensors the PyTorch forms of :mod:`.reference`.
 
@@ -25,9 +25,10 @@ BLOCKS = (16, 32, 64, 128)  # tokens of a block
 MAX_GROUP = 16  # query heads per key/value head, decode
 
 
-def blocked(kv_scales) -> bool:
-    """Whether kv_scales are those of a cache with a scale per block and head (tensors)."""
-    return isinstance(kv_scales[0], torch.Tensor)
+def blocked(kv_scales, cache) -> bool:
+    """Whether kv_scales are those of a cache with a scale per block and head: tensors, but not of one element, which is a scale of the
+    whole cache however it is held (unless codes of one block and one head have it in that shape)."""
+    return ref.blocked(kv_scales[0], cache)
 
 
 def alloc(num_blocks: int, n_kv: int, block_size: int, dtype=torch.int8, device="cuda"):

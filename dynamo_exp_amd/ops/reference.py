@@ -146,6 +146,11 @@ def to_codes(y: torch.Tensor, dtype) -> torch.Tensor:
     return c.to(dtype)
 
 
+def blocked(scale, cache: torch.Tensor) -> bool:
+    """Whether `scale` holds one for each block and head of the cache, and not one of a tensor (a number, or a tensor of one element)."""
+    return isinstance(scale, torch.Tensor) and (scale.numel() != 1 or (scale.shape == cache.shape[:2] and cache.dtype in CODE_MAX))
+
+
 def block_values(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     return codes.float() * scales[..., None, None]
 
@@ -223,7 +228,7 @@ def _gather_kv(cache, block_table_row, n_tokens, block_size, scale=1.0):
     nb = (n_tokens + block_size - 1) // block_size
     blocks = block_table_row[:nb].long()
     kv = cache[blocks].float()  # [nb, Hkv, BS, D]
-    kv = kv * (scale[blocks][..., None, None] if isinstance(scale, torch.Tensor) else scale)
+    kv = kv * (scale[blocks][..., None, None] if blocked(scale, cache) else scale)
     kv = kv.permute(0, 2, 1, 3).reshape(nb * block_size, cache.shape[1], cache.shape[3])
     return kv[:n_tokens]
 

@@ -1025,3 +1025,36 @@ def test_read_backs_are_their_callers(codes):
         assert torch.equal(at, torch.arange(len(b)))
         assert torch.equal(gk.cpu()[at], ref.block_values(k8.view(torch.uint8)[b].view(dtype), ks[b]).bfloat16())
         assert torch.equal(gv.cpu()[at], ref.block_values(v8.view(torch.uint8)[b].view(dtype), vs[b]).bfloat16())
+
+
+def one_element_run(device, dtype, ks, vs):
+    """All ops of a cache with one scale a tensor; what they write and give."""
+    bs, nkv, nq, T = 16, 2, 4, 21
+    g = torch.Generator().manual_seed(3)
+    k, v = (torch.zeros((4, nkv, bs, D), dtype=torch.bfloat16, device=device).to(dtype) for _ in range(2))
+    qkv = torch.randn((T, (nq + 2 * nkv) * D), generator=g).bfloat16().to(device)
+    slots, pos = torch.arange(16, 16 + T, device=device), torch.arange(T, device=device)
+    ops.rope_cache(qkv, pos, ref.rope_cos_sin(D, 64, 500000.0).to(device), slots, k, v, nq, nkv, D, bs, kv_scales=(ks, vs))
+    more = torch.randn((2, 5, nkv, D), generator=g).bfloat16().to(device)
+    ops.kv_write(more[0], more[1], torch.arange(48, 53, device=device), k, v, bs, kv_scales=(ks, vs))
+    bt = torch.tensor([[1, 2], [3, 0]], dtype=torch.int32, device=device)
+    ctx, cu = torch.tensor([21, 5], dtype=torch.int32, device=device), torch.tensor([0, 3, 5], dtype=torch.int32, device=device)
+    q = torch.randn((5, nq, D), generator=g).bfloat16().to(device)
+    outs = [torch.empty_like(q[:2]), torch.empty_like(q)]
+    ops.decode_attention(q[:2].contiguous(), k, v, bt, ctx, SCALE, outs[0], 1, kv_scales=(ks, vs))
+    ops.prefill_attention(q, k, v, bt, cu, ctx, SCALE, outs[1], kv_scales=(ks, vs))
+    if device != "cpu" and dtype != torch.bfloat16:
+        outs += [t.clone() for t in ops.kv_dequant_scratch(k, v, bt[:1], ctx[:1] * 0 + 16, kv_scales=(ks, vs))[:2]]
+        outs[2], outs[3] = outs[2][:1], outs[3][:1]
+    return [t.float().cpu() for t in (qkv, k, v, *outs)]
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float8_e4m3fn])
+@pytest.mark.parametrize("shape", [(), (1,), (1, 1)])
+def test_scales_of_one_element_are_a_tensors(device, dtype, shape):
+    """One scale a tensor, held as checkpoints hold it: the numbers' results, bit for bit."""
+    a, b = (0.5, 0.25) if dtype != torch.bfloat16 else (1.0, 1.0)
+    want = one_element_run(device, dtype, a, b)
+    got = one_element_run(device, dtype, torch.full(shape, a), torch.full(shape, b))
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
