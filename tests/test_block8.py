@@ -1056,5 +1056,5 @@ def test_scales_of_one_element_are_a_tensors(device, dtype, shape):
     """One scale a tensor, held as checkpoints hold it: the numbers' results, bit for bit."""
     a, b = (0.5, 0.25) if dtype != torch.bfloat16 else (1.0, 1.0)
     want = one_element_run(device, dtype, a, b)
-    got = one_element_run(device, dtype, torch.full(shape, a), torch.full(shape, b))
+    got = one_element_run(device, dtype, torch.full(shape, a, device=device), torch.full(shape, b, device=device))
     assert all(torch.equal(x, y) for x, y in zip(got, want))
