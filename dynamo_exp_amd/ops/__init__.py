@@ -629,13 +629,14 @@ def decode_attention(q, k_cache, v_cache, block_tables, ctx_lens, scale, out, n_
     kv_scales tensors: a block-scaled cache (block8); n_parts may be None then
     (as many as the table's width makes worth it) and workspace is taken from
     torch's allocator where None."""
+    by_block = block8.blocked(kv_scales, k_cache)
     if not q.is_cuda:
         B = q.shape[0]
         cu = torch.arange(B + 1, dtype=torch.int32)
         out.copy_(ref.paged_attention(q, k_cache, v_cache, block_tables, cu, ctx_lens, scale, k_cache.shape[2],
                                       kv_scales))
         return out
-    if block8.blocked(kv_scales, k_cache):
+    if by_block:
         return block8.decode(q, k_cache, v_cache, block_tables, ctx_lens, scale, out, n_parts, workspace, kv_scales)
     B, Hq, D = q.shape
     Hkv, BS = k_cache.shape[1], k_cache.shape[2]
@@ -759,11 +760,12 @@ def prefill_attention(q, k_cache, v_cache, block_tables, cu_seqlens_q, ctx_lens,
     `work` is a :func:`prefill_plan` then (None: made
     here, from lengths that are waited for).
     """
+    by_block = block8.blocked(kv_scales, k_cache)
     if not q.is_cuda:
         out.copy_(ref.paged_attention(q, k_cache, v_cache, block_tables, cu_seqlens_q, ctx_lens, scale, k_cache.shape[2],
                                       kv_scales, causal=causal))
         return out
-    if block8.blocked(kv_scales, k_cache):
+    if by_block:
         return block8.prefill(q, k_cache, v_cache, block_tables, cu_seqlens_q, ctx_lens, scale, out, work, kv_scales, causal)
     if _kv_fp8(k_cache):
         k_cache, v_cache, block_tables = kv_dequant_scratch(k_cache, v_cache, block_tables, ctx_lens, kv_scales,

@@ -28,7 +28,11 @@ MAX_GROUP = 16  # query heads per key/value head, decode
 def blocked(kv_scales, cache) -> bool:
     """Whether kv_scales are those of a cache with a scale per block and head: tensors, but not of one element, which is a scale of the
     whole cache however it is held (unless codes of one block and one head have it in that shape)."""
-    return ref.blocked(kv_scales[0], cache)
+    if ref.blocked(kv_scales[0], cache):
+        return True
+    if cache.dtype is torch.int8:  # (the kernels for one scale a tensor would read two bytes a value)
+        raise TypeError("KV cache: int8 codes have a scale for each block and head, kv_scales [num_blocks, Hkv] float32 each")
+    return False
 
 
 def alloc(num_blocks: int, n_kv: int, block_size: int, dtype=torch.int8, device="cuda"):
@@ -54,8 +58,8 @@ def _check_cache(k, v, kv_scales):
     dtype = k.dtype
     if dtype not in CODES or v.dtype is not dtype:
         raise TypeError(f"block-scaled cache: int8 or float8_e4m3fn codes, got {k.dtype} and {v.dtype}")
-    if ks.dtype is not torch.float32 or vs.dtype is not torch.float32:
-        raise TypeError("block-scaled cache: scales are float32")
+    if not isinstance(vs, torch.Tensor) or ks.dtype is not torch.float32 or vs.dtype is not torch.float32:
+        raise TypeError("block-scaled cache: scales are float32 tensors")
     shape = k.shape
     nb, hkv, bs, d = shape
     heads = (nb, hkv)

@@ -1058,3 +1058,22 @@ def test_scales_of_one_element_are_a_tensors(device, dtype, shape):
     want = one_element_run(device, dtype, a, b)
     got = one_element_run(device, dtype, torch.full(shape, a, device=device), torch.full(shape, b, device=device))
     assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
+def test_int8_codes_without_block_scales_are_refused():
+    """int8 codes beside numbers, or one scale a tensor: no op has such a form (the bf16 kernels would read past them)."""
+    k8, v8, scales = block8.alloc(4, 2, 16, torch.int8, "cpu")
+    q, rows = torch.zeros((1, 4, D), dtype=torch.bfloat16), torch.zeros((1, 8 * D), dtype=torch.bfloat16)
+    bt, ctx, cu = torch.zeros((1, 1), dtype=torch.int32), torch.ones(1, dtype=torch.int32), torch.tensor([0, 1], dtype=torch.int32)
+    zero = torch.zeros(1, dtype=torch.int64)
+    for s in ((1.0, 1.0), (torch.ones(1), torch.ones(1)), (torch.ones(()), torch.ones(()))):
+        for call in (lambda: ops.rope_cache(rows, zero, ref.rope_cos_sin(D, 4, 500000.0), zero, k8, v8, 4, 2, D, 16, kv_scales=s),
+                     lambda: ops.kv_write(q[:, :2], q[:, :2], zero, k8, v8, 16, kv_scales=s),
+                     lambda: ops.decode_attention(q, k8, v8, bt, ctx, SCALE, q.clone(), 1, kv_scales=s),
+                     lambda: ops.prefill_attention(q, k8, v8, bt, cu, ctx, SCALE, q.clone(), kv_scales=s),
+                     lambda: ops.kv_dequant_scratch(k8, v8, bt, ctx, kv_scales=s)):
+            with pytest.raises(TypeError, match="int8"):
+                call()
+    with pytest.raises(TypeError):
+        ops.kv_write(q[:, :2], q[:, :2], zero, k8, v8, 16, kv_scales=(scales[0], 1.0))
+    assert not bool(bits(k8).any())
