@@ -59,13 +59,12 @@ def _headers(d: Path) -> list[Path]:
     return sorted(d.glob("*.h"))
 
 
-# attn_prefill, block_prefill: scores are finite or -inf by construction, so fmax needs no NaN
+# attn_prefill: scores are finite or -inf by construction, so fmax needs no NaN
 # quieting (IEEE mode off: v_max3 without a v_mul canonicalize per score).
 # decode_attention: one wave a SIMD has registers of both kinds; without the
 # option all matrix products' accumulators are of the second kind, and those
 # of shared rows were copied to and fro in every tile (600 instructions of 1770).
 PER_FILE_FLAGS = {"attn_prefill.hip": ["-fno-honor-nans", "-mno-amdgpu-ieee"],
-                  "block_prefill.hip": ["-fno-honor-nans", "-mno-amdgpu-ieee"],
                   "decode_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 
 

@@ -55,6 +55,9 @@ __device__ __forceinline__ float sum2(uint32_t a, uint32_t b, float c) {
   return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(pair, a), __builtin_bit_cast(pair, b), c, false);
 }
 
+// the larger of two scores, NaN where one is: an instruction for two more (fmaxf would quiet each score first)
+__device__ __forceinline__ float top(float x, float y) { return __builtin_elementwise_maximum(x, y); }
+
 template <int I> using at_t = std::integral_constant<int, I>;
 
 // RW: row waves of 32 rows; KW: waves that share a tile's keys (1: 64 keys, or 4: 128, 32 each); ONE: a wave's keys of a tile lie in one block
@@ -195,13 +198,13 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
     float t_s;
     if constexpr (ONE) {
       float ta = s0[0], tb = s0[1];
-      if constexpr (SUBS == 2) ta = fmaxf(ta, s1[0]), tb = fmaxf(tb, s1[1]);
+      if constexpr (SUBS == 2) ta = top(ta, s1[0]), tb = top(tb, s1[1]);
 #pragma unroll
       for (int i = 2; i < 16; i += 2) {
-        ta = fmaxf(ta, s0[i]), tb = fmaxf(tb, s0[i + 1]);
-        if constexpr (SUBS == 2) ta = fmaxf(ta, s1[i]), tb = fmaxf(tb, s1[i + 1]);
+        ta = top(ta, s0[i]), tb = top(tb, s0[i + 1]);
+        if constexpr (SUBS == 2) ta = top(ta, s1[i]), tb = top(tb, s1[i + 1]);
       }
-      t_s = halves_max(fmaxf(ta, tb)) * sc[0][0];  // (scales are positive)
+      t_s = over_halves(top(ta, tb), top) * sc[0][0];  // (scales are positive)
     } else {
       t_s = -INFINITY;
 #pragma unroll
@@ -209,13 +212,13 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
         float ta = s0[8 * s2], tb = SUBS == 2 ? s1[8 * s2] : -INFINITY;
 #pragma unroll
         for (int i = 8 * s2 + 1; i < 8 * s2 + 8; ++i) {
-          ta = fmaxf(ta, s0[i]);
-          if constexpr (SUBS == 2) tb = fmaxf(tb, s1[i]);
+          ta = top(ta, s0[i]);
+          if constexpr (SUBS == 2) tb = top(tb, s1[i]);
         }
-        t_s = fmaxf(t_s, ta * sc[0][s2]);
-        if constexpr (SUBS == 2) t_s = fmaxf(t_s, tb * sc[1][s2]);
+        t_s = top(t_s, ta * sc[0][s2]);
+        if constexpr (SUBS == 2) t_s = top(t_s, tb * sc[1][s2]);
       }
-      t_s = halves_max(t_s);
+      t_s = over_halves(t_s, top);
     }
     const float m_new = t_s > m_i + kRescale ? t_s : m_i;
     const float alpha = fast_exp2(m_i - m_new);

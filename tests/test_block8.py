@@ -1077,3 +1077,69 @@ def test_int8_codes_without_block_scales_are_refused():
     with pytest.raises(TypeError):
         ops.kv_write(q[:, :2], q[:, :2], zero, k8, v8, 16, kv_scales=(scales[0], 1.0))
     assert not bool(bits(k8).any())
+
+
+NANS = [  # tiles of 64, 128 and 256 rows, their parts, few rows in one part and in parts
+    ([8], [600], {}), ([100, 30], [333, 300], {}), ([300], [700], {"WIDE_TILES": 0, "WIDE_WASTE": 9}), ([16], [4000], {}), ([3, 2], [90, 30], {"BESIDE_KEYS": -1}),
+    ([4], [2500], {})]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("where", ["k", "v", "q"])
+@pytest.mark.parametrize("bs", [16, 64])
+@pytest.mark.parametrize("new,ctx,rules", NANS)
+def test_prefill_nan_of_a_live_token(where, bs, new, ctx, rules, monkeypatch):
+    """A NaN that the append stored: in a key, every row of its head that sees it is NaN and no other; in a value, its column of those rows
+    (and perhaps of its chunk's rows in front of it, whose weights for it are zeros); in a query, its row."""
+    for name, x in rules.items():
+        monkeypatch.setattr(block8, name, x)
+    nq, nkv = 8, 2
+    table, k8, v8, ks, vs = cache_of("e4m3", nkv, bs, ctx, 5)
+    T, cu = sum(new), [sum(new[:i]) for i in range(len(new) + 1)]
+    q = torch.randn((T, nq, D), generator=torch.Generator().manual_seed(3)).bfloat16()
+    want, size = attention64(q, k8, v8, ks, vs, table, new, ctx)
+    j = ctx[0] - new[0] // 2 - 1  # a token of the first sequence's chunk; its second head's
+    sees, head = torch.arange(ctx[0] - new[0], ctx[0]) >= j, slice(nq // 2, nq)
+    nan, either = torch.zeros(q.shape, dtype=torch.bool), torch.zeros(q.shape, dtype=torch.bool)
+    if where == "q":
+        row = new[0] // 2
+        q[row, 3, 7] = NAN
+        nan[row, 3] = True
+    else:
+        codes = bits(k8 if where == "k" else v8)
+        codes[int(table[0, j // bs]), 1, j % bs, 9] = 0x7F
+        if where == "k":
+            nan[:new[0], head] = sees[:, None, None]
+        else:
+            nan[:new[0], head, 9] = sees[:, None]
+            either[:new[0], head, 9] = ~sees[:, None]
+    out = torch.zeros((T, nq, D), dtype=torch.bfloat16, device="cuda")
+    dev = on_gpu(q, k8, v8, table, torch.tensor(cu, dtype=torch.int32), torch.tensor(ctx, dtype=torch.int32))
+    ops.prefill_attention(*dev, SCALE, out, work=ops.prefill_plan(new, ctx, nq, nkv), kv_scales=tuple(on_gpu(ks, vs)))
+    got = out.cpu()
+    assert bool(got[nan].isnan().all())
+    left = ~nan & ~(either & got.isnan())
+    near(got[left], want[left], size[left], 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("where", ["k", "v", "q"])
+@pytest.mark.parametrize("n_parts", [1, 5])
+def test_decode_nan_of_a_live_token(where, n_parts):
+    nq, nkv, bs, ctx = 8, 2, 32, [700, 300]
+    table, k8, v8, ks, vs = cache_of("e4m3", nkv, bs, ctx, 5)
+    q = torch.randn((2, nq, D), generator=torch.Generator().manual_seed(3)).bfloat16()
+    want, size = attention64(q, k8, v8, ks, vs, table, [1, 1], ctx)
+    nan = torch.zeros(q.shape, dtype=torch.bool)
+    if where == "q":
+        q[0, 3, 7] = NAN
+        nan[0, 3] = True
+    else:
+        bits(k8 if where == "k" else v8)[int(table[0, 500 // bs]), 1, 500 % bs, 9] = 0x7F
+        nan[(0, slice(nq // 2, nq)) if where == "k" else (0, slice(nq // 2, nq), 9)] = True
+    out = torch.zeros((2, nq, D), dtype=torch.bfloat16, device="cuda")
+    dev = on_gpu(q, k8, v8, table, torch.tensor(ctx, dtype=torch.int32))
+    ops.decode_attention(*dev, SCALE, out, n_parts, kv_scales=tuple(on_gpu(ks, vs)))
+    got = out.cpu()
+    assert bool(got[nan].isnan().all())
+    near(got[~nan], want[~nan], size[~nan], 1)
