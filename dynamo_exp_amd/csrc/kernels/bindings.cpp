@@ -47,7 +47,7 @@ int dx_block_decode(void*, float*, float*, const void*, int64_t, const void*, co
                     int, const int*, int, int, int, int, int, int, int, float, int, hipStream_t);
 int dx_block_prefill(void*, float*, float*, float*, float*, const void*, int64_t, const void*, const void*, const float*, const float*,
                      const int*, int, int, const int*, const int*, const int*, int, int, const int*, int, int, int, int, int, int, int, int, int, int, int,
-                     int, int, float, int, int, hipStream_t);
+                     int, int, int, float, int, int, hipStream_t);
 int dx_w4_gemm(void*, int64_t, const void*, int64_t, const void*, const void*, const void*, float*, int, int, int, int, int, int, int, hipStream_t);
 int dx_rmsnorm_quant(void*, float*, const void*, void*, const void*, int, int, int64_t, int64_t, float, hipStream_t);
 int dx_decode_advance(void*, void*, void*, void*, void*, const void*, const void*, void*, void*, const int*, int, int,
@@ -161,10 +161,11 @@ PYBIND11_MODULE(_C_kernels, m) {
   m.def("block_prefill", [](u out, u wo, u wml, u fo, u fml, u q, int64_t qs, u kc, u vc, u ks, u vs, u bt, int bts, int btc, u cu, u ctx,
                             u work, int n_work, int n_few, u joins, int n_joins, int n_few_joins, int join_rows, int few_join_rows, int parts,
                             int few_parts, int tile, int few_groups, int hq, int hkv,
-                            int hd, int bs, int nb, float scale, int causal, int code, u st) {
+                            int hd, int bs, int nb, int tokens, float scale, int causal, int code, u st) {
     check(dx_block_prefill(P(out), (float*)wo, (float*)wml, (float*)fo, (float*)fml, P(q), qs, P(kc), P(vc), (const float*)ks, (const float*)vs,
                            (const int*)bt, bts, btc, (const int*)cu, (const int*)ctx, (const int*)work, n_work, n_few, (const int*)joins,
-                           n_joins, n_few_joins, join_rows, few_join_rows, parts, few_parts, tile, few_groups, hq, hkv, hd, bs, nb, scale, causal, code, S(st)),
+                           n_joins, n_few_joins, join_rows, few_join_rows, parts, few_parts, tile, few_groups, hq, hkv, hd, bs, nb, tokens, scale, causal,
+                           code, S(st)),
           "block_prefill");
   });
   m.def("w4_gemm", [](u y, int64_t ldy, u x, int64_t ldx, u w, u s, u z, u ws, int M, int N, int K, int group, int waves, int rt,

@@ -29,7 +29,7 @@ namespace {
 
 constexpr int D = 128, BQ = 32;
 constexpr float kRescale = 8.0f;
-constexpr int kItem = 6;  // seq, first row, first key, end of the keys, place of its sums (or -1), 0
+constexpr int kItem = 6;  // seq, first row, first key, end of the keys, place of its sums (or -1), rows of the sequence
 constexpr int kFewRows = 32;  // rows that block_rows_kernel takes
 constexpr int kJoin = 4;  // seq, first row, first place, places
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -45,7 +45,7 @@ struct PrefillArgs {
   const float *ks, *vs;
   const int *block_tables, *cu, *ctx_lens, *work;
   int64_t q_stride;
-  int bt_stride, bt_cols, n_kv, G, bs_shift, num_blocks, causal, tile;  // tile: rows of a place of sums
+  int bt_stride, bt_cols, n_kv, G, bs_shift, num_blocks, causal, tile, tokens;  // tile: rows of a place of sums
   float scale_log2e;
 };
 
@@ -57,6 +57,25 @@ __device__ __forceinline__ float sum2(uint32_t a, uint32_t b, float c) {
 
 // the larger of two scores, NaN where one is: an instruction for two more (fmaxf would quiet each score first)
 __device__ __forceinline__ float top(float x, float y) { return __builtin_elementwise_maximum(x, y); }
+
+// The new tokens of a sequence, wherever the step says they are: first and count, among those that there are.
+struct Tokens {
+  int first, n;
+};
+__device__ __forceinline__ Tokens tokens_of(const int* cu, int seq, int tokens) {
+  const int first = min(max(__builtin_amdgcn_readfirstlane(cu[seq]), 0), tokens);
+  return {first, min(max(__builtin_amdgcn_readfirstlane(cu[seq + 1]), first), tokens) - first};
+}
+
+// A sequence that has other rows than the plan's: those that no item has are NaN (the items' own are so by their row sum).
+__device__ __forceinline__ void rows_without_item(const PrefillArgs& a, int kvh, const Tokens& at, int from) {
+  const int n = (at.n * a.G - from) * (D / 8);
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const int f = from + i / (D / 8), tok = f / a.G;
+    *reinterpret_cast<raw4*>(a.out + ((int64_t)(at.first + tok) * a.n_kv * a.G + kvh * a.G + f - tok * a.G) * D + 8 * (i % (D / 8))) =
+        raw4{0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u};
+  }
+}
 
 template <int I> using at_t = std::integral_constant<int, I>;
 
@@ -80,7 +99,8 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
   const int* bt = a.block_tables + (int64_t)seq * a.bt_stride;
   // the blocks of the tiles, 64 at a time, a lane each (a table's columns are all that may be read of it)
   int first = key0 >> a.bs_shift, ids = bt[min(first + lane, a.bt_cols - 1)];
-  const int q_start = __builtin_amdgcn_readfirstlane(a.cu[seq]), qlen = __builtin_amdgcn_readfirstlane(a.cu[seq + 1]) - q_start;
+  const Tokens mine = tokens_of(a.cu, seq, a.tokens);
+  const int q_start = mine.first, qlen = mine.n;
   const int ctx = __builtin_amdgcn_readfirstlane((int)min((int64_t)a.ctx_lens[seq], (int64_t)a.bt_cols << a.bs_shift));
   const int last = max(ctx - 1, 0) >> a.bs_shift;
   // ... and what becomes of their scales: a score's factor (never 0: a masked score is -infinity times it), the logarithm of vs in
@@ -101,7 +121,8 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
     ones_l = pack_bf16x2(inv, inv);
   };
   ask();
-  const int pos0 = ctx - qlen, rows = qlen * G;
+  const int pos0 = ctx - qlen, rows = qlen * G, planned = __builtin_amdgcn_readfirstlane(item[5]);
+  if (rows != planned && key0 == 0 && row0 + BQ * RW >= planned) rows_without_item(a, kvh, mine, planned);
   const int w0 = row0 + BQ * rw, f = w0 + r;
   const bool valid = f < rows;
   const int tok = f / G, hq = f - tok * G;
@@ -171,7 +192,7 @@ __global__ void __launch_bounds__(64 * RW * KW, 2) block_prefill_kernel(const Pr
   f32x16 o_acc[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) o_acc[i] = f32x16{};
-  float m_i = -1e30f, l_i = 0.f;  // (l: of this lane's keys)
+  float m_i = -1e30f, l_i = rows == planned ? 0.f : __builtin_nanf("");  // (l: of this lane's keys)
   f32x16 s0, s1;                  // a tile's scores
   u16x8 pf[2][2];                 // its weights
   auto weights = [&](int j0) __attribute__((always_inline)) {
@@ -466,9 +487,12 @@ __global__ void __launch_bounds__(256, 2) block_rows_kernel(const PrefillArgs a)
   const int place = __builtin_amdgcn_readfirstlane(item[4]);
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, r = lane & 15;
-  const int q_start = __builtin_amdgcn_readfirstlane(a.cu[seq]), qlen = __builtin_amdgcn_readfirstlane(a.cu[seq + 1]) - q_start;
+  const Tokens mine = tokens_of(a.cu, seq, a.tokens);
+  const int q_start = mine.first, qlen = mine.n;
   const int ctx = __builtin_amdgcn_readfirstlane((int)min((int64_t)a.ctx_lens[seq], (int64_t)a.bt_cols << a.bs_shift));
-  const int rows = min(qlen * G, 16 * CG), pos0 = ctx - qlen;
+  const int rows = min(qlen * G, 16 * CG), pos0 = ctx - qlen, planned = __builtin_amdgcn_readfirstlane(item[5]);
+  if (qlen * G != planned && key0 == 0) rows_without_item(a, kvh, mine, planned);
+  if (rows == 0) return;
   const int p0 = key0, p1 = min(key1, ctx);
   char* vimg = image + wid * (CH * D * 2);
 
@@ -503,7 +527,7 @@ __global__ void __launch_bounds__(256, 2) block_rows_kernel(const PrefillArgs a)
   float m_i[CG], l_i[CG];
 #pragma unroll
   for (int c = 0; c < CG; ++c) {
-    m_i[c] = -1e30f, l_i[c] = 0.f;
+    m_i[c] = -1e30f, l_i[c] = qlen * G == planned ? 0.f : __builtin_nanf("");
 #pragma unroll
     for (int db = 0; db < 8; ++db) oacc[c][db] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -658,13 +682,14 @@ __global__ void __launch_bounds__(256, 2) block_rows_kernel(const PrefillArgs a)
 // workgroup, by all eight groups of 32 lanes where they are many, each taking every eighth part, two of them on their way at once.
 template <int GROUPS>
 __global__ void __launch_bounds__(256) block_prefill_join_kernel(bf16_t* __restrict__ out, const float* __restrict__ ws_o, const float* __restrict__ ws_ml,
-                                                                 const int* __restrict__ joins, const int* __restrict__ cu, int n_kv, int G, int tile) {
+                                                                 const int* __restrict__ joins, const int* __restrict__ cu, int tokens, int n_kv, int G, int tile) {
   __shared__ __attribute__((aligned(16))) f32x4 other[8][D / 4];
   __shared__ float dens[8];
   const int grp = threadIdx.x >> 5, col = threadIdx.x & 31, in = blockIdx.x * (8 / GROUPS) + grp / GROUPS, kvh = blockIdx.y;
   const int* item = joins + (int64_t)blockIdx.z * kJoin;
   const int seq = item[0], f = item[1] + in, place = item[2], n = item[3];
-  const int q_start = cu[seq], rows = (cu[seq + 1] - q_start) * G;
+  const Tokens mine = tokens_of(cu, seq, tokens);
+  const int q_start = mine.first, rows = mine.n * G;
   if (in >= tile || f >= rows) return;  // (of one row: all of the workgroup)
   const int64_t step = (int64_t)n_kv * tile, row = ((int64_t)place * n_kv + kvh) * tile + in;
   float M = -1e30f;
@@ -699,22 +724,22 @@ __global__ void __launch_bounds__(256) block_prefill_join_kernel(bf16_t* __restr
 void join_parts(const PrefillArgs& a, const int* joins, int n_joins, int rows, int parts, int tile, hipStream_t stream) {
   if (!n_joins) return;
   if (parts <= 4)
-    block_prefill_join_kernel<1><<<dim3((rows + 7) / 8, a.n_kv, n_joins), 256, 0, stream>>>(a.out, a.ws_o, a.ws_ml, joins, a.cu, a.n_kv, a.G, tile);
+    block_prefill_join_kernel<1><<<dim3((rows + 7) / 8, a.n_kv, n_joins), 256, 0, stream>>>(a.out, a.ws_o, a.ws_ml, joins, a.cu, a.tokens, a.n_kv, a.G, tile);
   else
-    block_prefill_join_kernel<8><<<dim3(rows, a.n_kv, n_joins), 256, 0, stream>>>(a.out, a.ws_o, a.ws_ml, joins, a.cu, a.n_kv, a.G, tile);
+    block_prefill_join_kernel<8><<<dim3(rows, a.n_kv, n_joins), 256, 0, stream>>>(a.out, a.ws_o, a.ws_ml, joins, a.cu, a.tokens, a.n_kv, a.G, tile);
 }
 
 }  // namespace
 
-// q [T, Hq, 128] rows q_stride apart (16-byte aligned); out [T, Hq, 128]; work [n_work + n_few][6] (tiles, then sequences of few rows),
+// q [T, Hq, 128] rows q_stride apart (16-byte aligned); out [T, Hq, 128]; tokens: T; work [n_work + n_few][6] (tiles, then sequences of few rows),
 // joins [n_joins + n_few_joins][4] and the places of their sums (ws_o [places, Hkv, tile, 128], ws_ml [..., 2] fp32; few: [places, Hkv,
 // 32, ...]) as the plan says; join_rows, most_parts: rows and parts that a joined item has at most; tile: rows of a work item (64, 128, 256); few_groups: 16s of rows (1, 2).  code: 0 int8, 1 e4m3fn.
 extern "C" int dx_block_prefill(void* out, float* ws_o, float* ws_ml, float* few_o, float* few_ml, const void* q, int64_t q_stride, const void* k,
                                 const void* v, const float* ks, const float* vs, const int* block_tables, int bt_stride, int bt_cols, const int* cu,
                                 const int* ctx_lens, const int* work, int n_work, int n_few, const int* joins, int n_joins, int n_few_joins, int join_rows,
-                                int few_join_rows, int most_parts, int few_most_parts, int tile, int few_groups, int n_q, int n_kv, int head_dim, int block_size, int num_blocks, float scale, int causal, int code,
+                                int few_join_rows, int most_parts, int few_most_parts, int tile, int few_groups, int n_q, int n_kv, int head_dim, int block_size, int num_blocks, int tokens, float scale, int causal, int code,
                                 hipStream_t stream) {
-  if (head_dim != D || block_size < 16 || (block_size & (block_size - 1)) || n_kv < 1 || n_kv > 65535 || n_q % n_kv || q_stride % 8 || bt_cols < 1 ||
+  if (head_dim != D || block_size < 16 || (block_size & (block_size - 1)) || n_kv < 1 || n_kv > 65535 || tokens < 0 || n_q % n_kv || q_stride % 8 || bt_cols < 1 ||
       (tile != 64 && tile != 128 && tile != 256) || (few_groups != 1 && few_groups != 2) || n_work > 65535 || n_few > 65535 || n_joins > 65535 ||
       n_few_joins > 65535 || (n_joins && (join_rows < 1 || join_rows > tile)) || (n_few_joins && (few_join_rows < 1 || few_join_rows > kFewRows)))
     return -1;
@@ -723,7 +748,7 @@ extern "C" int dx_block_prefill(void* out, float* ws_o, float* ws_ml, float* few
   a.k = (const uint8_t*)k, a.v = (const uint8_t*)v, a.ks = ks, a.vs = vs;
   a.block_tables = block_tables, a.cu = cu, a.ctx_lens = ctx_lens, a.work = work;
   a.q_stride = q_stride, a.bt_stride = bt_stride, a.bt_cols = bt_cols;
-  a.n_kv = n_kv, a.G = n_q / n_kv, a.bs_shift = __builtin_ctz((unsigned)block_size), a.num_blocks = num_blocks, a.causal = causal;
+  a.n_kv = n_kv, a.G = n_q / n_kv, a.bs_shift = __builtin_ctz((unsigned)block_size), a.num_blocks = num_blocks, a.causal = causal, a.tokens = tokens;
   a.scale_log2e = scale * 1.4426950408889634f;
   if (n_work) {
     const dim3 grid(n_kv, n_work);

@@ -758,7 +758,8 @@ def prefill_attention(q, k_cache, v_cache, block_tables, cu_seqlens_q, ctx_lens,
     cache goes through :func:`kv_dequant_scratch` first (`scratch`: its packed
     table).  kv_scales tensors: a block-scaled cache (block8), read as it is;
     `work` is a :func:`prefill_plan` then (None: made
-    here, from lengths that are waited for).
+    here, from lengths that are waited for), of the same new tokens in each
+    sequence: rows of a sequence that the plan has others of are NaN.
     """
     by_block = block8.blocked(kv_scales, k_cache)
     if not q.is_cuda:

@@ -299,13 +299,17 @@ FEW_ROWS, FEW_WGS, FEW_KEYS = 32, 256, 256
 # apart and together: 5 and 4 tokens, 14 / 2 heads, alone 14.2, 7.6, behind 1700 and 1200 24.1, 12.8; 32 / 8 heads, four of 300 and eight of 4
 # behind 296 23.0, 15.6, 5000 and four of 6 behind 1794 236, 220.
 BESIDE_KEYS = 65536
+NO_END = 2 ** 31 - 1  # the end of a tile's last part: as far as the context that the call comes with
 
 
 def prefill_plan(q_lens: list[int], ctx_lens: list[int], n_q: int, n_kv: int, device="cuda", causal: bool = True) -> PrefillPlan:
     """Cuts prompt chunks (q_lens new tokens each, the last of ctx_lens tokens) into work items for ``prefill_attention`` over a
     block-scaled cache: tiles of query rows, heaviest first, and where those are too few for the chip, parts of their keys.  Sequences of
     at most 32 rows a key/value head (new tokens times query heads per key/value head) go to a kernel of their own, where they have many keys
-    or are alone."""
+    or are alone.
+
+    A plan holds for these new tokens, sequence by sequence: rows of a sequence that comes with others are NaN.  Contexts may have grown or
+    shrunk since (a captured call's do); the work is only less evenly cut then."""
     if len(q_lens) != len(ctx_lens) or any(q < 0 or c < q for q, c in zip(q_lens, ctx_lens)):
         raise ValueError(f"prefill_plan: {list(q_lens)} new tokens of {list(ctx_lens)}")
     if n_kv < 1 or n_q % n_kv:
@@ -335,20 +339,21 @@ def prefill_plan(q_lens: list[int], ctx_lens: list[int], n_q: int, n_kv: int, de
             tile, items = 256, wide
 
     def cut(items, unit, per, most):
-        """items (units of keys, sequence, first row) -> work and joins: those of over 1.5 `per` units in parts of about `per`."""
+        """items (units of keys, sequence, first row) -> work and joins: those of over 1.5 `per` units in parts of about `per`, the last
+        without an end."""
         work, joins, places, rows, cuts = [], [], 0, 0, 0
         for n, s, r0 in items:
             parts = -(-n // per) if 2 * n > 3 * per else 1
             each = -(-n // parts)
             parts = -(-n // each)
             if parts == 1:
-                work.append((n, [s, r0, 0, unit * n, -1, 0]))
+                work.append((n, [s, r0, 0, NO_END, -1, q_lens[s] * g]))
                 continue
             joins += [s, r0, places, parts]
             rows, cuts = max(rows, min(most, q_lens[s] * g - r0)), max(cuts, parts)
             for p in range(parts):
                 end = min((p + 1) * each, n)
-                work.append((end - p * each, [s, r0, unit * p * each, unit * end, places + p, 0]))
+                work.append((end - p * each, [s, r0, unit * p * each, NO_END if p == parts - 1 else unit * end, places + p, q_lens[s] * g]))
             places += parts
         if len(work) > 65535:
             raise ValueError(f"prefill_plan: {len(work)} work items, at most 65535")
@@ -360,6 +365,11 @@ def prefill_plan(q_lens: list[int], ctx_lens: list[int], n_q: int, n_kv: int, de
     unit = 128 if tile == 64 else 64
     per = max(PREFILL_KEYS // unit, -(-total * n_kv // wgs)) if len(items) * n_kv < wgs else 1 << 30
     work, joins, places, rows, parts = cut(items, unit, per, tile)
+    for s, ql in enumerate(q_lens):  # (a sequence without rows has an item all the same, which looks whether it has come with some)
+        if ql == 0:
+            work += [s, 0, 0, 0, -1, 0]
+    if len(work) > 6 * 65535:
+        raise ValueError(f"prefill_plan: {len(work) // 6} work items, at most 65535")
     items = [(-(-ctx_lens[s] // 128), s, 0) for s in few]
     total = sum(i[0] for i in items)
     few_work, few_joins, few_places, few_rows, few_parts = cut(items, 128, max(FEW_KEYS // 128, -(-total * n_kv // FEW_WGS)), FEW_ROWS)
@@ -399,5 +409,5 @@ def prefill(q, k_cache, v_cache, block_tables, cu_seqlens_q, ctx_lens, scale, ou
                                     table_rows, cols, cu_seqlens_q.data_ptr(), ctx_lens.data_ptr(), work, plan.n_work,
                                     plan.n_few, work + 24 * (plan.n_work + plan.n_few), plan.n_joins, plan.n_few_joins, plan.join_rows, plan.few_join_rows, plan.parts,
                                     plan.few_parts, plan.tile, plan.few_groups,
-                                    hq, hkv, d, bs, nb, float(scale), int(causal), CODES[k_cache.dtype], _stream(q))
+                                    hq, hkv, d, bs, nb, T, float(scale), int(causal), CODES[k_cache.dtype], _stream(q))
     return out

@@ -1143,3 +1143,105 @@ def test_decode_nan_of_a_live_token(where, n_parts):
     got = out.cpu()
     assert bool(got[nan].isnan().all())
     near(got[~nan], want[~nan], size[~nan], 1)
+
+
+def planned_run(codes, nq, nkv, bs, planned, new, ctx, seed=0, causal=True, cu=None, behind=0):
+    """prefill_attention of rows `new` behind contexts `ctx` by a plan of others; (result, wanted, size, plan)."""
+    table, k8, v8, ks, vs = cache_of(codes, nkv, bs, ctx, seed)
+    T = sum(new)
+    q = torch.randn((T, nq, D), generator=torch.Generator().manual_seed(seed + 9)).bfloat16()
+    cu = [sum(new[:i]) for i in range(len(new) + 1)] if cu is None else cu
+    plan = ops.prefill_plan(*planned, nq, nkv, "cuda", causal)
+    dev = on_gpu(q, k8, v8, table, torch.tensor(cu, dtype=torch.int32), torch.tensor(ctx, dtype=torch.int32))
+    out = torch.full((T + behind, nq, D), 7.0, dtype=torch.bfloat16, device="cuda")
+    ops.prefill_attention(*dev, SCALE, out[:T], work=plan, kv_scales=tuple(on_gpu(ks, vs)), causal=causal)
+    want, size = attention64(q, k8, v8, ks, vs, table, new, ctx, causal)
+    return out.cpu(), want, size, plan
+
+
+@pytest.mark.gpu
+@both
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("new,was,ctx,rules", [
+    ([70, 43], [500, 500], [5000, 500], {}), ([70, 43], [3000, 2000], [900, 70], {}), ([16], [4000], [16], {}), ([8], [600], [3000], {}), ([3, 5], [200, 5], [2500, 700], {"BESIDE_KEYS": -1}),
+    ([4], [2500], [77], {}), ([4], [2500], [9000], {}), ([300, 200], [300, 200], [1000, 3000], {"WIDE_TILES": 0, "WIDE_WASTE": 9})])
+def test_plan_of_other_contexts(codes, causal, new, was, ctx, rules, monkeypatch):
+    """A plan serves contexts that have grown, or shrunk, since: it says how the work is cut, not how far a row sees."""
+    for name, x in rules.items():
+        monkeypatch.setattr(block8, name, x)
+    got, want, size, plan = planned_run(codes, 8, 2, 64, (new, was), new, ctx, seed=3, causal=causal)
+    near(got, want, size, 2)
+
+
+@pytest.mark.gpu
+@both
+@pytest.mark.parametrize("planned,new,past,rules", [
+    ([70, 43], [43, 70], [900, 100], {}), ([113, 0, 5], [43, 70, 5], [0, 0, 300], {}), ([3, 30, 9], [30, 3, 9], [2000, 1000, 40], {"BESIDE_KEYS": -1}),
+    ([1, 8], [8, 1], [3000, 3000], {"BESIDE_KEYS": -1}), ([300, 10, 20], [20, 290, 20], [50, 60, 70], {"WIDE_TILES": 0, "WIDE_WASTE": 9}), ([33, 100], [100, 33], [4000, 0], {}),
+    ([21, 200], [32, 189], [700, 0], {}), ([0, 12], [12, 0], [100, 100], {})])
+def test_plan_of_other_rows_gives_nan(codes, planned, new, past, rules, monkeypatch):
+    """As many rows in all, but not sequence by sequence: those of the sequences that differ are NaN, not what the memory held."""
+    for name, x in rules.items():
+        monkeypatch.setattr(block8, name, x)
+    ctx = [n + p for n, p in zip(new, past)]
+    got, want, size, plan = planned_run(codes, 8, 2, 16, (planned, [max(p + q, c) for p, q, c in zip(planned, past, ctx)]), new, ctx, seed=3, behind=2)
+    at = 0
+    for a, n in zip(planned, new):
+        rows = slice(at, at + n)
+        if a == n:
+            near(got[rows], want[rows], size[rows], 2)
+        else:
+            assert bool(got[rows].isnan().all())
+        at += n
+    assert bool((got[at:] == 7).all())
+
+
+@pytest.mark.gpu
+def test_rows_past_the_queries_are_left():
+    """Row numbers past the rows that there are are cut to them: as many as planned then, or NaN; nothing lies behind them."""
+    for planned, cu in (([70, 43], [0, 70, 5000]), ([43, 70], [0, 70, 5000]), ([70, 43], [-9, 70, 2 ** 31 - 1])):
+        got, want, size, _ = planned_run("int8", 8, 2, 16, (planned, [70, 70]), [70, 43], [70, 43], cu=cu, behind=60)
+        near(got[:113], want, size, 2) if planned == [70, 43] else None
+        assert bool(got[:113].isnan().all()) == (planned != [70, 43]) and bool((got[113:] == 7).all())
+    for planned, cu in (([3, 2], [-7, 3, 60]), ([2, 3], [-7, 3, 60])):
+        got, want, size, _ = planned_run("int8", 8, 2, 16, (planned, [3, 3]), [3, 2], [3, 2], cu=cu, behind=60)
+        near(got[:5], want, size, 2) if planned == [3, 2] else None
+        assert bool(got[:5].isnan().all()) == (planned != [3, 2]) and bool((got[5:] == 7).all())
+
+
+@pytest.mark.gpu
+@both
+def test_captured_prompt_whose_contexts_grow(codes):
+    """A captured call replayed behind contexts that the plan did not know."""
+    nq, nkv, bs, new, most = 8, 2, 64, [40, 5], [3000, 1500]
+    table, k8, v8, ks, vs = cache_of(codes, nkv, bs, most, 3)
+    plan = ops.prefill_plan(new, [100, 20], nq, nkv)
+    q = torch.randn((45, nq, D), generator=torch.Generator().manual_seed(8)).bfloat16()
+    dev = on_gpu(q, k8, v8, table, torch.tensor([0, 40, 45], dtype=torch.int32), torch.tensor([100, 20], dtype=torch.int32))
+    scales, out = tuple(on_gpu(ks, vs)), torch.zeros((45, nq, D), dtype=torch.bfloat16, device="cuda")
+    call = lambda: ops.prefill_attention(*dev, SCALE, out, work=plan, kv_scales=scales)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.inference_mode(), torch.cuda.graph(graph):
+        call()
+    for ctx in ([100, 20], [1700, 64], [41, 700], most):
+        dev[5].copy_(torch.tensor(ctx, dtype=torch.int32))
+        out.fill_(NAN)
+        graph.replay()
+        torch.cuda.synchronize()
+        near(out.cpu(), *attention64(q, k8, v8, ks, vs, table, new, ctx), 2)
+
+
+def test_plan_has_no_ends_and_knows_its_rows():
+    """The last part of a tile's keys has no end, every item knows its sequence's rows, and a sequence without rows has one."""
+    for new, ctx in (([70, 0, 3, 500], [3000, 9, 4000, 500]), ([3], [9000]), ([0], [0]), ([40, 2], [900, 3])):
+        p = ops.prefill_plan(new, ctx, 8, 2, "cpu")
+        flat = p.work.tolist()
+        items = [flat[6 * i:6 * i + 6] for i in range(p.n_work + p.n_few)]
+        assert {x[0] for x in items} == set(range(len(new)))
+        assert all(x[5] == 4 * new[x[0]] for x in items)
+        for s in [s for s, n in enumerate(new) if n]:
+            for r0 in {x[1] for x in items if x[0] == s}:
+                ends = sorted(x[3] for x in items if x[:2] == [s, r0])
+                assert ends[-1] == 2 ** 31 - 1 and all(e % 64 == 0 for e in ends[:-1])
