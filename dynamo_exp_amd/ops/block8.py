@@ -173,12 +173,13 @@ def read_back(k_cache, v_cache, kv_scales, block_tables, ctx_lens, scratch):
         return ks, vs, table
     stream, blocks = _stream(k_cache), max(need, 1)
     if scratch is None:  # (the kernel writes it)
-        table = k_cache.new_empty((n, cols), dtype=torch.int32)
+        table = block_tables.new_empty((n, cols))
     else:
         table = scratch[0]
         if table.dtype != torch.int32 or table.shape != (n, cols) or not table.is_contiguous() or table.get_device() != dev:
             raise ValueError(f"kv_dequant_scratch: the scratch's table is [{n}, {cols}] int32, contiguous, on {k_cache.device}")
-    ks, vs = (k_cache.new_empty((blocks, hkv, bs, HEAD_DIM), dtype=torch.bfloat16) for _ in range(2))
+    ks = k_cache.new_empty((blocks, hkv, bs, HEAD_DIM), dtype=torch.bfloat16)
+    vs = torch.empty_like(ks)
     _native.kernels().block_dequant(k_cache.data_ptr(), v_cache.data_ptr(), kv_scales[0].data_ptr(), kv_scales[1].data_ptr(), ks.data_ptr(),
                                     vs.data_ptr(), block_tables.data_ptr(), rows, ctx_lens.data_ptr(), table.data_ptr(),
                                     int(scratch is None), n, cols, nb, blocks, hkv, bs, HEAD_DIM, CODES[k_cache.dtype], stream)
