@@ -246,7 +246,7 @@ extern "C" int dx_block_decode(void* out, float* tmp_out, float* tmp_ml, const v
                                const float* ks, const float* vs, const int* block_tables, int bt_stride, int bt_cols, const int* ctx_lens,
                                int batch, int n_q, int n_kv, int head_dim, int block_size, int num_blocks, int n_parts, float scale, int code,
                                hipStream_t stream) {
-  if (head_dim != D || block_size < 16 || (block_size & (block_size - 1)) || n_parts < 1 || n_kv < 1 || n_q % n_kv || n_q / n_kv > 16 ||
+  if (head_dim != D || block_size < 16 || (block_size & (block_size - 1)) || n_parts < 1 || n_kv < 1 || n_q < 1 || n_q % n_kv || n_q / n_kv > 16 ||
       q_stride % 8 || batch > 65535 || n_kv > 65535 || bt_cols < 1)
     return -1;
   if (batch == 0) return 0;

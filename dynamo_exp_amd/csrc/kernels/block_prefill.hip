@@ -739,7 +739,7 @@ extern "C" int dx_block_prefill(void* out, float* ws_o, float* ws_ml, float* few
                                 const int* ctx_lens, const int* work, int n_work, int n_few, const int* joins, int n_joins, int n_few_joins, int join_rows,
                                 int few_join_rows, int most_parts, int few_most_parts, int tile, int few_groups, int n_q, int n_kv, int head_dim, int block_size, int num_blocks, int tokens, float scale, int causal, int code,
                                 hipStream_t stream) {
-  if (head_dim != D || block_size < 16 || (block_size & (block_size - 1)) || n_kv < 1 || n_kv > 65535 || tokens < 0 || n_q % n_kv || q_stride % 8 || bt_cols < 1 ||
+  if (head_dim != D || block_size < 16 || (block_size & (block_size - 1)) || n_kv < 1 || n_kv > 65535 || tokens < 0 || n_q < 1 || n_q % n_kv || q_stride % 8 || bt_cols < 1 ||
       (tile != 64 && tile != 128 && tile != 256) || (few_groups != 1 && few_groups != 2) || n_work > 65535 || n_few > 65535 || n_joins > 65535 ||
       n_few_joins > 65535 || (n_joins && (join_rows < 1 || join_rows > tile)) || (n_few_joins && (few_join_rows < 1 || few_join_rows > kFewRows)))
     return -1;

@@ -194,7 +194,7 @@ def _check_reader(q, out, k_cache, v_cache, kv_scales, block_tables, ctx_lens, n
         raise ValueError("attention over a block-scaled cache: the cache has no block")
     if q.dtype is not torch.bfloat16 or out.dtype is not torch.bfloat16:
         raise TypeError("attention over a block-scaled cache: q and out are bfloat16")
-    if d != HEAD_DIM or hq % hkv or out.shape != shape or not out.is_contiguous():
+    if d != HEAD_DIM or hkv < 1 or hq < 1 or hq % hkv or out.shape != shape or not out.is_contiguous():
         raise ValueError(f"attention over a block-scaled cache: q {tuple(q.shape)}, out {tuple(out.shape)}, {hkv} key/value heads")
     rows = 0
     if T:
@@ -313,7 +313,7 @@ def prefill_plan(q_lens: list[int], ctx_lens: list[int], n_q: int, n_kv: int, de
     shrunk since (a captured call's do); the work is only less evenly cut then."""
     if len(q_lens) != len(ctx_lens) or any(q < 0 or c < q for q, c in zip(q_lens, ctx_lens)):
         raise ValueError(f"prefill_plan: {list(q_lens)} new tokens of {list(ctx_lens)}")
-    if n_kv < 1 or n_q % n_kv:
+    if n_kv < 1 or n_q < 1 or n_q % n_kv:
         raise ValueError(f"prefill_plan: {n_q} query heads, {n_kv} key/value heads")
     g = n_q // n_kv
     few = [s for s, ql in enumerate(q_lens) if 0 < ql * g <= FEW_ROWS]

@@ -1245,3 +1245,17 @@ def test_plan_has_no_ends_and_knows_its_rows():
             for r0 in {x[1] for x in items if x[0] == s}:
                 ends = sorted(x[3] for x in items if x[:2] == [s, r0])
                 assert ends[-1] == 2 ** 31 - 1 and all(e % 64 == 0 for e in ends[:-1])
+
+
+def test_readers_refuse_no_heads():
+    """No query heads: a group of none has no last head for the lanes behind it."""
+    k8, v8, scales = block8.alloc(4, 2, 16, torch.int8, "cpu")
+    q = torch.zeros((1, 0, D), dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        block8._check_reader(q, q.clone(), k8, v8, scales, torch.zeros((1, 1), dtype=torch.int32), torch.ones(1, dtype=torch.int32), 1)
+    for heads in ((0, 2), (0, 1), (-2, 2)):
+        with pytest.raises(ValueError):
+            ops.prefill_plan([3], [4], *heads, "cpu")
+    none = block8.alloc(4, 0, 16, torch.int8, "cpu")
+    with pytest.raises(ValueError):
+        block8._check_reader(q, q.clone(), none[0], none[1], none[2], torch.zeros((1, 1), dtype=torch.int32), torch.ones(1, dtype=torch.int32), 1)
