@@ -101,8 +101,8 @@ def append(q, k, v, positions, cos_sin, slot_mapping, k_cache, v_cache, kv_scale
     T, hkv, d = k.shape
     if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or (q is not None and q.dtype != torch.bfloat16):
         raise TypeError("append: q, k, v are bfloat16")
-    if v.shape != k.shape or (q is not None and (q.dim() != 3 or q.shape[0] != T or q.shape[2] != d)):
-        raise ValueError(f"append: k {tuple(k.shape)}, v {tuple(v.shape)}")
+    if d != HEAD_DIM or v.shape != k.shape or (q is not None and (q.dim() != 3 or q.shape[0] != T or q.shape[2] != d)):
+        raise ValueError(f"append: k {tuple(k.shape)}, v {tuple(v.shape)}, heads of {HEAD_DIM}")
     stride = k.stride(0)
     for t in (q, k, v):
         if t is not None and T > 0 and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != d) or (T > 1 and t.stride(0) != stride)):

@@ -1259,3 +1259,34 @@ def test_readers_refuse_no_heads():
     none = block8.alloc(4, 0, 16, torch.int8, "cpu")
     with pytest.raises(ValueError):
         block8._check_reader(q, q.clone(), none[0], none[1], none[2], torch.zeros((1, 1), dtype=torch.int32), torch.ones(1, dtype=torch.int32), 1)
+
+
+def test_append_refuses_heads_of_other_widths(monkeypatch):
+    """K and V of 64 columns a head: the kernel reads 128 of each.  (No GPU here: what the op would start stands still.)"""
+    k8, v8, scales = block8.alloc(4, 2, 16, torch.int8, "cpu")
+    started = []
+    monkeypatch.setattr(block8, "append_rows", lambda *a: started.append(a))
+    zero = torch.zeros(3, dtype=torch.int64)
+
+    class Rows(torch.Tensor):  # (CPU memory that says it is the GPU's)
+        is_cuda = True
+
+    rows = lambda d: torch.zeros((3, 8, d), dtype=torch.bfloat16).as_subclass(Rows).split((4, 2, 2), 1)  # noqa: E731
+    block8.append(*rows(D), None, None, zero, k8, v8, scales)
+    assert len(started) == 1
+    for d in (64, 32, 256):
+        q, k, v = rows(d)
+        with pytest.raises(ValueError, match="heads of 128"):
+            block8.append(q, k, v, None, None, zero, k8, v8, scales)
+        with pytest.raises(ValueError, match="heads of 128"):
+            block8.append(None, k, v, None, None, zero, k8, v8, scales)
+    assert len(started) == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 256])
+def test_append_refuses_heads_of_other_widths_gpu(d):
+    k8, v8, scales = block8.alloc(4, 2, 16, torch.int8)
+    k = torch.zeros((3, 2, d), dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="heads of 128"):
+        ops.kv_write(k, k, torch.arange(3, device="cuda"), k8, v8, 16, kv_scales=scales)
