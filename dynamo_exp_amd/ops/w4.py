@@ -122,6 +122,26 @@ def _shape(m: int, n: int, k: int) -> tuple[int, int, int]:
     return waves, rt, splits
 
 
+def _check_weight(weight: W4Weight) -> int:
+    """What the kernel takes for granted of a weight's tensors; their device's number.  (Each thing is asked once: a product of one row
+    takes these checks nearly as long as its kernel.)"""
+    p, s, z, n, k, group = weight
+    if p.dtype is not torch.int32 or s.dtype is not torch.bfloat16 or (z is not None and z.dtype is not torch.uint8):
+        raise TypeError(f"w4_linear: a weight of {p.dtype}, scales of {s.dtype}{'' if z is None else f', zeros of {z.dtype}'}, not as w4_pack lays it out")
+    if group not in GROUPS or n < 1 or k < group or k % group:
+        raise ValueError(f"w4_linear: a weight {(n, k)} in groups of {group}")
+    chunks = -(-n // 16) * -(-k // 128)
+    if (p.numel() != 256 * chunks or s.numel() * group != 2048 * chunks or not p.is_contiguous() or not s.is_contiguous()
+            or p.data_ptr() % 16 or s.data_ptr() % 8):
+        raise ValueError(f"w4_linear: a weight {(n, k)} in groups of {group} laid out as {tuple(p.shape)} and {tuple(s.shape)}, contiguous and 16-byte aligned")
+    dev = p.get_device()
+    if s.get_device() != dev:
+        raise ValueError(f"w4_linear: a weight on {p.device}, its scales on {s.device}")
+    if z is not None and (z.numel() != s.numel() or not z.is_contiguous() or z.data_ptr() % 4 or z.get_device() != dev):
+        raise ValueError(f"w4_linear: zeros {tuple(z.shape)} on {z.device} beside scales {tuple(s.shape)} on {s.device}")
+    return dev
+
+
 def w4_linear(x: torch.Tensor, weight: W4Weight, out: torch.Tensor | None = None) -> torch.Tensor:
     """y [m, n] = x [m, k] . w^T for up to 256 rows of bf16, sums in fp32."""
     shape, (p, s, z, n, k, group) = x.shape, weight
@@ -140,11 +160,8 @@ def w4_linear(x: torch.Tensor, weight: W4Weight, out: torch.Tensor | None = None
     if m and (cols != 1 or (m > 1 and rows % 8) or xp % 16):
         raise ValueError("w4_linear: rows of x have unit stride and are 16-byte aligned")
     dev = torch._C._cuda_getDevice()
-    if number != dev or p.get_device() != dev or s.get_device() != dev or (z is not None and z.get_device() != dev):
+    if number != dev or _check_weight(weight) != dev:
         raise ValueError(f"w4_linear: x on {x.device}, the weight on {p.device}, current device cuda:{dev}")
-    chunks = -(-n // 16) * -(-k // 128)
-    if p.numel() != 256 * chunks or s.numel() * group != 2048 * chunks or (z is not None and z.numel() != s.numel()):
-        raise ValueError(f"w4_linear: a weight {(n, k)} in groups of {group} laid out as {tuple(p.shape)} and {tuple(s.shape)}")
     if out is None:
         out = x.new_empty((m, n))
     elif out.shape != (m, n) or out.dtype is not x.dtype or out.get_device() != dev or (m and out.stride(1) != 1):

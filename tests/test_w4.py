@@ -217,3 +217,30 @@ def test_bands_of_rows(m, n, k):
     codes, scales, z, w = make(n, k, 64, True, seed=n)
     x = torch.randn((m, k), generator=torch.Generator().manual_seed(k)).bfloat16()
     near(ops.w4_linear(x.cuda(), ops.w4_pack(codes.cuda(), scales.cuda(), z.cuda(), 64)).cpu(), x, w, scales, 64)
+
+
+def test_weights_that_the_kernel_cannot_read_are_refused():
+    """Types, strides and alignment of a weight's tensors: what the kernel takes for granted of the memory behind them."""
+    from dynamo_exp_amd.ops import w4
+    codes, scales, z, _ = make(48, 256, 32, True)
+    w = ops.w4_pack(codes, scales, z, 32)
+    w4._check_weight(w)
+    one = torch.zeros(w.packed.numel() + 1, dtype=torch.int32)
+    for bad, kind in ((w._replace(packed=w.packed.to(torch.int64)), TypeError), (w._replace(packed=w.packed.to(torch.uint8)), TypeError), (w._replace(scales=w.scales.float()), TypeError),
+                      (w._replace(scales=w.scales.view(torch.float16)), TypeError), (w._replace(scales=w.scales.to(torch.float8_e4m3fn)), TypeError), (w._replace(zeros=w.zeros.int()), TypeError),
+                      (w._replace(packed=w.packed[:1].expand(3, -1, -1, -1)), ValueError), (w._replace(scales=w.scales[:1].expand(3, -1, -1, -1)), ValueError),
+                      (w._replace(zeros=w.zeros[:1].expand(3, -1, -1, -1)), ValueError), (w._replace(packed=w.packed.transpose(0, 1)), ValueError),
+                      (w._replace(packed=one[1:].view(w.packed.shape)), ValueError), (w._replace(n=64), ValueError), (w._replace(n=0), ValueError), (w._replace(k=2 ** 20), ValueError),
+                      (w._replace(group=64), ValueError), (w._replace(group=0), ValueError), (w._replace(k=250), ValueError), (w._replace(zeros=w.zeros[:, :1]), ValueError)):
+        with pytest.raises(kind):
+            w4._check_weight(bad)
+
+
+@pytest.mark.gpu
+def test_weights_that_the_kernel_cannot_read_are_refused_gpu():
+    codes, scales, z, _ = make(48, 256, 32, True)
+    w = ops.w4_pack(codes.cuda(), scales.cuda(), z.cuda(), 32)
+    x = torch.zeros((2, 256), dtype=torch.bfloat16, device="cuda")
+    for bad, kind in ((w._replace(scales=w.scales.to(torch.float8_e4m3fn)), TypeError), (w._replace(packed=w.packed[:1].expand(3, -1, -1, -1)), ValueError), (w._replace(zeros=w.zeros.int()), TypeError)):
+        with pytest.raises(kind):
+            ops.w4_linear(x, bad)
