@@ -5,8 +5,9 @@
 // the x rows are the rows of A.  A code becomes bf16 by being put in the mantissa of 128 (0x4300 | c = 128 + c, exact), two by
 // one and-or; what that adds is taken off group by group, with the sum of the group's x from a product with ones:
 //   sum x (c - z) = sum x (128 + c) - (128 + z) sum x
-// The two sums are exact to fp32's 2^-24 of their size, 136 / 4.6 times the wanted one's at random codes: 2^-19, against the
-// 2^-8 of y's own rounding.
+// The two sums are off by 2^-24 of their size an addition.  Beside the wanted sum that size is 136 / 4.6 where x has mean zero and codes are
+// random (2^-19, against the 2^-8 of y's own rounding), and grows with the root of the group where x has a common part: 136 sqrt(128) / 4.6,
+// 330 times (2^-15).  Where x is infinite, or so large that 143 x is, they leave no number, and the result is summed column by column.
 //
 // Weights are laid out once (ops.w4_pack): [N / 16][K / 128][lane][4] words, lane = 16 (k quarter) + row, word s the lane's eight
 // columns 32 s + 8 (lane / 16) .. of the 128, column 2 i in nibble i, 2 i + 1 in nibble 4 + i: one 1 KB load of a wave is 16 rows x
@@ -43,6 +44,33 @@ __device__ __forceinline__ bf16x8_t codes_bf16(uint32_t w, uint32_t base) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) o[i] = ((w >> (4 * i)) & 0x000F000Fu) | base;
   return __builtin_bit_cast(bf16x8_t, o);
+}
+
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
+
+// A result by its definition, column by column, over the chunks of 128 columns that a workgroup has (`per` of them side by side): where x is
+// infinite, or 143 x is, (128 + c) x and (128 + z) x leave no number between them.  Only such results come here.
+template <int GS, bool ZERO> __device__ __forceinline__ float sum_by_column(const W4Args& a, int row, int tok, int per) {
+  constexpr int GC = 4 / GS;
+  const bf16_t* x = a.x + (int64_t)tok * a.ldx;
+  float sum = 0.f;
+  for (int c0 = per * blockIdx.z; c0 < a.chunks; c0 += per * gridDim.z)
+    for (int c = c0; c < min(c0 + per, a.chunks); ++c) {
+      const int64_t at = (int64_t)(row >> 4) * a.chunks + c;
+      for (int s = 0; s < 4 && 128 * c + 32 * s < a.K; ++s) {
+        const int64_t group = (at * 16 + (row & 15)) * GC + s / GS;
+        const float sc = bf16lo((uint32_t)a.s[group]), zc = ZERO ? (float)a.z[group] - 128.f : 8.f;
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t w = reinterpret_cast<const uint32_t*>(a.w + at * 64 + 16 * q + (row & 15))[s];
+          for (int e = 0; e < 8; ++e) {
+            const float code = (float)((w >> (4 * (e / 2 + 4 * (e & 1)))) & 15u);
+            sum += bf16lo((uint32_t)*reinterpret_cast<const uint16_t*>(x + 128 * c + 32 * s + 8 * q + e)) * ((code - zc) * sc);
+          }
+        }
+        if (sum != sum) return sum;  // (and so it stays)
+      }
+    }
+  return sum;
 }
 
 // RT: 16-row tiles of weights a wave; T: tiles of 4 E rows of x (E of every four rows of A); GS: k steps of 32 in a group; DW: chunks on
@@ -182,6 +210,7 @@ __global__ void __launch_bounds__(512) w4_kernel(const W4Args a) {
     if (row >= a.N || tok >= a.M) continue;
     float sum = 0.f;
     for (int w = 0; w < waves; ++w) sum += red[w * (RT * T * E * 64) + o];
+    if (!finite(sum)) sum = sum_by_column<GS, ZERO>(a, row, tok, waves);
     if (gridDim.z == 1) a.y[(int64_t)tok * a.ldy + row] = f32_to_bf16(sum);
     else a.ws[((int64_t)blockIdx.z * a.M + tok) * a.N + row] = sum;
   }
@@ -317,6 +346,7 @@ __global__ void __launch_bounds__(512) w4_wide_kernel(const W4Args a) {
   }
   __syncthreads();
   if (half) return;
+  bool odd = false;
 #pragma unroll
   for (int i = 0; i < RT; ++i)
 #pragma unroll
@@ -329,9 +359,22 @@ __global__ void __launch_bounds__(512) w4_wide_kernel(const W4Args a) {
         if (row < a.N && tok < a.M) {
           if (gridDim.z == 1) a.y[(int64_t)tok * a.ldy + row] = f32_to_bf16(acc[i][t][e]);
           else a.ws[((int64_t)blockIdx.z * a.M + tok) * a.N + row] = acc[i][t][e];
+          odd |= !finite(acc[i][t][e]);
         }
       }
     }
+  if (!odd) return;
+#pragma unroll 1
+  for (int o = 0; o < RT * T * 4; ++o) {  // (a lane's results once more: the sums are in registers, which have no number at run time)
+    const int row = 16 * (nt0 + o / (T * 4)) + r, tok = m0 + 16 * (o / 4 % T) + 4 * q + o % 4;
+    if (row >= a.N || tok >= a.M) continue;
+    bf16_t* y = a.y + (int64_t)tok * a.ldy + row;
+    float* part = a.ws + ((int64_t)blockIdx.z * a.M + tok) * a.N + row;
+    if (finite(gridDim.z == 1 ? bf16lo((uint32_t)*reinterpret_cast<const uint16_t*>(y)) : *part)) continue;
+    const float sum = sum_by_column<GS, ZERO>(a, row, tok, 2);
+    if (gridDim.z == 1) *y = f32_to_bf16(sum);
+    else *part = sum;
+  }
 }
 
 // y = the splits' sums, in their order

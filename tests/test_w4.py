@@ -244,3 +244,32 @@ def test_weights_that_the_kernel_cannot_read_are_refused_gpu():
     for bad, kind in ((w._replace(scales=w.scales.to(torch.float8_e4m3fn)), TypeError), (w._replace(packed=w.packed[:1].expand(3, -1, -1, -1)), ValueError), (w._replace(zeros=w.zeros.int()), TypeError)):
         with pytest.raises(kind):
             ops.w4_linear(x, bad)
+
+
+def infinite(got, want, x, w):
+    """Infinities and NaN where the definition has them; the rest within sums in fp32 of its products, one by one."""
+    size = x.double().nan_to_num(0, 0, 0).abs() @ w.abs().T
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isposinf(), want.isposinf()) and torch.equal(got.isneginf(), want.isneginf())
+    ok = want.isfinite()
+    err = (got.double() - want).abs()[ok]
+    assert bool((err <= 2 ** -8 * want.abs()[ok] * 1.01 + (w.shape[1] + 4) * 2 ** -24 * size[ok]).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("m,n,k,group", [(1, 33, 256, 32), (4, 48, 1152, 128), (7, 40, 640, 64), (16, 100, 896, 128), (16, 64, 8192, 64), (40, 48, 1152, 32), (100, 17, 16000, 128), (64, 8192, 8448, 64)])
+def test_infinite_and_huge_rows(m, n, k, group, zeros):
+    """x that is infinite, or so large that 128 and 143 times it is: the definition's results, as on the CPU."""
+    codes, scales, z, w = make(n, k, group, zeros, seed=m)
+    scales = (scales.float() * 2.0 ** -6).bfloat16()
+    w = w * 2.0 ** -6
+    x = torch.randn((m, k), generator=torch.Generator().manual_seed(k)).bfloat16()
+    x[0, 5] = float("inf")
+    if m > 1:
+        x[1, 9], x[1, k - 1] = float("inf"), float("-inf")
+        x[2] *= 2.0 ** 119
+        x[3, k // 2] = -3e38
+    weight = ops.w4_pack(codes.cuda(), scales.cuda(), None if z is None else z.cuda(), group)
+    want = x.double() @ w.T
+    assert bool((want[0].isinf() | want[0].isnan()).all()) and (m == 1 or bool(want[2:4].isfinite().all()))
+    infinite(ops.w4_linear(x.cuda(), weight).cpu(), want, x, w)
