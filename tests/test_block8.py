@@ -1290,3 +1290,168 @@ def test_append_refuses_heads_of_other_widths_gpu(d):
     k = torch.zeros((3, 2, d), dtype=torch.bfloat16, device="cuda")
     with pytest.raises(ValueError, match="heads of 128"):
         ops.kv_write(k, k, torch.arange(3, device="cuda"), k8, v8, 16, kv_scales=scales)
+
+
+# ---------------------------------------------------------------- every key in its place
+def unit_cache(codes, nkv, bs, ctx, seed):
+    """Keys of zeros, so that every key that a row sees has the same weight (1 before the division: exact), and values that say where they
+    lie: a token of 16-key unit u has 1 + u // 128 in column u % 128, under scales of 1."""
+    table, k8, v8, ks, vs = cache_of(codes, nkv, bs, ctx, seed)
+    bits(k8)[:] = 0
+    v = torch.zeros(v8.shape)
+    for i, x in enumerate(ctx):
+        j = torch.arange(x)
+        v[table[i].long()[j // bs], :, j % bs, j // 16 % 128] = (1 + j // 16 // 128).float()[:, None]
+    used = torch.cat([table[i, : -(-x // bs)] for i, x in enumerate(ctx)]).long()
+    ks[used], vs[used] = 0.5, 1.0
+    return table, k8, v.to(CODES[codes]), ks, vs
+
+
+def in_place(got, want):
+    """Sums of small whole numbers over their count: fp32 holds the sum, the quotient has 2^-23, the result its rounding to bf16.  (Needles:
+    one value, and e^-80 = 2^-115 of values below 2^11.)"""
+    return bool(((got.double() - want).abs() <= 2 ** -8 * want.abs() * (1 + 2 ** -10) + 2 ** -100).all())
+
+
+def needle_cache(codes, nkv, bs, ctx, seed):
+    """Keys of +-1: a query of 16 times one of them scores 16 * 128 * SCALE = 181 there and N(0, 16) elsewhere, so that its weight is 1 and
+    the others' e^-80 together, and the result that key's value."""
+    table, k8, v8, ks, vs = cache_of(codes, nkv, bs, ctx, seed)
+    g = torch.Generator().manual_seed(seed + 3)
+    signs = (torch.randint(0, 2, k8.shape, generator=g) * 2 - 1).float().to(CODES[codes])
+    for i, x in enumerate(ctx):
+        j = torch.arange(x)
+        b = table[i].long()[j // bs]
+        bits(k8)[b, :, j % bs] = bits(signs)[b, :, j % bs]
+        ks[b] = 1.0
+    return table, k8, v8, ks, vs
+
+
+def needles(table, k8, v8, vs, i, bs, targets, nq):
+    """(queries, wanted) [rows, nq, D] that look for keys targets [rows, nq] of sequence i."""
+    nkv = k8.shape[1]
+    kv = (torch.arange(nq) * nkv // nq).expand_as(targets)
+    b = table[i].long()[targets // bs]
+    return (16 * k8.float()[b, kv, targets % bs]).bfloat16(), (v8.float()[b, kv, targets % bs] * vs[b, kv][..., None]).double()
+
+
+def spread(rows, nq, nkv, seen):
+    """Targets [rows, nq]: each key/value head's are spread evenly over the keys that their rows see, the last among them."""
+    g = nq // nkv
+    n = torch.arange(rows * g).view(rows, g).repeat(1, nkv)
+    return (n * (seen[:, None] - 1) // max(rows * g - 1, 1)).long()
+
+
+@pytest.mark.gpu
+@both
+@pytest.mark.parametrize("bs", [16, 64])
+@pytest.mark.parametrize("B,ctx,n_parts", [(40, 9001, 1), (40, 9001, 17), (40, 9001, 65), (40, 9001, None), (20, 700, 1), (20, 700, 6), (300, 700, 1), (20, 2100, 4), (3, 50, 2)])
+def test_decode_every_key_in_its_place(codes, bs, B, ctx, n_parts):
+    """Sequences that share a context: eight waves and four, parts, refills of the 64 blocks at hand, the join."""
+    nq, nkv = 16, 1
+    for kind in ("units", "needles"):
+        table, k8, v8, ks, vs = (unit_cache if kind == "units" else needle_cache)(codes, nkv, bs, [ctx], 7)
+        if kind == "units":
+            q = torch.randn((B, nq, D), generator=torch.Generator().manual_seed(1)).bfloat16()
+            want = attention64(q[:1], k8, v8, ks, vs, table, [1], [ctx])[0].expand(B, nq, D)
+        else:
+            targets = spread(B, nq, nkv, torch.full((B,), ctx))
+            assert B < 40 or ctx < 9000 or len(set((targets // 16).flatten().tolist())) == -(-ctx // 16)
+            q, want = needles(table, k8, v8, vs, 0, bs, targets, nq)
+        dev = on_gpu(q, k8, v8, table.expand(B, -1), torch.full((B,), ctx, dtype=torch.int32))
+        out = torch.empty((B, nq, D), dtype=torch.bfloat16, device="cuda")
+        ops.decode_attention(*dev, SCALE, out, n_parts, kv_scales=tuple(on_gpu(ks, vs)))
+        assert in_place(out.cpu(), want)
+
+
+@pytest.mark.gpu
+@both
+@pytest.mark.parametrize("bs", [16, 64])
+@pytest.mark.parametrize("new,ctx,nq,nkv,rules", [
+    ([70, 40], [9000, 5000], 8, 2, {}), ([16], [4000], 32, 8, {}), ([33], [6000], 4, 1, {}), ([21], [700], 8, 2, {}), ([70, 3], [3000, 900], 8, 2, {}),
+    ([8, 5], [9000, 3000], 4, 1, {"BESIDE_KEYS": -1}), ([2], [9000], 8, 2, {"BESIDE_KEYS": -1}), ([4, 1], [200, 300], 4, 1, {"FEW_KEYS": 10 ** 8}),
+    ([257, 130], [5000, 200], 8, 2, {"WIDE_TILES": 0, "WIDE_WASTE": 9}), ([300], [9000], 8, 2, {"WIDE_TILES": 0, "WIDE_WASTE": 9, "PREFILL_KEYS": 10 ** 8}),
+    ([130], [7000], 8, 2, {"PREFILL_KEYS": 10 ** 8}), ([12], [7000], 4, 1, {"PREFILL_KEYS": 10 ** 8})])
+def test_prompt_every_key_in_its_place(codes, bs, new, ctx, nq, nkv, rules, monkeypatch):
+    """Tiles of 64, 128 and 256 rows and few rows, whole and in parts, few parts and many to join, refills of the 64 blocks at hand."""
+    for name, x in rules.items():
+        monkeypatch.setattr(block8, name, x)
+    T, cu = sum(new), [sum(new[:i]) for i in range(len(new) + 1)]
+    plan = ops.prefill_plan(new, ctx, nq, nkv)
+    for kind in ("units", "needles"):
+        table, k8, v8, ks, vs = (unit_cache if kind == "units" else needle_cache)(codes, nkv, bs, ctx, 7)
+        if kind == "units":
+            q = torch.randn((T, nq, D), generator=torch.Generator().manual_seed(1)).bfloat16()
+            want = attention64(q, k8, v8, ks, vs, table, new, ctx)[0]
+        else:
+            both_ = [needles(table, k8, v8, vs, i, bs, spread(n, nq, nkv, torch.arange(x - n, x) + 1), nq) for i, (n, x) in enumerate(zip(new, ctx))]
+            q, want = (torch.cat(t) for t in zip(*both_))
+        dev = on_gpu(q, k8, v8, table, torch.tensor(cu, dtype=torch.int32), torch.tensor(ctx, dtype=torch.int32))
+        out = torch.empty((T, nq, D), dtype=torch.bfloat16, device="cuda")
+        ops.prefill_attention(*dev, SCALE, out, work=plan, kv_scales=tuple(on_gpu(ks, vs)))
+        assert in_place(out.cpu(), want)
+
+
+def test_a_lost_or_doubled_chunk_is_seen():
+    """The check above against an oracle without, and with twice, each 32 keys of 9001 (planted here, on the CPU)."""
+    n = 9001
+    u = torch.arange(n) // 16
+    v = torch.zeros((n, D), dtype=torch.float64)
+    v[torch.arange(n), u % 128] = (1 + u // 128).double()
+    want = v.mean(0)
+    for at in range(0, n, 32):
+        part = v[at:at + 32]
+        assert not in_place(((v.sum(0) - part.sum(0)) / (n - len(part))).bfloat16(), want)
+        assert not in_place(((v.sum(0) + part.sum(0)) / (n + len(part))).bfloat16(), want)
+        assert not in_place(((v.sum(0) - part.sum(0) + v[(at + 64) % 8960:][:len(part)].sum(0)) / n).bfloat16(), want)
+
+
+def closer(got, q, k8, v8, ks, vs, table, new, ctx, of_rounded):
+    """A weight p is off by at most 2^-8 of itself (rounded to bf16), and 2^-11 by its score's products in fp32; taken as independent, their
+    sum passes 8 times the root of the sum of the squares once in 10^13 (2 exp(-8^2 / 2)); the prompt kernels' row sum has as many.  The
+    result's own rounding, and weights too small to be numbers, as above."""
+    bs, nkv, nq = k8.shape[2], k8.shape[1], q.shape[1]
+    at = 0
+    for i, (n, x) in enumerate(zip(new, ctx)):
+        b = table[i, : -(-x // bs)].long()
+        k, v = ((c.view(torch.uint8)[b].view(c.dtype).double() * s.double()[b][..., None, None]).transpose(1, 2).reshape(-1, nkv, D)[:x] for c, s in ((k8, ks), (v8, vs)))
+        hide = torch.arange(x) > torch.arange(x - n, x)[:, None]
+        for h in range(nq):
+            kv = h * nkv // nq
+            p = torch.softmax((q[at:at + n, h].double() @ k[:, kv].T * SCALE).masked_fill(hide, -INF), -1)
+            want = p @ v[:, kv]
+            root = ((p * p) @ (v[:, kv] * v[:, kv])).sqrt() + (want.abs() * (p * p).sum(-1, keepdim=True).sqrt() if of_rounded else 0)
+            tol = 8 * (2 ** -8 + 2 ** -11) * root + 2 ** -8 * want.abs() * 1.01 + 2 ** -101
+            err = (got[at:at + n, h].double() - want).abs()
+            assert bool((err <= tol).all()), (i, h, float((err / tol).max()))
+        at += n
+
+
+@pytest.mark.gpu
+@both
+@pytest.mark.parametrize("ctx,n_parts", [([9001, 5, 4096], 1), ([9001, 5, 4096], 17), ([700, 333], None)])
+def test_decode_closer(codes, ctx, n_parts):
+    nq, nkv, bs = 4, 1, 16
+    table, k8, v8, ks, vs = cache_of(codes, nkv, bs, ctx, 3)
+    q = torch.randn((len(ctx), nq, D), generator=torch.Generator().manual_seed(12)).bfloat16()
+    out = torch.empty((len(ctx), nq, D), dtype=torch.bfloat16, device="cuda")
+    dev = on_gpu(q, k8, v8, table, torch.tensor(ctx, dtype=torch.int32))
+    ops.decode_attention(*dev, SCALE, out, n_parts, kv_scales=tuple(on_gpu(ks, vs)))
+    closer(out.cpu(), q, k8, v8, ks, vs, table, [1] * len(ctx), ctx, False)
+
+
+@pytest.mark.gpu
+@both
+@pytest.mark.parametrize("new,ctx,rules", [([70, 3], [3000, 900], {}), ([16], [4000], {}), ([33], [6000], {}), ([8], [9000], {"BESIDE_KEYS": -1}), ([300, 200], [900, 3000], {"WIDE_TILES": 0, "WIDE_WASTE": 9})])
+def test_prompt_closer(codes, new, ctx, rules, monkeypatch):
+    for name, x in rules.items():
+        monkeypatch.setattr(block8, name, x)
+    nq, nkv, bs = 4, 1, 16
+    table, k8, v8, ks, vs = cache_of(codes, nkv, bs, ctx, 3)
+    T = sum(new)
+    q = torch.randn((T, nq, D), generator=torch.Generator().manual_seed(12)).bfloat16()
+    cu = torch.tensor([sum(new[:i]) for i in range(len(new) + 1)], dtype=torch.int32)
+    out = torch.empty((T, nq, D), dtype=torch.bfloat16, device="cuda")
+    dev = on_gpu(q, k8, v8, table, cu, torch.tensor(ctx, dtype=torch.int32))
+    ops.prefill_attention(*dev, SCALE, out, work=ops.prefill_plan(new, ctx, nq, nkv), kv_scales=tuple(on_gpu(ks, vs)))
+    closer(out.cpu(), q, k8, v8, ks, vs, table, new, ctx, True)
