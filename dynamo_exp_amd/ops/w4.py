@@ -99,7 +99,10 @@ def _shape(m: int, n: int, k: int) -> tuple[int, int, int]:
     """(waves of a workgroup, 16-row tiles of weights a wave, workgroups that K is split over).  Tiles share x's way from L2, but need
     workgroups enough for 256 CUs; us with 1, 2 and 4 tiles, groups of 128, one row: 4096 x 4096 (256 tiles of rows) 4.4, 5.0, -;
     6144 x 4096 6.3, 5.2, 7.2; 28672 x 4096 13.9, 13.3, 12.4; 16 rows: 8192 x 8192 (512) -, 11.9, 13.2; 11008 x 4096 (688) -, 11.5, 9.7.
-    More than 8 rows of a long K take two tiles and halve K: 16 rows of 4096 x 14336 18.2 -> 12.9 (8 rows 10.9, 10.8).  Few rows of weights
+    More than 8 rows of a long K take two tiles, and halve K while a CU has one workgroup at most: 16 rows, one tile, two, two and halves, of
+    4096 x 6144 9.1, 10.0, 8.8, x 8192 10.9, 11.9, 10.2, x 14336 16.9, 18.6, 13.4, of 4352 x 8192 18.1, 11.9, 14.3, x 14336 29.5, 18.7, 20.7, of
+    5600 x 11008 23.7, 15.3, 17.7; 9 rows of 4096 x 8192 8.3, 9.4, 8.8, x 14336 12.7, 14.6, 11.3; 8 of 4096 x 14336 10.9, -, 10.8; 48 of 1024 x 11008
+    13.2, 14.4, 11.8, of 1536 x 11008 23.2, 14.5, 16.8.  Few rows of weights
     split K until there are 256 workgroups or a wave has its one chunk: 17 x 16000 26 -> 4.6, 1000 x 8192 11 -> 5.3.  More than 16 rows are
     bands of 16, which add to the workgroups, or (0 tiles) w4_wide_kernel's, which splits K up to 16 times: 64 rows of 28672 x 4096 (224 workgroups)
     31 in one part, 42 in two."""
@@ -110,7 +113,7 @@ def _shape(m: int, n: int, k: int) -> tuple[int, int, int]:
     rt = 4 if work >= (640 if m > 8 else 1024) else 2 if work >= 384 else 1
     splits = 1
     if work < 384 and m > 8 and k >= 8192:
-        rt = splits = 2
+        rt, splits = 2, 2 if work <= 256 else 1
     groups = -(-tiles // rt) * bands
     if groups < 128:
         splits = max(splits, min(chunks // 8, 256 // groups))

@@ -273,3 +273,21 @@ def test_infinite_and_huge_rows(m, n, k, group, zeros):
     want = x.double() @ w.T
     assert bool((want[0].isinf() | want[0].isnan()).all()) and (m == 1 or bool(want[2:4].isfinite().all()))
     infinite(ops.w4_linear(x.cuda(), weight).cpu(), want, x, w)
+
+
+def test_a_long_k_is_halved_where_cus_are_free():
+    """More than 8 rows of a long K: two tiles a wave, and halves of K only while these are a workgroup a CU at most (256)."""
+    from dynamo_exp_amd.ops import w4
+    for m, n, k in ((9, 4096, 8192), (16, 4097, 8192), (16, 4352, 14336), (16, 6128, 20480), (32, 2048, 11008), (32, 2304, 11008), (48, 1365, 8192), (48, 1536, 8192), (64, 1040, 14336)):
+        bands = -(-m // 16)
+        waves, rt, splits = w4._shape(m, n, k)
+        assert rt == 2 and splits == (2 if -(-n // 16) * bands <= 256 else 1)
+        assert waves == 8 and (splits == 1 or -(-n // 32) * bands * splits <= 256)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(9, 4352, 8192), (16, 4104, 11008), (32, 2304, 8192), (48, 1536, 8320)])
+def test_long_rows_of_more_tiles_than_cus(m, n, k):
+    codes, scales, z, w = make(n, k, 64, True, seed=n)
+    x = torch.randn((m, k), generator=torch.Generator().manual_seed(k)).bfloat16()
+    near(ops.w4_linear(x.cuda(), ops.w4_pack(codes.cuda(), scales.cuda(), z.cuda(), 64)).cpu(), x, w, scales, 64)
