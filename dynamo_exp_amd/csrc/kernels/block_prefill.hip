@@ -17,7 +17,8 @@
 // (2^-100 at least: what lies further apart is taken for that, and weights under 2^-26 of it are lost to the row sum).
 //
 // 8000 tokens of 64 / 8 heads, e4m3: 925 us, 1133 TFLOP/s (matrix cores busy half of the cycles, vector issue two thirds, the clock at 1.9
-// GHz); two of up to 5000, 32 / 8 heads, int8: 372 to 389; six chunks behind up to 900 tokens, e4m3: 41; 16 tokens behind 20000: 22 with the join.
+// GHz); two of up to 5000, 32 / 8 heads, int8: 372 to 389; six chunks behind up to 900 tokens, e4m3: 40 to 42; 16 tokens behind 20000: 22 with the join.
+// One to four tokens behind 20000 (block_rows_kernel) 15, eight 19, with the join.
 //
 // Few rows behind many keys are split over the keys (the plan says where), each part leaves its sums in fp32, and a second kernel
 // joins them.

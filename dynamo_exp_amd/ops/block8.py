@@ -3,7 +3,9 @@
 codes [num_blocks, Hkv, BS, 128] int8 or float8_e4m3fn, scales [num_blocks, Hkv] float32, value = code * scale, for K and V each.
 The engine ops of the package take such a cache where their ``kv_scales`` are tensors [num_blocks, Hkv]: ``rope_cache`` and ``kv_write`` append to it,
 ``decode_attention`` and ``prefill_attention`` read it, ``kv_dequant_scratch`` hands its blocks back as bf16.  GPU tensors run
-csrc/kernels/block_cache.hip, block_decode.hip and block_prefill.hip, CPU tensors the PyTorch forms of :mod:`.reference`.
+csrc/kernels/block_cache.hip, block_decode.hip and block_prefill.hip, CPU tensors the PyTorch forms of :mod:`.reference`.  (These take
+other widths and types too; the kernels' rows are bf16, their heads 128 wide, decode has at most 16 query heads a key/value head, and
+prompt attention no negative scale: other calls are refused.)
 
 Scales are made by the append, as powers of two, so that nothing has to be calibrated: a block's grows when a token needs it,
 and the block's codes move with it (see :func:`append`).  A cache needs no clearing: a block's first token (offset 0) starts its
@@ -244,8 +246,9 @@ def decode(q, k_cache, v_cache, block_tables, ctx_lens, scale, out, n_parts, wor
 
 CUS = 256
 # Tokens that eight waves take whole where a CU has one workgroup at most.  us on the GPU, whole and in the best number of parts with their
-# join: 30 sequences of 700 tokens, 8 key/value heads 11.5 and 14.6, 30 of 300 7.6 and 11.0, one of 400 7.2 and 7.0, one of 700 8.9 and
-# 7.3; a second launch costs the host 4 us more where launches are not captured.
+# join: 30 sequences of 700 tokens, 8 key/value heads 11.5 and 14.6, 30 of 300 7.6 and 11.0, 16 of 700 10.4 and 10.7, but one of 400 7.2 and 6.7,
+# one of 700 8.7 and 7.1, eight 9.7 and 8.8.  These too are left whole: an eager call's host takes 4 us to start the join.  A caller that captures
+# few short contexts names the number of parts.
 WHOLE = 768
 
 

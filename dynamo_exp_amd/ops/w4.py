@@ -146,7 +146,7 @@ def _check_weight(weight: W4Weight) -> int:
 
 
 def w4_linear(x: torch.Tensor, weight: W4Weight, out: torch.Tensor | None = None) -> torch.Tensor:
-    """y [m, n] = x [m, k] . w^T for up to 256 rows of bf16, sums in fp32."""
+    """y [m, n] = x [m, k] . w^T for up to 256 rows of bf16, sums in fp32.  (CPU tensors: any number of rows of any type.)"""
     shape, (p, s, z, n, k, group) = x.shape, weight
     if len(shape) != 2 or shape[1] != k:
         raise ValueError(f"w4_linear: x {tuple(shape)}, weight {(n, k)}")
